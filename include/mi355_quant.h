@@ -43,6 +43,8 @@ typedef enum mi355_status {
 #define MI355_DTYPE_FP16 1
 #define MI355_DTYPE_FP32 2   /* accepted where a function's comment says so */
 #define MI355_DTYPE_INT32 3  /* likewise */
+#define MI355_DTYPE_INT8 4   /* likewise */
+#define MI355_DTYPE_INT64 5  /* likewise */
 
 /* Output formats of mi355_quant_matmul. */
 #define MI355_OUT_BF16 0
@@ -414,6 +416,85 @@ int mi355_probe_clock(unsigned long long *out, int workgroups, int iters, void *
 
 /* Measurement aid: a kernel that does nothing, `workgroups` x 256 threads (the per-launch floor inside a captured graph). */
 int mi355_probe_empty_launch(int workgroups, void *stream);
+
+/* ---- paged key-value cache ----
+ *
+ * Not in the reference's tree; named and laid out like the operators above.  A cache holds the keys and values of one
+ * layer in blocks ("pages") of block_size tokens that sequences own in any order.  Slot s is token s % block_size of
+ * block s / block_size; a block table lists a sequence's blocks in the order of its positions.
+ */
+typedef struct mi355_paged_cache {
+    void *key, *value;                    /* [num_blocks, block_size, kv_heads, head_dim] of dtype, the last dimension contiguous */
+    float *key_scale, *value_scale;       /* [num_blocks, block_size, kv_heads] for int8 (element = code * scale), else NULL */
+    int dtype;                            /* MI355_DTYPE_BF16, MI355_DTYPE_FP16 or MI355_DTYPE_INT8 */
+    int64_t num_blocks, block_size, kv_heads, head_dim;   /* num_blocks * block_size < 2^31 */
+    int64_t key_stride[3], value_stride[3];               /* elements between blocks, tokens and heads */
+    int64_t key_scale_stride[3], value_scale_stride[3];
+} mi355_paged_cache;
+
+/*
+ * Writes the keys and values of new tokens into their slots.
+ *   key, value  [tokens, kv_heads, head_dim] of dtype (bf16 / fp16; the cache's own type unless that is int8), the last
+ *               dimension contiguous; *_stride[0], *_stride[1]: elements between tokens and between heads
+ *   slots       [tokens] int32 or int64 (slots_dtype), distinct; a token whose slot lies outside the cache is skipped
+ * An int8 cache gets, per token and head, scale = max_d |x_d| / 127 and code_d = rint_half_even(x_d / scale), the rule of
+ * mi355_dynamic_quant, and the scale.
+ */
+int mi355_paged_cache_write(const mi355_paged_cache *cache, const void *key, const int64_t *key_stride, const void *value,
+                            const int64_t *value_stride, int dtype, const void *slots, int slots_dtype, int64_t tokens, void *stream);
+
+/*
+ * Copies the tokens of `slots` out of the cache, in their order: key, value [tokens, kv_heads, head_dim] of dtype (the
+ * cache's own type; from int8 bf16 or fp16, round(code * scale)).  A slot outside the cache gives zeros.
+ */
+int mi355_paged_cache_read(const mi355_paged_cache *cache, void *key, const int64_t *key_stride, void *value,
+                           const int64_t *value_stride, int dtype, const void *slots, int slots_dtype, int64_t tokens, void *stream);
+
+/*
+ * Attention of one new token per sequence over the sequence's cached tokens.  With the positions j of sequence b that are
+ * seen (j < context_lens[b], not hidden by `mask`, in a block that the table names), and the key/value head of query
+ * head h being h / (heads / kv_heads):
+ *   s_j = scale * sum_d q[b,h,d] key[j,d]       lse = log sum_j exp(s_j)
+ *   out[b,h,:] = sum_j exp(s_j - lse) value[j,:]
+ *   attn_sums[b, kv head, j] += sum over the kv head's query heads of exp(s_j - lse)
+ * Scores, sums and outputs are accumulated in float32.  Where nothing is seen out is 0 and lse -infinity.  Values and keys
+ * that are not seen have no influence, NaN included.
+ *   q             [batch, heads, head_dim] of q_dtype (the cache's own type; bf16 or fp16 with int8), strides in elements
+ *   out           [batch, heads, head_dim] of q_dtype, contiguous; lse float32 [batch, heads] or NULL
+ *   block_table   int32 [batch, max_blocks], rows table_stride elements apart; entries outside [0, num_blocks) name no block
+ *   context_lens  int32 [batch], clamped to [0, max_blocks * block_size]
+ *   mask          NULL, or bytes [batch, max_blocks * block_size], rows mask_stride apart; nonzero hides a position
+ *   attn_sums     NULL, or float32 [batch, kv_heads, max_blocks * block_size], positions contiguous, updated where seen
+ *   workspace     mi355_paged_decode_attention_workspace() bytes, 16-byte aligned, whatever it holds; used until the
+ *                 launches of this call are done
+ */
+size_t mi355_paged_decode_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_blocks,
+                                              int64_t block_size, int with_sums);
+int mi355_paged_decode_attention(const mi355_paged_cache *cache, const void *q, int q_dtype, int64_t q_stride_batch, int64_t q_stride_head,
+                                 void *out, float *lse, int64_t batch, int64_t heads, const int32_t *block_table, int64_t table_stride,
+                                 int64_t max_blocks, const int32_t *context_lens, float scale, const uint8_t *mask, int64_t mask_stride,
+                                 float *attn_sums, int64_t sums_stride_batch, int64_t sums_stride_head, void *workspace,
+                                 size_t workspace_bytes, void *stream);
+
+/*
+ * Eviction: every sequence that is longer than `keep` is brought down to `keep` tokens, each key/value head choosing its
+ * own.  A head keeps the tokens whose position exceeds the largest one minus `recent`, then those with the largest sums
+ * (NaN counts as the lowest), the lower place first among equals.  Kept tokens that lie at or behind place `keep` move into
+ * the places of evicted ones before it, in ascending order on both sides; nothing else moves.  With n = context_lens[b]
+ * (clamped to [0, max_blocks * block_size]):
+ *   sums, positions          float32 / int32 [batch, kv_heads, max_blocks * block_size]: per place the summed attention
+ *                            weight and the token's position in its sequence; strides in elements, places contiguous
+ *   new_lens                 int32 [batch]: min(n, keep)
+ *   new_sums, new_positions  contiguous, the same shape: moved like the tokens; 0 and -1 from place new_lens on
+ * Cache rows (and int8 scales) are moved in place.  A row whose old or new block the table does not name is not moved.
+ * Sequences must not share blocks.  workspace: mi355_paged_cache_evict_workspace() bytes, 16-byte aligned.
+ */
+size_t mi355_paged_cache_evict_workspace(int64_t batch, int64_t kv_heads, int64_t max_blocks, int64_t block_size, int64_t keep);
+int mi355_paged_cache_evict(const mi355_paged_cache *cache, const int32_t *block_table, int64_t table_stride, int64_t max_blocks,
+                            const int32_t *context_lens, int64_t batch, const float *sums, int64_t sums_stride_batch,
+                            int64_t sums_stride_head, const int32_t *positions, int64_t positions_stride_batch,
+                            int64_t positions_stride_head, int64_t keep, int64_t recent, int32_t *new_lens, float *new_sums,
+                            int32_t *new_positions, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Peak engine clock (kHz) and compute-unit count of the current device from the HIP runtime; either pointer may be NULL. */
 int mi355_device_info(int *clock_khz, int *compute_units);

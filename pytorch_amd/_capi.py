@@ -20,7 +20,9 @@ EXPORTS = ("mi355_status_string", "mi355_quant_abi_version", "mi355_dynamic_quan
            "mi355_anti_quant", "mi355_unpack_int4", "mi355_dynamic_quant_asymmetric", "mi355_quantize",
            "mi355_trans_quant_param", "mi355_quant_matmul_qparam", "mi355_swiglu_quant_smooth", "mi355_set_tuning",
            "mi355_quant_matmul_noalloc", "mi355_stream_capture_id", "mi355_probe_clock", "mi355_device_info", "mi355_transpose_int8", "mi355_probe_empty_launch",
-           "mi355_workspace_status", "mi355_workspace_zero_bytes")
+           "mi355_workspace_status", "mi355_workspace_zero_bytes",
+           "mi355_paged_cache_write", "mi355_paged_cache_read", "mi355_paged_decode_attention_workspace", "mi355_paged_decode_attention",
+           "mi355_paged_cache_evict_workspace", "mi355_paged_cache_evict")
 
 _lib = None
 

@@ -20,6 +20,7 @@
 #include <array>
 #include <string>
 #include <tuple>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -72,6 +73,19 @@ struct Arg<int64_t> {
     }
     bool load_default(const c10::IValue &d) { return d.isInt() ? (v = d.toInt(), true) : false; }
     int64_t get() const { return v; }
+};
+template <>
+struct Arg<std::optional<double>> {
+    std::optional<double> v;
+    bool load(PyObject *o)
+    {
+        if (o == Py_None) return true;
+        if (!PyFloat_CheckExact(o)) return false;
+        v = PyFloat_AS_DOUBLE(o);
+        return true;
+    }
+    bool load_default(const c10::IValue &d) { return d.isNone(); }
+    std::optional<double> get() const { return v; }
 };
 template <>
 struct Arg<bool> {
@@ -209,12 +223,18 @@ struct Op<R(A...)> {
         std::tuple<Arg<A>...> v;
         constexpr auto each = std::index_sequence_for<A...>{};
         if (!fits || !load(v, slot, each)) return fall_back(self, args, kwargs);
-        std::optional<R> r;
-        {
+        if constexpr (std::is_void_v<R>) {
             NoGil no_gil;
-            r.emplace(invoke(v, each));
+            invoke(v, each);
+        } else {
+            std::optional<R> r;
+            {
+                NoGil no_gil;
+                r.emplace(invoke(v, each));
+            }
+            return to_python(std::move(*r));
         }
-        return to_python(std::move(*r));
+        Py_RETURN_NONE;
         END_HANDLE_TH_ERRORS
     }
 };
@@ -270,6 +290,12 @@ using SwigluQuant = std::tuple<Tensor, Tensor>(const Tensor &, const OptTensor &
                                                OptType);
 using AntiQuant = Tensor(const Tensor &, const Tensor &, const OptTensor &, OptType, OptType);
 using TransParam = Tensor(const Tensor &, const OptTensor &);
+using PagedWrite = void(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const OptTensor &, const OptTensor &);
+using PagedRead = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const OptTensor &, const OptTensor &, OptType);
+using PagedAttention = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const OptTensor &,
+                                                  const OptTensor &, std::optional<double>, const OptTensor &, const OptTensor &, bool);
+using PagedEvict = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                                      int64_t, int64_t, const OptTensor &, const OptTensor &);
 using Quantize = Tensor(const Tensor &, const Tensor &, const OptTensor &, at::ScalarType, int64_t, bool);
 
 // ---- forward passes of the contrib modules.  A module stores [out_features, in_features] weights and [N, G] parameters and the
@@ -353,7 +379,11 @@ PyObject *install(PyObject *, PyObject *args)
                     install_one<struct T5, SwigluQuant>(namespace_, "npu_swiglu_quant") &&
                     install_one<struct T6, AntiQuant>(namespace_, "npu_anti_quant") &&
                     install_one<struct T7, TransParam>(namespace_, "npu_trans_quant_param") &&
-                    install_one<struct T8, Quantize>(namespace_, "npu_quantize");
+                    install_one<struct T8, Quantize>(namespace_, "npu_quantize") &&
+                    install_one<struct T9, PagedWrite>(namespace_, "npu_paged_cache_write") &&
+                    install_one<struct T10, PagedRead>(namespace_, "npu_paged_cache_read") &&
+                    install_one<struct T11, PagedAttention>(namespace_, "npu_paged_decode_attention") &&
+                    install_one<struct T12, PagedEvict>(namespace_, "npu_paged_cache_evict");
     if (!ok) return nullptr;
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
