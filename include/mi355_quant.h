@@ -465,8 +465,8 @@ int mi355_paged_cache_read(const mi355_paged_cache *cache, void *key, const int6
  *   context_lens  int32 [batch], clamped to [0, max_blocks * block_size]
  *   mask          NULL, or bytes [batch, max_blocks * block_size], rows mask_stride apart; nonzero hides a position
  *   attn_sums     NULL, or float32 [batch, kv_heads, max_blocks * block_size], positions contiguous, updated where seen
- *   workspace     mi355_paged_decode_attention_workspace() bytes, 16-byte aligned, whatever it holds; used until the
- *                 launches of this call are done
+ *   workspace     mi355_paged_decode_attention_workspace() bytes, 16-byte aligned, its first MI355_WORKSPACE_ZERO_BYTES zero
+ *                 and left zero, as for mi355_quant_matmul
  */
 size_t mi355_paged_decode_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_blocks,
                                               int64_t block_size, int with_sums);

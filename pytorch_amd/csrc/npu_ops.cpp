@@ -941,6 +941,8 @@ Tensor quantize_hip(const Tensor &x, const Tensor &scales, const optional<Tensor
 
 } // namespace
 
+at::Tensor mi355_ops::workspace(const at::Tensor &like, size_t bytes, bool large_for_call) { return zeroed_workspace(like, bytes, large_for_call); }
+
 TORCH_LIBRARY_FRAGMENT(npu, m)
 {
     m.def("npu_dynamic_quant(Tensor input, *, Tensor? smooth_scales=None, Tensor? group_index=None, "

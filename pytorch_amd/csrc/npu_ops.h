@@ -8,6 +8,11 @@
 
 #include "mi355_quant.h"
 
+namespace mi355_ops {
+// the stream's workspace, its zero area (MI355_WORKSPACE_ZERO_BYTES) zero (npu_ops.cpp)
+at::Tensor workspace(const at::Tensor &like, size_t bytes, bool large_for_call = false);
+} // namespace mi355_ops
+
 namespace {
 
 using at::Tensor;

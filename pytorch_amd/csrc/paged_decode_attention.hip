@@ -20,18 +20,21 @@
 // values multiplies its probability, in float32.
 //
 // Work is dealt out on the device, because the lengths are known only there: the positions of every (sequence, head) pair
-// are cut into units of 128, all units are numbered, and every workgroup takes the same number of consecutive ones.  A pair
-// that lies within one workgroup is finished there; of a pair that is cut, every workgroup leaves (sums, m, l) in the
-// workspace and the join kernel adds them in order.
+// are cut into halves of a tile, 16 positions of one block (fewer at a block's end), eight halves make a unit, all units are
+// numbered, and every workgroup takes the same number of consecutive ones.  A pair that lies within one workgroup is
+// finished there; of a pair that is cut, every workgroup leaves (sums, m, l) in the workspace, and the last one to arrive adds
+// them in their order.
 #include "paged_cache.h"
 #include "weight_quant_common.h"
 
 namespace mi355 {
 namespace {
 
-constexpr int kUnit = 128;                   // positions per unit: 32 for each wavefront of a workgroup
+constexpr int kHalf = 16;                    // positions of half a tile: rows of one MFMA operand
+constexpr int kUnit = 8;                     // halves per unit: a tile of two for each wavefront of a workgroup
 constexpr int kHeads = 16;                   // query heads of one tile
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+constexpr int kSC1 = 16;                     // cache-policy bit: agent scope, past the caches of one XCD
 
 struct AttnArgs {
     PagedCache cache;
@@ -43,80 +46,119 @@ struct AttnArgs {
     int64_t table_stride;
     const uint8_t *mask;
     int64_t mask_stride;
+    uint32_t *arrived;                       // [workgroups] zero before and after
     float *part;                             // [workgroups][2][rows][DP]
     float *part_ml;                          // [workgroups][2][kHeads][2]: maximum, sum
     float *scores;                           // [batch * heads][score_pitch] z_j, or null
     float *lse2;                             // [batch * heads] m + log2 l, with scores
     float *sums;
     int64_t score_pitch, sums_batch, sums_head;
+    FastDiv by_pairs, by_workgroups;
+    FastDiv span, halves;                    // positions that are cut into halves together (a block, or 16), and their halves
     int batch, heads, group, rows, tiles, pairs, workgroups;    // pairs = key/value heads * tiles, of one sequence
-    int capacity;                            // max_blocks * block_size
+    int capacity, max_blocks;                // capacity = max_blocks * block_size
+    uint32_t part_bytes;
     float scale2;                            // scale * log2(e)
-    int vec;                                 // rows are read in 16-byte (int8: up to 16-byte) pieces
 };
 
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform64(int64_t v)
+// The kernel's arguments where the launch put them, in constant memory.  A kernel of several phases would otherwise load every
+// field that a later phase needs at the start, and spill a hundred scalar registers; behind args_now() they are read again.
+// What such a pointer leads to has to be named global memory (at()), since the compiler no longer sees where it came from.
+typedef const __attribute__((address_space(4))) AttnArgs *Args;
+__device__ __forceinline__ Args args_now()
 {
-    return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
+    auto p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
 }
+// The thread's number, out of the compiler's sight for the same reason: what is derived from it is derived where it is used
+// and not kept in vector registers through the phases before.
+__device__ __forceinline__ int thread_now()
+{
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+template <class T>
+using Global = __attribute__((address_space(1))) T;
+template <class T>
+__device__ __forceinline__ Global<T> *at(T *p) { return (Global<T> *)p; }
+__device__ __forceinline__ uint32_t divide(uint32_t n, const __attribute__((address_space(4))) FastDiv &f)
+{
+    return (uint32_t)(((uint64_t)n * f.mul) >> f.shift);
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) { return (int64_t)(((uint64_t)uniform((uint32_t)(v >> 32)) << 32) | uniform((uint32_t)v)); }
+// read-only words through the scalar cache
+__device__ __forceinline__ int scalar_load(const int32_t *p) { return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p; }
 
 // What sums over a maximum `m` count for under the maximum `top`.  Nothing seen yet: m = -infinity, sums 0 - or NaN, from NaN
 // scores, which the product with 0 keeps.
 __device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top); }
 
-__device__ __forceinline__ int length_of(const AttnArgs &a, int b) { return min(max(a.lens[b], 0), a.capacity); }
-__device__ __forceinline__ uint32_t units_of(int len) { return ((uint32_t)len + kUnit - 1) / kUnit; }
+__device__ __forceinline__ int clamp_len(Args a, int len) { return min(max(len, 0), a->capacity); }
+__device__ __forceinline__ uint32_t halves_of(Args a, int len)
+{
+    const uint32_t whole = divide((uint32_t)len, a->span);
+    return whole * a->halves.d + ((uint32_t)len - whole * a->span.d + kHalf - 1) / kHalf;
+}
+__device__ __forceinline__ uint32_t units_of(Args a, int len) { return (halves_of(a, len) + kUnit - 1) / kUnit; }
 
-// The numbering of units: sequence by sequence, in it pair by pair.  `before(b)`: units of one pair in the sequences before
-// b; total: in all.  Thread t of 256 counts a run of consecutive sequences.
+// The numbering of units: sequence by sequence, in it pair by pair.  Every wavefront counts for itself, lane i a run of
+// consecutive sequences; no barrier, no LDS.
 struct Numbering {
-    uint32_t run_before, run_sum, total;
-    int run, first;                          // sequences per thread, the thread's first
+    uint32_t before, sum, total;             // units of one pair: in the runs before this lane's, in it, in all
+    int run, len;                            // sequences per lane; the length of the first
 
-    __device__ Numbering(const AttnArgs &a, uint32_t *lds /* 4 */)
+    __device__ explicit Numbering(Args a)
     {
-        run = (a.batch + 255) / 256;
-        first = threadIdx.x * run;
-        run_sum = 0;
-        for (int i = 0; i < run && first + i < a.batch; i++) run_sum += units_of(length_of(a, first + i));
-        uint32_t scan = run_sum;
-        const int lane = threadIdx.x & 63;
+        const int lane = threadIdx.x & 63, batch = a->batch;
+        run = (batch + 63) / 64;
+        sum = 0;
+        len = lane * run < batch ? clamp_len(a, at(a->lens)[lane * run]) : 0;
+        sum = units_of(a, len);
+        for (int i = lane * run + 1; i < min((lane + 1) * run, batch); i++) sum += units_of(a, clamp_len(a, at(a->lens)[i]));
+        uint32_t scan = sum;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const uint32_t o = (uint32_t)__shfl_up((int)scan, off, 64);
             if (lane >= off) scan += o;
         }
-        if (lane == 63) lds[threadIdx.x >> 6] = scan;
-        __syncthreads();
-        run_before = scan - run_sum;
-        total = 0;
-        for (int w = 0; w < 4; w++) {
-            if (w < (int)(threadIdx.x >> 6)) run_before += lds[w];
-            total += lds[w];
+        before = scan - sum;
+        total = (uint32_t)__builtin_amdgcn_readlane((int)scan, 63);
+    }
+    // the sequence that holds unit y of one pair, how many units come before it, and its own
+    __device__ void find(Args a, uint32_t y, int &b, uint32_t &units_before, uint32_t &units) const
+    {
+        const int lane = __builtin_ctzll(__ballot(y >= before && y - before < sum));
+        b = lane * run;
+        units_before = (uint32_t)__builtin_amdgcn_readlane((int)before, lane);
+        units = units_of(a, __builtin_amdgcn_readlane(len, lane));
+        while (y - units_before >= units) {
+            units_before += units;
+            units = units_of(a, clamp_len(a, scalar_load(a->lens + ++b)));
         }
-        total = (uint32_t)uniform((int)total);
     }
 };
 
-__device__ __forceinline__ int64_t share_of(const AttnArgs &a, int64_t all) { return (all + a.workgroups - 1) / a.workgroups; }
-
-// Eight (four) 16-bit values or bytes from any address: what the vector loads do for aligned rows.
+// BYTES of a row from any address, of which `valid` belong to the row; the rest is zero and not read.
 template <int BYTES>
-__device__ __forceinline__ void load_piece(uint32_t *to, const char *from, bool vec, int valid_bytes)
+__device__ __forceinline__ void load_piece(uint32_t *to, const Global<char> *from, int valid)
 {
-    if (valid_bytes >= BYTES && vec) {
-        __builtin_memcpy(to, __builtin_assume_aligned(from, BYTES), BYTES);
+    if (valid >= BYTES) {
+        typedef uint32_t piece __attribute__((ext_vector_type(BYTES / 4)));
+        typedef piece anywhere __attribute__((aligned(1)));
+        const piece v = *(const Global<anywhere> *)from;
+        __builtin_memcpy(to, &v, BYTES);
         return;
     }
+    uint64_t low = 0, high = 0;
+#pragma unroll 1
+    for (int i = 0; i < valid; i++) (i < 8 ? low : high) |= (uint64_t)(uint8_t)from[i] << (8 * (i & 7));
 #pragma unroll
-    for (int w = 0; w < BYTES / 4; w++) {
-        uint32_t v = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (w * 4 + i < valid_bytes) v |= (uint32_t)(uint8_t)from[w * 4 + i] << (8 * i);
-        to[w] = v;
-    }
+    for (int w = 0; w < BYTES / 4; w++) to[w] = (uint32_t)((w < 2 ? low : high) >> (32 * (w & 1)));
 }
 
 template <int W>
@@ -133,316 +175,520 @@ __device__ __forceinline__ void buffer_load(uint32_t (&to)[W], __amdgpu_buffer_r
     }
 }
 
-// DP: head_dim rounded up to 64, 128 or 256.  QT: type of q and out (0 bf16, 1 fp16).  UNI: the 16 positions of a half tile
-// lie in one block at a small stride, so that addresses are one scalar descriptor per half and per-lane constants.
-template <int DP, bool QUANT, int QT, bool UNI>
-struct Tile {
+// How the rows of half a tile are addressed.
+//   kRows   lane by lane: any block size, stride, width and alignment
+//   kBlock  the half lies in one block: a scalar descriptor that ends with the half's last row, constant lane offsets; rows in
+//           16-byte pieces.  Rows behind the end read as zero without traffic, so the loop needs no edge code.
+//   kBlockScales  the same, and (int8) the scales of four tokens of a head are 16 aligned bytes
+//   kBlockMask  as kBlock, with a mask, whose bytes are read four at a time
+enum Addressing { kRows, kBlock, kBlockScales, kBlockMask };
+
+// DP: head_dim rounded up to 64, 128 or 256.  QT: type of q and out (0 bf16, 1 fp16).
+template <int DP, bool QUANT, int QT, Addressing AD>
+struct Decode {
     static constexpr int ES = QUANT ? 1 : 2;
     static constexpr int NCH = DP / 32;                          // chunks of 32 d, one MFMA each
     static constexpr int KL = QUANT ? NCH / 2 : NCH;             // 16-byte loads of a key row per lane
     static constexpr int PE = DP >= 128 ? 8 : 4;                 // consecutive d of a value row per lane and piece
     static constexpr int NP = DP / (16 * PE);
     static constexpr int VW = PE * ES / 4;                       // registers of a piece
+    static constexpr int PT = QUANT ? 0 : QT;                    // type of the probabilities and of the values' images
+    // fp16 probabilities are 2^14 times as large, so that ones down to 2^-38 of the largest keep their place
+    static constexpr float kShift = PT == 1 ? 14.0f : 0.0f;
 
-    uint32_t k[2][KL][4];
-    uint32_t v[2][4][NP][VW];
+    // where the two halves of a tile are
+    struct Place {
+        int n[2], key[2], id[2];                                 // positions seen from the half's first one on, that one, its block
+        uint32_t off[2];                                         // and its token within the block
+    };
+
+    const Args a;
+    const int wave, col, g, D;
+    uint32_t koff[KL], voff[4][NP], soff[2][4];                  // lane offsets of key pieces, value pieces, scales
+    uint32_t k[2][KL][4], v[2][4][NP][VW], hidden[2];
     float ks[2][4], vs[2][4];
-    int valid_rows[2];                                           // UNI
-    uint32_t valid;                                              // bit 4 s + r: position s * 16 + lane group * 4 + r is seen
+    uint32_t lane_slot[2], v_slot[2];                            // kRows: slot of position 16 s + col of the tile, or ~0
+    u32x4 q[NCH];
+    f32x4 acc[NP][PE];
+    float m, l;
+
+    // of the pair that is being worked on
+    int b, kvh, len, half_end;
+    const int32_t *table;
+    const char *kbase, *vbase;
+
+    __device__ explicit Decode(Args args)
+        : Decode(args, thread_now())
+    {
+    }
+    __device__ __forceinline__ Decode(Args args, int thread) : a(args), wave(uniform(thread >> 6)), col(thread & 15), g((thread & 63) >> 4), D(args->cache.dim)
+    {
+        if constexpr (AD != kRows) {
+#pragma unroll
+            for (int c = 0; c < KL; c++) {
+                const int d = first_d(c);
+                koff[c] = d < D ? (uint32_t)col * (uint32_t)a->cache.key.token + d * ES : kOutOfRange;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+                for (int h = 0; h < NP; h++) {
+                    const int d = h * 128 + col * PE;
+                    voff[j][h] = d < D ? (uint32_t)(g * 4 + j) * (uint32_t)a->cache.value.token + d * ES : kOutOfRange;
+                }
+                if constexpr (QUANT) {
+                    soff[0][j] = (uint32_t)(g * 4 + j) * (uint32_t)a->cache.key_scale.token;
+                    soff[1][j] = (uint32_t)(g * 4 + j) * (uint32_t)a->cache.value_scale.token;
+                }
+            }
+        }
+    }
+
+    using ArgArray = const __attribute__((address_space(4))) PagedArray;
+    __device__ __forceinline__ int64_t offset(ArgArray &x, uint32_t slot) const
+    {
+        const uint32_t block = divide(slot, a->cache.page);
+        return block * x.block + (int64_t)(slot - block * a->cache.page.d) * x.token + kvh * x.head;
+    }
+    // first d of the lane's key piece c; an int8 piece serves the chunks 2c and 2c + 1
+    __device__ __forceinline__ int first_d(int c) const { return QUANT ? c * 64 + g * 16 : c * 32 + g * 8; }
+
+    __device__ __forceinline__ void start(int b_, int kvh_, int head0, int rows, int len_, int half_end_)
+    {
+        b = b_, kvh = kvh_, len = len_, half_end = half_end_;
+        table = a->table + b * a->table_stride;
+        kbase = a->cache.key.base + kvh * a->cache.key.head;
+        vbase = a->cache.value.base + kvh * a->cache.value.head;
+        const uint16_t *row = a->q + b * a->q_batch + (head0 + min(col, rows - 1)) * a->q_head;
+#pragma unroll
+        for (int c = 0; c < NCH; c++) {
+            const int d = QUANT ? first_d(c / 2) + (c % 2) * 8 : first_d(c);
+            uint32_t w[4];
+            load_piece<16>(w, (const Global<char> *)(row + d), col < rows ? 2 * (D - d) : 0);
+            q[c] = u32x4{w[0], w[1], w[2], w[3]};
+        }
+        m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int h = 0; h < NP; h++)
+#pragma unroll
+            for (int i = 0; i < PE; i++) acc[h][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    __device__ __forceinline__ Place place(int tile) const
+    {
+        Place p;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const uint32_t half = uniform((uint32_t)tile * 2 + s);
+            const uint32_t span = divide(half, a->halves);
+            p.off[s] = (half - span * a->halves.d) * kHalf;
+            p.key[s] = (int)(span * a->span.d + p.off[s]);
+            const int n = min(min(kHalf, (int)(a->span.d - p.off[s])), len - p.key[s]);
+            p.n[s] = uniform((int)half < half_end ? max(n, 0) : 0);
+            p.id[s] = AD != kRows ? scalar_load(table + min(span, (uint32_t)a->max_blocks - 1)) : 0;
+        }
+        return p;
+    }
+    // a block that the table does not name holds nothing
+    __device__ __forceinline__ void settle(Place &p) const
+    {
+        if constexpr (AD != kRows) {
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+                if ((uint32_t)p.id[s] >= (uint32_t)a->cache.num_blocks) p.n[s] = 0, p.id[s] = 0;
+        }
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char *base, ArgArray &x, const Place &p, int s, int row_bytes) const
+    {
+        const uint64_t block = (uint64_t)(uint32_t)p.id[s] * (uint32_t)x.block, first = (uint64_t)base + block + p.off[s] * (uint32_t)x.token;
+        const uint32_t bytes = p.n[s] > 0 ? (uint32_t)(p.n[s] - 1) * (uint32_t)x.token + row_bytes : 0;
+        return make_rsrc((const char *)uniform((int64_t)first), uniform(bytes));
+    }
+    // positions of the tile, their keys, key scales and mask bytes
+    __device__ __forceinline__ void load_keys(const Place &p)
+    {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            if constexpr (AD != kRows) {
+                const __amdgpu_buffer_rsrc_t r = rows_of(kbase, a->cache.key, p, s, D * ES);
+#pragma unroll
+                for (int c = 0; c < KL; c++) buffer_load<4>(k[s][c], r, koff[c]);
+                if constexpr (QUANT) load_scales(ks[s], a->cache.key_scale, p, s, soff[0]);
+            } else {
+                const int key = p.key[s] + col;
+                const uint32_t block = divide((uint32_t)key, a->cache.page);
+                const int id = col < p.n[s] ? at(table)[block] : -1;
+                bool there = (uint32_t)id < (uint32_t)a->cache.num_blocks;
+                if (a->mask && there) there = at(a->mask)[b * a->mask_stride + key] == 0;
+                lane_slot[s] = there ? (uint32_t)id * a->cache.page.d + ((uint32_t)key - block * a->cache.page.d) : ~0u;
+                const Global<char> *row = at(a->cache.key.base) + (there ? offset(a->cache.key, lane_slot[s]) : 0);
+#pragma unroll
+                for (int c = 0; c < KL; c++) load_piece<16>(k[s][c], row + first_d(c) * ES, there ? (D - first_d(c)) * ES : 0);
+                if constexpr (QUANT) {
+                    const float mine = there ? *(const Global<float> *)(at(a->cache.key_scale.base) + offset(a->cache.key_scale, lane_slot[s])) : 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) ks[s][r] = __shfl(mine, g * 4 + r, 64);
+                }
+            }
+            if constexpr (AD == kBlockMask) {                    // (the host: blocks of a multiple of 4 tokens)
+                const uint64_t first = (uint64_t)a->mask + (uint64_t)(b * a->mask_stride) + (uint32_t)p.key[s];
+                const __amdgpu_buffer_rsrc_t r = make_rsrc((const void *)uniform((int64_t)first), (uint32_t)(p.n[s] + 3) & ~3u);
+                hidden[s] = __builtin_amdgcn_raw_buffer_load_b32(r, g * 4, 0, 0);
+            }
+        }
+    }
+    __device__ __forceinline__ void load_scales(float (&to)[4], ArgArray &x, const Place &p, int s, const uint32_t (&off)[4]) const
+    {
+        const __amdgpu_buffer_rsrc_t r = rows_of(x.base + kvh * x.head, x, p, s, 4);
+        if constexpr (AD == kBlockScales) {
+            const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(r, g * 16, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) to[i] = __uint_as_float(w[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) to[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off[i], 0, 0));
+        }
+    }
+    __device__ __forceinline__ void load_values(const Place &p)
+    {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            if constexpr (AD != kRows) {
+                const __amdgpu_buffer_rsrc_t r = rows_of(vbase, a->cache.value, p, s, D * ES);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int h = 0; h < NP; h++) buffer_load<VW>(v[s][j][h], r, voff[j][h]);
+                if constexpr (QUANT) load_scales(vs[s], a->cache.value_scale, p, s, soff[1]);
+            } else {
+                const int64_t mine = lane_slot[s] == ~0u ? -1 : offset(a->cache.value, lane_slot[s]);
+                if constexpr (QUANT) {
+                    const float scale = mine >= 0 ? *(const Global<float> *)(at(a->cache.value_scale.base) + offset(a->cache.value_scale, lane_slot[s])) : 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) vs[s][r] = __shfl(scale, g * 4 + r, 64);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int64_t from = __shfl(mine, g * 4 + j, 64);
+                    const Global<char> *row = at(a->cache.value.base) + (from < 0 ? 0 : from);
+#pragma unroll
+                    for (int h = 0; h < NP; h++) {
+                        const int d = h * 128 + col * PE;
+                        load_piece<VW * 4>(v[s][j][h], row + d * ES, from < 0 ? 0 : (D - d) * ES);
+                    }
+                }
+            }
+        }
+    }
+    // bit 4 s + r: position 16 s + 4 g + r of the tile is seen
+    __device__ __forceinline__ uint32_t seen(const Place &p) const
+    {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            uint32_t four;
+            if constexpr (AD != kRows) {
+                four = (1u << min(max(p.n[s] - g * 4, 0), 4)) - 1;
+                if constexpr (AD == kBlockMask) {
+                    // a mask byte that is not 0 leaves bit 7 of its sum with 0x7f set, or has it itself
+                    const uint32_t set = (((hidden[s] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | hidden[s]) & 0x80808080u;
+                    four &= ~((set * 0x00204081u) >> 28);
+                }
+            } else {
+                four = 0;
+#pragma unroll
+                for (int r = 0; r < 4; r++) four |= (uint32_t)(__shfl((int)lane_slot[s], g * 4 + r, 64) != -1) << r;
+            }
+            bits |= four << (4 * s);
+        }
+        return bits;
+    }
+
+    // z_j of the tile's positions
+    __device__ __forceinline__ void score(const Place &p, uint32_t valid, f32x4 (&z)[2]) const
+    {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            z[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NCH; c++) {
+                u32x4 image;
+                if constexpr (QUANT) {
+                    const u32x2 lo = sbytes_act4<QT>(k[s][c / 2][(c % 2) * 2]), hi = sbytes_act4<QT>(k[s][c / 2][(c % 2) * 2 + 1]);
+                    image = u32x4{lo.x, lo.y, hi.x, hi.y};
+                } else {
+                    image = u32x4{k[s][c][0], k[s][c][1], k[s][c][2], k[s][c][3]};
+                }
+                z[s] = mfma_act<QT>(image, q[c], z[s]);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                z[s][r] = QUANT ? z[s][r] * (a->scale2 * ks[s][r]) : z[s][r] * a->scale2;
+                if (!full(p)) z[s][r] = (valid >> (4 * s + r)) & 1 ? z[s][r] : -INFINITY;
+            }
+    }
+    // every position of the tile is seen, known without a look at the lanes
+    __device__ __forceinline__ bool full(const Place &p) const { return (AD == kBlock || AD == kBlockScales) && p.n[0] + p.n[1] == 2 * kHalf; }
+    __device__ __forceinline__ void store_scores(const Place &p, const f32x4 (&z)[2], int head0, int rows) const
+    {
+        if (col >= rows) return;
+        Global<float> *to = at(a->scores) + ((int64_t)b * a->heads + head0 + col) * a->score_pitch + g * 4;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int n = AD != kRows ? min(kHalf, (int)(a->span.d - p.off[s])) : kHalf;        // a block's places, seen or not
+            const int left = (p.key[s] < len ? min(n, len - p.key[s]) : 0) - g * 4;
+            if (left <= 0) continue;
+            if (a->span.d % 4 == 0) {
+                *(Global<f32x4> *)(to + p.key[s]) = z[s];
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (r < left) to[p.key[s] + r] = z[s][r];
+            }
+        }
+    }
+    // probabilities under the running maximum, and what they weigh
+    __device__ __forceinline__ void add(const Place &place, uint32_t valid, const f32x4 (&z)[2], u32x4 &ph, u32x4 &pl)
+    {
+        float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])), fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (__any(top > m)) {
+            const float higher = fmaxf(m, top), f = weight_of(m, higher);
+            m = higher;
+            l *= f;
+#pragma unroll
+            for (int h = 0; h < NP; h++)
+#pragma unroll
+                for (int i = 0; i < PE; i++) acc[h][i] *= f;
+        }
+        const float base = m == -INFINITY ? 0.0f : m - kShift;
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            p[i] = __builtin_amdgcn_exp2f(z[i / 4][i % 4] - base);
+            l += p[i];
+        }
+        if constexpr (QUANT) {
+            // probabilities times value scales in two bf16 terms: 16 significant bits of any magnitude
+            float hi[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                p[i] = p[i] * vs[i / 4][i % 4];
+                if (!full(place)) p[i] = (valid >> i) & 1 ? p[i] : 0.0f;
+                hi[i] = bf16_1(f32_to_bf16(p[i]));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                ph[i] = pack_bf16x2(hi[2 * i], hi[2 * i + 1]);
+                pl[i] = pack_bf16x2(p[2 * i] - hi[2 * i], p[2 * i + 1] - hi[2 * i + 1]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) ph[i] = pack_act2<PT>(p[2 * i], p[2 * i + 1]);
+        }
+    }
+    __device__ __forceinline__ void weigh(const Place &place, uint32_t valid, const u32x4 &ph, const u32x4 &pl)
+    {
+        if constexpr (!QUANT) {
+            // a value that is not seen must not turn 0 * NaN into NaN (codes are always finite)
+            if (!full(place)) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const uint32_t keep = (valid >> i) & 1 ? ~0u : 0u;
+#pragma unroll
+                    for (int h = 0; h < NP; h++)
+#pragma unroll
+                        for (int w = 0; w < VW; w++) v[i / 4][i % 4][h][w] &= keep;
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < NP; h++)
+#pragma unroll
+            for (int i = 0; i < PE; i++) {
+                u32x4 image;
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const int s = w / 2, j = (w % 2) * 2;
+                    if constexpr (QUANT)
+                        image[w] = pack_bf16x2(sbyte_f32(v[s][j][h][i / 4], i % 4), sbyte_f32(v[s][j + 1][h][i / 4], i % 4));
+                    else
+                        image[w] = __builtin_amdgcn_perm(v[s][j + 1][h][i / 2], v[s][j][h][i / 2], i % 2 ? 0x07060302u : 0x05040100u);
+                }
+                acc[h][i] = mfma_act<PT>(image, ph, acc[h][i]);
+                if constexpr (QUANT) acc[h][i] = mfma_act<PT>(image, pl, acc[h][i]);
+            }
+    }
+
+    // The wavefront's tiles of this stretch.  The next tile's keys are requested as soon as this one's scores are out of the
+    // registers, its values as soon as this one's are, so about a tile is always on the way.
+    __device__ __forceinline__ void run(int tile, int tile_end, int head0, int rows)
+    {
+        Place cur = place(tile);
+        settle(cur);
+        load_keys(cur);
+        __builtin_amdgcn_sched_barrier(0);
+        load_values(cur);
+        __builtin_amdgcn_sched_barrier(0);
+        Place next = place(tile + 4);
+        for (; tile < tile_end; tile += 4) {
+            const uint32_t valid = seen(cur);
+            f32x4 z[2];
+            score(cur, valid, z);
+            if (a->scores) store_scores(cur, z, head0, rows);
+            settle(next);
+            if constexpr (AD != kRows) load_keys(next);
+            __builtin_amdgcn_sched_barrier(0);                   // requests stay in this order, so that a wait for one leaves the later ones out
+            u32x4 ph, pl;
+            add(cur, valid, z, ph, pl);
+            weigh(cur, valid, ph, pl);
+            if constexpr (AD == kRows) load_keys(next);          // the slots of this tile's values are no longer needed
+            load_values(next);
+            __builtin_amdgcn_sched_barrier(0);
+            cur = next;
+            next = place(tile + 8);
+        }
+    }
 };
 
-template <int DP, bool QUANT, int QT, bool UNI>
-__global__ __launch_bounds__(256) void paged_decode_kernel(AttnArgs a)
+template <int QT>
+__device__ __forceinline__ void store_out(Args a, int64_t row, int d, f32x4 v)
 {
-    using T = Tile<DP, QUANT, QT, UNI>;
-    constexpr int PT = QUANT ? 0 : QT;                           // type of the probabilities and value images
-    // fp16 probabilities are 2^14 times as large, so that ones down to 2^-38 of the largest keep their place
-    constexpr float kShift = PT == 1 ? 14.0f : 0.0f;
+    const int D = a->cache.dim;
+    Global<uint16_t> *o = at(a->out) + row * D + d;
+    const u32x2 w = {pack_act2<QT>(v[0], v[1]), pack_act2<QT>(v[2], v[3])};
+    if (d + 4 <= D) {
+        typedef u32x2 anywhere __attribute__((aligned(2)));
+        *(Global<anywhere> *)o = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+            if (d + i < D) o[i] = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
+    }
+}
+__device__ __forceinline__ void store_lse(Args a, int64_t row, float m, float l, float shift)
+{
+    const float lse2 = l == 0.0f ? -INFINITY : m + (__builtin_amdgcn_logf(l) - shift);
+    if (a->lse) at(a->lse)[row] = lse2 * kLn2;
+    if (a->lse2) at(a->lse2)[row] = lse2;
+}
+
+// Adds the partial sums that workgroups w0 .. w1 left for one pair, in their order, and finishes the pair.  Every thread
+// takes quads of consecutive d; two halves of the workgroup take the even and the odd partials when there are few quads.
+template <int DP, int QT>
+__device__ void join(Args a, int b, int head0, int rows, int w0, int w1, bool first_at_0, float shift, float (*lds)[4])
+{
+    constexpr int QPR = DP / 4;
+    const __amdgpu_buffer_rsrc_t part = make_rsrc(a->part, a->part_bytes);
+    const __amdgpu_buffer_rsrc_t mls = make_rsrc(a->part_ml, (uint32_t)a->workgroups * 2 * kHeads * 2 * 4);
+    const int thread = thread_now();
+    for (int e0 = 0; e0 < rows * QPR; e0 += 128) {
+        const int e = e0 + (thread & 127), row = min(e / QPR, rows - 1), d = (e % QPR) * 4, odd = thread >> 7;
+        float m = -INFINITY, l = 0.0f;
+        f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int w = w0 + odd; w <= w1; w += 16) {
+            f32x4 v[8];
+            u32x2 ml[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {                        // eight in flight; past the end they read zeros
+                const int wi = w + 2 * i;
+                const uint32_t at = (uint32_t)wi * 2 + (wi > w0 || first_at_0 ? 0 : 1);
+                const uint32_t po = (at * (uint32_t)a->rows + row) * (DP * 4) + d * 4, mo = (at * kHeads + row) * 8;
+                v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, wi <= w1 ? po : kOutOfRange, 0, kSC1));
+                ml[i] = __builtin_amdgcn_raw_buffer_load_b64(mls, wi <= w1 ? mo : kOutOfRange, 0, kSC1);
+            }
+            float top = m;
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = w + 2 * i <= w1 ? fmaxf(top, __uint_as_float(ml[i].x)) : top;
+            const float f = weight_of(m, top);
+            m = top;
+            l *= f;
+            sum *= f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (w + 2 * i > w1) break;
+                const float fi = weight_of(__uint_as_float(ml[i].x), top);
+                l += __uint_as_float(ml[i].y) * fi;
+                sum += v[i] * fi;
+            }
+        }
+        __syncthreads();
+        if (odd) {
+            const int t = thread & 127;
+            lds[2 * t][0] = m, lds[2 * t][1] = l;
+            *reinterpret_cast<f32x4 *>(lds[2 * t + 1]) = sum;
+        }
+        __syncthreads();
+        if (odd || e >= rows * QPR) continue;
+        const int t = thread;
+        const float top = fmaxf(m, lds[2 * t][0]), f0 = weight_of(m, top), f1 = weight_of(lds[2 * t][0], top);
+        l = l * f0 + lds[2 * t][1] * f1;
+        sum = sum * f0 + *reinterpret_cast<const f32x4 *>(lds[2 * t + 1]) * f1;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        store_out<QT>(a, (int64_t)b * a->heads + head0 + row, d, sum * inv);
+        if (d == 0) store_lse(a, (int64_t)b * a->heads + head0 + row, top, l, shift);
+    }
+}
+
+template <int DP, bool QUANT, int QT, Addressing AD>
+__global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void paged_decode_kernel(AttnArgs)
+{
+    using W = Decode<DP, QUANT, QT, AD>;
     constexpr int RP = 128 + 4;                                  // row pitch of the sums in LDS, 4 words past a bank cycle
     __shared__ float red[4][kHeads][RP];
     __shared__ float ml[4][kHeads][2];
-    __shared__ int where[4];
-    __shared__ uint32_t scan[4];
+    __shared__ int last_here;
 
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int D = a.cache.dim;
-    int64_t x, x_end;
-    int b, pair, unit, units;
+    uint32_t x, x_begin, x_end, share;                           // all units are fewer than 2^31 - workgroups: the host checks
+    int b = 0, pair = 0, unit = 0;
     {
-        const Numbering n(a, scan);
-        const int64_t all = (int64_t)n.total * a.pairs, share = share_of(a, all);
-        x = (int64_t)blockIdx.x * share;
+        const Args a = args_now();
+        const Numbering n(a);
+        const uint32_t all = n.total * (uint32_t)a->pairs;
+        share = divide(all + a->workgroups - 1, a->by_workgroups);
+        x = x_begin = min(blockIdx.x * share, all);
         x_end = min(x + share, all);
-        if (x >= all) return;
-        const uint32_t y = (uint32_t)((uint64_t)x / (uint32_t)a.pairs);
-        if (y >= n.run_before && y - n.run_before < n.run_sum) {           // one thread
-            uint32_t before = n.run_before;
-            int i = n.first;
-            for (;; i++) {
-                const uint32_t u = units_of(length_of(a, i));
-                if (y - before < u) break;
-                before += u;
-            }
-            const uint32_t u = units_of(length_of(a, i));
-            const uint64_t in = (uint64_t)x - (uint64_t)before * (uint32_t)a.pairs;
-            where[0] = i;
-            where[1] = (int)(in / u);
-            where[2] = (int)(in % u);
+        if (x < x_end) {
+            uint32_t before, units;
+            n.find(a, divide(x, a->by_pairs), b, before, units);
+            const uint32_t in = x - before * (uint32_t)a->pairs;
+            pair = (int)(in / units);
+            unit = (int)(in - pair * units);
         }
-        __syncthreads();
-        b = uniform(where[0]), pair = uniform(where[1]), unit = uniform(where[2]);
-    }
-    int slot = 0;
-    const int64_t kstep = a.cache.key.token, vstep = a.cache.value.token;
-    uint32_t koff[T::KL], voff[4][T::NP];
-    if constexpr (UNI) {
-#pragma unroll
-        for (int c = 0; c < T::KL; c++) {
-            const int d = QUANT ? c * 64 + g * 16 : c * 32 + g * 8;
-            koff[c] = d < D ? (uint32_t)(col * kstep) + d * T::ES : kOutOfRange;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int h = 0; h < T::NP; h++) {
-                const int d = h * 128 + col * T::PE;
-                voff[j][h] = d < D ? (uint32_t)((g * 4 + j) * vstep) + d * T::ES : kOutOfRange;
-            }
     }
 
     while (x < x_end) {
-        int len = uniform(length_of(a, b));
-        units = (int)units_of(len);
-        while (units == 0) {                                     // the sequence is over: the next one that has positions
-            b++;
-            len = uniform(length_of(a, b));
-            units = (int)units_of(len);
-        }
-        const int last = (int)min((int64_t)units, unit + (x_end - x));     // units [unit, last) of this pair
-        const int kvh = pair / a.tiles, head0 = kvh * a.group + (pair % a.tiles) * kHeads;
-        const int rows = min(kHeads, (kvh + 1) * a.group - head0);
-        const int end = min(len, last * kUnit);
-
-        u32x4 q[T::NCH];
+        int head0, rows, units, last;
+        float l, m;
+        f32x4 acc[W::NP][W::PE];
         {
-            const uint16_t *row = a.q + b * a.q_batch + (head0 + min(col, rows - 1)) * a.q_head;
+            W w(args_now());
+            b = uniform(b), pair = uniform(pair), unit = uniform(unit);
+            int len = clamp_len(w.a, scalar_load(w.a->lens + b));
+            while (len == 0) len = clamp_len(w.a, scalar_load(w.a->lens + ++b));     // the next sequence that has positions
+            const int halves = (int)halves_of(w.a, len);
+            units = (halves + kUnit - 1) / kUnit;
+            last = min(units, unit + (int)(x_end - x));      // units [unit, last) of this pair
+            const int kvh = pair / w.a->tiles;
+            head0 = kvh * w.a->group + (pair % w.a->tiles) * kHeads;
+            rows = min(kHeads, (kvh + 1) * w.a->group - head0);
+            last = uniform(last);
+            w.start(b, kvh, head0, rows, len, min(halves, last * kUnit));
+            w.run(unit * (kUnit / 2) + w.wave, last * (kUnit / 2), head0, rows);
+            l = w.l, m = w.m;
 #pragma unroll
-            for (int c = 0; c < T::NCH; c++) {
-                const int d = QUANT ? (c / 2) * 64 + g * 16 + (c % 2) * 8 : c * 32 + g * 8;
-                uint32_t w[4];
-                load_piece<16>(w, reinterpret_cast<const char *>(row + d), a.vec, col < rows ? 2 * (D - d) : 0);
-                q[c] = u32x4{w[0], w[1], w[2], w[3]};
-            }
-        }
-        float m = -INFINITY, l = 0.0f;
-        f32x4 acc[T::NP][T::PE] = {};
-
-        const int32_t *table = a.table + b * a.table_stride;
-        const int64_t khead = kvh * a.cache.key.head, vhead = kvh * a.cache.value.head;
-
-        T t;
-        uint32_t lane_slot[2];                                   // !UNI: slot of position s * 16 + col, or ~0
-        // where the tile's rows are
-        const auto place = [&](int tile, int64_t (&kb)[2], int64_t (&vb)[2], int64_t (&sb)[2]) {
-            (void)sb;
+            for (int h = 0; h < W::NP; h++)
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
-                const int key0 = tile * 32 + s * 16;
-                if constexpr (UNI) {
-                    int n = min(max(end - key0, 0), 16);
-                    const uint32_t block = div_by((uint32_t)key0, a.cache.page);
-                    const uint32_t off = (uint32_t)key0 - block * a.cache.page.d;
-                    int id = n > 0 ? table[block] : 0;
-                    if ((uint32_t)id >= (uint32_t)a.cache.num_blocks) n = 0, id = 0;
-                    t.valid_rows[s] = uniform(n);
-                    kb[s] = uniform64(id * a.cache.key.block + off * kstep + khead);
-                    vb[s] = uniform64(id * a.cache.value.block + off * vstep + vhead);
-                    lane_slot[s] = (uint32_t)uniform((int)((uint32_t)id * a.cache.page.d + off));
-                } else {
-                    const int key = key0 + col;
-                    const uint32_t block = div_by((uint32_t)key, a.cache.page);
-                    const int id = key < end ? table[block] : -1;
-                    lane_slot[s] = (uint32_t)id < (uint32_t)a.cache.num_blocks ? (uint32_t)id * a.cache.page.d + ((uint32_t)key - block * a.cache.page.d) : ~0u;
-                }
-            }
-        };
-        const auto load_k = [&](const int64_t (&kb)[2]) {
-#pragma unroll
-            for (int s = 0; s < 2; s++) {
-                if constexpr (UNI) {
-                    const int n = t.valid_rows[s];
-                    const __amdgpu_buffer_rsrc_t r = make_rsrc(a.cache.key.base + kb[s], n > 0 ? (uint32_t)((n - 1) * kstep) + D * T::ES : 0);
-#pragma unroll
-                    for (int c = 0; c < T::KL; c++) buffer_load<4>(t.k[s][c], r, koff[c]);
-                } else {
-                    const uint32_t sl = lane_slot[s];
-                    const char *row = a.cache.key.base + (sl == ~0u ? 0 : a.cache.offset(a.cache.key, sl, kvh));
-#pragma unroll
-                    for (int c = 0; c < T::KL; c++) {
-                        const int d = QUANT ? c * 64 + g * 16 : c * 32 + g * 8;
-                        load_piece<16>(t.k[s][c], row + d * T::ES, a.vec, sl == ~0u ? 0 : (D - d) * T::ES);
-                    }
-                }
-            }
-        };
-        const auto load_v = [&](const int64_t (&vb)[2]) {
-#pragma unroll
-            for (int s = 0; s < 2; s++) {
-                if constexpr (UNI) {
-                    const int n = t.valid_rows[s];
-                    const __amdgpu_buffer_rsrc_t r = make_rsrc(a.cache.value.base + vb[s], n > 0 ? (uint32_t)((n - 1) * vstep) + D * T::ES : 0);
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-#pragma unroll
-                        for (int h = 0; h < T::NP; h++) buffer_load<T::VW>(t.v[s][j][h], r, voff[j][h]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t sl = (uint32_t)__shfl((int)lane_slot[s], g * 4 + j, 64);
-                        const char *row = a.cache.value.base + (sl == ~0u ? 0 : a.cache.offset(a.cache.value, sl, kvh));
-#pragma unroll
-                        for (int h = 0; h < T::NP; h++) {
-                            const int d = h * 128 + col * T::PE;
-                            load_piece<T::VW * 4>(t.v[s][j][h], row + d * T::ES, a.vec, sl == ~0u ? 0 : (D - d) * T::ES);
-                        }
-                    }
-                }
-            }
-        };
-        // which positions are seen, and their scales
-        const auto load_seen = [&](int tile) {
-            t.valid = 0;
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int i = g * 4 + r, key = tile * 32 + s * 16 + i;
-                    bool seen;
-                    uint32_t sl;
-                    if constexpr (UNI) {
-                        seen = i < t.valid_rows[s];
-                        sl = lane_slot[s] + i;
-                    } else {
-                        sl = (uint32_t)__shfl((int)lane_slot[s], i, 64);
-                        seen = sl != ~0u;
-                    }
-                    if constexpr (QUANT) {
-                        t.ks[s][r] = seen ? *reinterpret_cast<const float *>(a.cache.key_scale.base + a.cache.offset(a.cache.key_scale, sl, kvh)) : 0.0f;
-                        t.vs[s][r] = seen ? *reinterpret_cast<const float *>(a.cache.value_scale.base + a.cache.offset(a.cache.value_scale, sl, kvh)) : 0.0f;
-                    }
-                    if (a.mask && seen) seen = a.mask[b * a.mask_stride + key] == 0;
-                    t.valid |= (uint32_t)seen << (4 * s + r);
-                }
-        };
-
-        const int t_end = (end + 31) / 32;
-        for (int tile = unit * 4 + wave; tile < t_end; tile += 4) {
-            int64_t kb[2], vb[2], sb[2];
-            place(tile, kb, vb, sb);
-            load_k(kb);
-            load_v(vb);
-            load_seen(tile);
-            f32x4 z[2] = {};
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int c = 0; c < T::NCH; c++) {
-                    u32x4 image;
-                    if constexpr (QUANT) {
-                        const u32x2 lo = sbytes_act4<QT>(t.k[s][c / 2][(c % 2) * 2]), hi = sbytes_act4<QT>(t.k[s][c / 2][(c % 2) * 2 + 1]);
-                        image = u32x4{lo.x, lo.y, hi.x, hi.y};
-                    } else {
-                        image = u32x4{t.k[s][c][0], t.k[s][c][1], t.k[s][c][2], t.k[s][c][3]};
-                    }
-                    z[s] = mfma_act<QT>(image, q[c], z[s]);
-                }
-            float top = -INFINITY;
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    z[s][r] = QUANT ? z[s][r] * (a.scale2 * t.ks[s][r]) : z[s][r] * a.scale2;
-                    if (!((t.valid >> (4 * s + r)) & 1)) z[s][r] = -INFINITY;
-                    top = fmaxf(top, z[s][r]);
-                }
-            if (a.scores && col < rows) {
-                float *to = a.scores + ((int64_t)b * a.heads + head0 + col) * a.score_pitch + tile * 32 + g * 4;
-#pragma unroll
-                for (int s = 0; s < 2; s++)
-                    if (tile * 32 + s * 16 + g * 4 < end) *reinterpret_cast<f32x4 *>(to + s * 16) = z[s];
-            }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (__any(top > m)) {
-                const float higher = fmaxf(m, top);
-                const float f = weight_of(m, higher);
-                m = higher;
-                l *= f;
-#pragma unroll
-                for (int h = 0; h < T::NP; h++)
-#pragma unroll
-                    for (int i = 0; i < T::PE; i++) acc[h][i] *= f;
-            }
-            const float base = m == -INFINITY ? 0.0f : m - kShift;
-            float p[8];
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    p[4 * s + r] = __builtin_amdgcn_exp2f(z[s][r] - base);
-                    l += p[4 * s + r];
-                }
-            // a value that is not seen must not turn 0 * NaN into NaN
-            if (!__all(t.valid == 0xffu)) {
-#pragma unroll
-                for (int s = 0; s < 2; s++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t keep = (t.valid >> (4 * s + j)) & 1 ? ~0u : 0u;
-#pragma unroll
-                        for (int h = 0; h < T::NP; h++)
-#pragma unroll
-                            for (int w = 0; w < T::VW; w++) t.v[s][j][h][w] &= keep;
-                        if constexpr (QUANT) t.vs[s][j] = keep ? t.vs[s][j] : 0.0f;
-                    }
-            }
-            u32x4 ph, pl;
-            if constexpr (QUANT) {
-                // probabilities times value scales in two bf16 terms: 16 significant bits of any magnitude
-                float hi[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    p[i] *= t.vs[i / 4][i % 4];
-                    hi[i] = bf16_1(f32_to_bf16(p[i]));
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    ph[i] = pack_bf16x2(hi[2 * i], hi[2 * i + 1]);
-                    pl[i] = pack_bf16x2(p[2 * i] - hi[2 * i], p[2 * i + 1] - hi[2 * i + 1]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) ph[i] = pack_act2<PT>(p[2 * i], p[2 * i + 1]);
-            }
-#pragma unroll
-            for (int h = 0; h < T::NP; h++)
-#pragma unroll
-                for (int i = 0; i < T::PE; i++) {
-                    u32x4 image;
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const int s = w / 2, j = (w % 2) * 2;
-                        if constexpr (QUANT)
-                            image[w] = pack_bf16x2(sbyte_f32(t.v[s][j][h][i / 4], i % 4), sbyte_f32(t.v[s][j + 1][h][i / 4], i % 4));
-                        else
-                            image[w] = __builtin_amdgcn_perm(t.v[s][j + 1][h][i / 2], t.v[s][j][h][i / 2], i % 2 ? 0x07060302u : 0x05040100u);
-                    }
-                    acc[h][i] = mfma_act<PT>(image, ph, acc[h][i]);
-                    if constexpr (QUANT) acc[h][i] = mfma_act<PT>(image, pl, acc[h][i]);
-                }
+                for (int i = 0; i < W::PE; i++) acc[h][i] = w.acc[h][i];
         }
 
         // the four wavefronts' sums on a common maximum
+        const Args a = args_now();
+        const int thread = thread_now(), lane = thread & 63, wave = thread >> 6, col = lane & 15, g = lane >> 4;
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (g == 0) ml[wave][col][0] = m, ml[wave][col][1] = l;
@@ -450,111 +696,77 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(AttnArgs a)
         const float top = fmaxf(fmaxf(ml[0][col][0], ml[1][col][0]), fmaxf(ml[2][col][0], ml[3][col][0]));
         const float f = weight_of(m, top);
         const bool whole = unit == 0 && last == units;
-        const int64_t part_at = ((int64_t)blockIdx.x * 2 + slot) * a.rows;
+        const int slot = x == x_begin ? 0 : 1;
+        const uint32_t part_at = (blockIdx.x * 2 + slot) * (uint32_t)a->rows;
 #pragma unroll
-        for (int h = 0; h < T::NP; h++) {
+        for (int h = 0; h < W::NP; h++) {
             if (h) __syncthreads();
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int i = 0; i < T::PE; i += 4)
-                    *reinterpret_cast<f32x4 *>(&red[wave][col][(g * 4 + r) * T::PE + i]) =
+                for (int i = 0; i < W::PE; i += 4)
+                    *reinterpret_cast<f32x4 *>(&red[wave][col][(g * 4 + r) * W::PE + i]) =
                         f32x4{acc[h][i][r] * f, acc[h][i + 1][r] * f, acc[h][i + 2][r] * f, acc[h][i + 3][r] * f};
             __syncthreads();
-            constexpr int QPR = 16 * T::PE / 4;                  // quads of a row
-            for (int e = threadIdx.x; e < rows * QPR; e += 256) {
+            constexpr int QPR = 16 * W::PE / 4;                  // quads of a row
+            for (int e = thread; e < rows * QPR; e += 256) {
                 const int row = e / QPR, d = (e % QPR) * 4;
                 f32x4 sum = *reinterpret_cast<const f32x4 *>(&red[0][row][d]);
 #pragma unroll
-                for (int w = 1; w < 4; w++) sum += *reinterpret_cast<const f32x4 *>(&red[w][row][d]);
+                for (int i = 1; i < 4; i++) sum += *reinterpret_cast<const f32x4 *>(&red[i][row][d]);
                 if (whole) {
                     const float rt = fmaxf(fmaxf(ml[0][row][0], ml[1][row][0]), fmaxf(ml[2][row][0], ml[3][row][0]));
                     float total = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < 4; w++) total += ml[w][row][1] * weight_of(ml[w][row][0], rt);
+                    for (int i = 0; i < 4; i++) total += ml[i][row][1] * weight_of(ml[i][row][0], rt);
                     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-                    uint16_t *o = a.out + ((int64_t)b * a.heads + head0 + row) * D + h * 128 + d;
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (h * 128 + d + i < D) o[i] = (uint16_t)pack_act2<QT>(sum[i] * inv, 0.0f);
+                    store_out<QT>(a, (int64_t)b * a->heads + head0 + row, h * 128 + d, sum * inv);
                 } else {
-                    *reinterpret_cast<f32x4 *>(a.part + (part_at + row) * DP + h * 128 + d) = sum;
+                    const __amdgpu_buffer_rsrc_t part = make_rsrc(a->part, a->part_bytes);
+                    buffer_store_b128<kSC1>(__builtin_bit_cast(u32x4, sum), part, ((part_at + row) * DP + h * 128 + d) * 4, 0);
                 }
             }
         }
         if (wave == 0 && g == 0 && col < rows) {
             float total = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) total += ml[w][col][1] * weight_of(ml[w][col][0], top);
+            for (int i = 0; i < 4; i++) total += ml[i][col][1] * weight_of(ml[i][col][0], top);
             if (whole) {
-                const float lse2 = total == 0.0f ? -INFINITY : top + (__builtin_amdgcn_logf(total) - kShift);
-                const int64_t at = (int64_t)b * a.heads + head0 + col;
-                if (a.lse) a.lse[at] = lse2 * kLn2;
-                if (a.lse2) a.lse2[at] = lse2;
+                store_lse(a, (int64_t)b * a->heads + head0 + col, top, total, W::kShift);
             } else {
-                float *to = a.part_ml + (((int64_t)blockIdx.x * 2 + slot) * kHeads + col) * 2;
-                to[0] = top;
-                to[1] = total;
+                const __amdgpu_buffer_rsrc_t mls = make_rsrc(a->part_ml, (uint32_t)a->workgroups * 2 * kHeads * 2 * 4);
+                const u32x2 two = {__float_as_uint(top), __float_as_uint(total)};
+                __builtin_amdgcn_raw_buffer_store_b64(two, mls, ((blockIdx.x * 2 + slot) * kHeads + col) * 8, 0, kSC1);
             }
+        }
+        if (!whole) {
+            // the last of the pair's workgroups to arrive adds everybody's sums; the first one's counter counts them
+            const uint32_t x0 = x - unit;
+            const int w0 = (int)(x0 / share), w1 = (int)((x0 + units - 1) / share);
+            wait_vmcnt<0>();                                     // this wavefront's sums have reached the coherence point
+            __syncthreads();
+            if (thread == 0) {
+                const uint32_t old = __hip_atomic_fetch_add(at(a->arrived) + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                last_here = old == (uint32_t)(w1 - w0);
+                if (last_here) __hip_atomic_store(at(a->arrived) + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);     // for the next launch
+            }
+            __syncthreads();
+            if (last_here)
+                join<DP, QT>(args_now(), b, head0, rows, w0, w1, w0 * share == x0, W::kShift, reinterpret_cast<float (*)[4]>(&red[0][0][0]));
         }
         __syncthreads();                                         // ml and red are free again
-        slot = 1;
         x += last - unit;
         unit = 0;
-        if (last == units && ++pair == a.pairs) pair = 0, b++;
+        if (last == units && ++pair == a->pairs) pair = 0, b++;
     }
-}
 
-// One workgroup per (sequence, pair): nothing to do for a pair that one workgroup finished; zeros where there are no
-// positions; else the partial sums of the workgroups that met in it, in their order.
-template <int DP, int QT>
-__global__ __launch_bounds__(256) void paged_decode_join_kernel(AttnArgs a, float shift)
-{
-    __shared__ uint32_t scan[4];
-    __shared__ uint32_t mine;
-    const int b = blockIdx.x / a.pairs, pair = blockIdx.x % a.pairs;
-    const Numbering n(a, scan);
-    if (b >= n.first && b < n.first + n.run) {
-        uint32_t before = n.run_before;
-        for (int i = n.first; i < b; i++) before += units_of(length_of(a, i));
-        mine = before;
-    }
-    __syncthreads();
-    const int units = (int)units_of(length_of(a, b));
-    const int kvh = pair / a.tiles, head0 = kvh * a.group + (pair % a.tiles) * kHeads;
-    const int rows = min(kHeads, (kvh + 1) * a.group - head0);
-    const int64_t all = (int64_t)n.total * a.pairs, share = max(share_of(a, all), (int64_t)1);
-    const int64_t x0 = (int64_t)mine * a.pairs + (int64_t)pair * units;
-    const int w0 = (int)(x0 / share), w1 = units ? (int)((x0 + units - 1) / share) : w0;
-    if (units && w0 == w1) return;
-    const int D = a.cache.dim;
-    const auto slot_of = [&](int w) { return w * share >= x0 ? 0 : 1; };
-    for (int e = threadIdx.x; e < rows * (DP / 4); e += 256) {
-        const int row = e / (DP / 4), d = (e % (DP / 4)) * 4;
-        float top = -INFINITY;
-        if (units)
-            for (int w = w0; w <= w1; w++) top = fmaxf(top, a.part_ml[(((int64_t)w * 2 + slot_of(w)) * kHeads + row) * 2]);
-        f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
-        float total = 0.0f;
-        if (units)
-            for (int w = w0; w <= w1; w++) {
-                const int64_t at = (int64_t)w * 2 + slot_of(w);
-                const float mw = a.part_ml[(at * kHeads + row) * 2], lw = a.part_ml[(at * kHeads + row) * 2 + 1];
-                const float f = weight_of(mw, top);
-                total += lw * f;
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(a.part + (at * a.rows + row) * DP + d);
-                sum += v * f;
-            }
-        const int64_t at = (int64_t)b * a.heads + head0 + row;
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (d + i < D) a.out[at * D + d + i] = (uint16_t)pack_act2<QT>(sum[i] * inv, 0.0f);
-        if (d == 0) {
-            const float lse2 = total == 0.0f ? -INFINITY : top + (__builtin_amdgcn_logf(total) - shift);
-            if (a.lse) a.lse[at] = lse2 * kLn2;
-            if (a.lse2) a.lse2[at] = lse2;
-        }
+    // sequences without positions
+    const Args a = args_now();
+    for (int e = blockIdx.x; e < a->batch; e += gridDim.x) {
+        if (clamp_len(a, scalar_load(a->lens + e)) != 0) continue;
+        for (int i = threadIdx.x; i < a->heads * a->cache.dim; i += 256) at(a->out)[(int64_t)e * a->heads * a->cache.dim + i] = 0;
+        for (int i = threadIdx.x; i < a->heads; i += 256)
+            if (a->lse) at(a->lse)[(int64_t)e * a->heads + i] = -INFINITY;
     }
 }
 
@@ -563,7 +775,7 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(AttnArgs a, floa
 __global__ __launch_bounds__(256) void paged_sums_kernel(AttnArgs a)
 {
     const int b = blockIdx.z, kvh = blockIdx.y;
-    const int len = length_of(a, b);
+    const int len = min(max(a.lens[b], 0), a.capacity);
     for (int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; j < len; j += (int64_t)gridDim.x * 1024) {
         f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int h = 0; h < a.group; h++) {
@@ -583,6 +795,7 @@ __global__ __launch_bounds__(256) void paged_sums_kernel(AttnArgs a)
 struct AttnSizes {
     int64_t rows, tiles, pairs, units, workgroups, dp, score_pitch;
     size_t part, part_ml, lse2, scores, bytes;                    // offsets in the workspace, and its size
+    uint32_t part_bytes;
 };
 
 constexpr size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -598,40 +811,45 @@ bool plan_attention(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head
     p->rows = group < kHeads ? group : kHeads;
     p->tiles = (group + kHeads - 1) / kHeads;
     p->pairs = kv_heads * p->tiles;
-    p->units = (capacity + kUnit - 1) / kUnit;
-    if (p->units && batch > 0x7fffffff / p->units) return false;
+    // halves per position at most: one for each block's remainder beside its sixteens
+    const int64_t halves = capacity / kHalf + max_blocks + 1;
+    p->units = (halves + kUnit - 1) / kUnit;
+    if (batch * p->pairs > 0x7ffff000 / p->units) return false;
     p->dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-    const int64_t most = batch * p->units;
-    p->workgroups = 768;
-    if (most < p->workgroups && most * p->pairs < p->workgroups) p->workgroups = most * p->pairs > 0 ? most * p->pairs : 1;
+    p->workgroups = kNumCU * (p->dp == 256 ? 2 : 3);              // as many as the card holds at once
+    if (batch * p->units * p->pairs < p->workgroups) p->workgroups = batch * p->units * p->pairs;
     p->score_pitch = (capacity + 3) / 4 * 4;
-    size_t at = 0;
+    size_t at = MI355_WORKSPACE_ZERO_BYTES;                       // the arrival counters lie at its start
     const auto take = [&](size_t bytes) { const size_t o = at; at += round256(bytes); return o; };
-    p->part = take((size_t)(p->workgroups * 2 * p->rows * p->dp) * 4);
+    p->part_bytes = (uint32_t)(p->workgroups * 2 * p->rows * p->dp * 4);
+    p->part = take(p->part_bytes);
     p->part_ml = take((size_t)(p->workgroups * 2 * kHeads * 2) * 4);
     p->lse2 = take(sums ? (size_t)(batch * heads) * 4 : 0);
     p->scores = take(sums ? (size_t)(batch * heads) * (size_t)p->score_pitch * 4 : 0);
     p->bytes = at;
     return true;
 }
+static_assert(kNumCU * 3 * sizeof(uint32_t) <= kWorkspaceCounterBytes, "arrival counters");
 
 template <int DP, bool QUANT, int QT>
-void launch_attention(const AttnArgs &a, bool uni, hipStream_t s)
+void launch_attention(const AttnArgs &a, Addressing ad, hipStream_t s)
 {
-    if (uni) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, true>), dim3(a.workgroups), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, false>), dim3(a.workgroups), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((paged_decode_join_kernel<DP, QT>), dim3((unsigned)(a.batch * a.pairs)), dim3(256), 0, s, a, QUANT || QT == 0 ? 0.0f : 14.0f);
+    const dim3 grid(a.workgroups), block(256);
+    if (ad == kRows) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kRows>), grid, block, 0, s, a);
+    else if (QUANT && ad == kBlockScales) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, QUANT ? kBlockScales : kBlock>), grid, block, 0, s, a);
+    else if (ad == kBlockMask) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlockMask>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlock>), grid, block, 0, s, a);
 }
 
 template <int DP>
-void launch_attention(const AttnArgs &a, bool quant, bool fp16, bool uni, hipStream_t s)
+void launch_attention(const AttnArgs &a, bool quant, bool fp16, Addressing ad, hipStream_t s)
 {
     if (quant) {
-        if (fp16) launch_attention<DP, true, 1>(a, uni, s);
-        else launch_attention<DP, true, 0>(a, uni, s);
+        if (fp16) launch_attention<DP, true, 1>(a, ad, s);
+        else launch_attention<DP, true, 0>(a, ad, s);
     } else {
-        if (fp16) launch_attention<DP, false, 1>(a, uni, s);
-        else launch_attention<DP, false, 0>(a, uni, s);
+        if (fp16) launch_attention<DP, false, 1>(a, ad, s);
+        else launch_attention<DP, false, 0>(a, ad, s);
     }
 }
 
@@ -679,6 +897,7 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     a.mask = mask;
     a.mask_stride = mask_stride;
     char *ws = static_cast<char *>(workspace);
+    a.arrived = reinterpret_cast<uint32_t *>(ws);
     a.part = reinterpret_cast<float *>(ws + p.part);
     a.part_ml = reinterpret_cast<float *>(ws + p.part_ml);
     a.scores = attn_sums ? reinterpret_cast<float *>(ws + p.scores) : nullptr;
@@ -694,18 +913,31 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     a.tiles = (int)p.tiles;
     a.pairs = (int)p.pairs;
     a.workgroups = (int)p.workgroups;
+    a.by_pairs = fast_div((uint32_t)p.pairs);
+    a.by_workgroups = fast_div((uint32_t)p.workgroups);
     a.capacity = (int)(max_blocks * cache->block_size);
+    a.max_blocks = (int)max_blocks;
+    a.part_bytes = p.part_bytes;
     a.scale2 = scale * kLog2e;
     const int es = quant ? 1 : 2;
-    // pieces of 16 bytes: rows and q on 16-byte boundaries, and no piece reaching past a row's end
-    a.vec = cache->head_dim * es % 16 == 0 && rows_aligned(a.cache.key, 16) && rows_aligned(a.cache.value, 16) && aligned(q, 16) &&
-            q_stride_batch % 8 == 0 && q_stride_head % 8 == 0;
-    const int64_t reach = (int64_t)1 << 26;                       // 16 rows stay within a 31-bit offset
-    const bool uni = a.vec && cache->block_size % 16 == 0 && a.cache.key.token < reach && a.cache.value.token < reach;
+    // pieces of 16 bytes: rows on 16-byte boundaries, and no piece reaching past a row's end
+    const bool pieces = cache->head_dim * es % 16 == 0 && rows_aligned(a.cache.key, 16) && rows_aligned(a.cache.value, 16);
+    // Halves that lie in one block: block by block, the last half of a block may be short, so blocks of fewer than 8 tokens
+    // would leave most of a tile empty.  Offsets within a block have 31 bits, a block's own offset is a 32 x 32-bit product.
+    const PagedArray *const arrays[] = {&a.cache.key, &a.cache.value, &a.cache.key_scale, &a.cache.value_scale};
+    bool blocks = pieces && cache->block_size >= 8, scales = cache->block_size % 4 == 0;
+    for (int i = 0; i < (quant ? 4 : 2); i++) {
+        const PagedArray &x = *arrays[i];
+        blocks = blocks && (!mask || cache->block_size % 4 == 0) && x.block >= 0 && x.block <= 0xffffffffll && x.token >= 0 && x.token <= 0x7fffffff / (cache->block_size + 16);
+        if (i >= 2) scales = scales && x.token == 4 && aligned(x.base, 16) && x.block % 16 == 0 && x.head % 16 == 0;
+    }
+    const Addressing ad = !blocks ? kRows : mask ? kBlockMask : quant && scales ? kBlockScales : kBlock;
+    a.span = ad != kRows ? a.cache.page : fast_div(kHalf);
+    a.halves = fast_div((a.span.d + kHalf - 1) / kHalf);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (p.dp == 64) launch_attention<64>(a, quant, fp16, uni, s);
-    else if (p.dp == 128) launch_attention<128>(a, quant, fp16, uni, s);
-    else launch_attention<256>(a, quant, fp16, uni, s);
+    if (p.dp == 64) launch_attention<64>(a, quant, fp16, ad, s);
+    else if (p.dp == 128) launch_attention<128>(a, quant, fp16, ad, s);
+    else launch_attention<256>(a, quant, fp16, ad, s);
     if (attn_sums && a.capacity > 0) {
         const int64_t chunks = (a.capacity + 1023) / 1024;
         for (int64_t b0 = 0; b0 < batch; b0 += 65535) {           // a grid's third dimension has 16 bits

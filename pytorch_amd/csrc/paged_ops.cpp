@@ -214,7 +214,7 @@ std::tuple<Tensor, Tensor> attention_hip(const Tensor &query, const Tensor &key_
     const Tensor hidden = !mask || inner_contiguous(*mask) ? (mask ? *mask : Tensor()) : mask->contiguous();
     const mi355_paged_cache c = describe(key_cache, value_cache, ks, vs);
     const size_t bytes = mi355_paged_decode_attention_workspace(batch, heads, kv_heads, q.size(2), table.size(1), key_cache.size(1), sums != nullptr);
-    const Tensor ws = new_empty(kLaunch, q, {(int64_t)bytes}, at::kChar);
+    const Tensor ws = mi355_ops::workspace(q, bytes, sums != nullptr);
     const double scale = scale_value.has_value() ? *scale_value : 1.0 / std::sqrt((double)q.size(2));
     check_status(mi355_paged_decode_attention(&c, q.data_ptr(), act_code(q.scalar_type()), q.stride(0), q.stride(1), out.data_ptr(),
                                               softmax_lse ? lse.data_ptr<float>() : nullptr, batch, heads, table.data_ptr<int32_t>(), table.stride(0),
