@@ -1,11 +1,16 @@
 // npu_paged_cache_evict for gfx950: sequences that outgrew their budget keep the newest tokens and those with the largest
 // summed attention weights, each key/value head its own.
 //
-// Per (sequence, head) with n > keep tokens a token's worth is a 32-bit key that orders like (recent, sum): all ones for the
-// recent ones, else the sum's bits with the sign flipped into place, 0 for NaN.  The keep-th largest key is found digit by
-// digit (four histograms of 8 bits); among tokens with exactly that key the lowest places stay.  Kept tokens behind place
+// Per (sequence, head) with n > keep a token's worth is a 32-bit key that orders like (recent, sum): all ones for the recent
+// ones, else the sum's bits with the sign flipped into place, 0 for NaN.  The keep-th largest key is found digit by digit
+// (histograms of 11, 11 and 10 bits); among tokens with exactly that key the lowest places stay.  Kept tokens behind place
 // `keep` then fill the holes before it, both in ascending order: the fewest rows move, sources and destinations are disjoint,
 // so all of them move at once, in place.
+//
+// One workgroup of 1024 threads chooses for one (sequence, head).  Thread t holds the places t, t + 1024, ..., whose keys stay
+// in registers over the three digits (rows of more than 32768 places are read again for each); ranks in the order of the places
+// come from ballots, counted per wavefront and 1024 places, and one scan over those counts.  Bound by latency: a dozen
+// barriers and three trips to memory.
 #include "paged_cache.h"
 
 namespace mi355 {
@@ -21,7 +26,7 @@ struct EvictArgs {
     int32_t *new_lens, *new_positions;
     float *new_sums;
     int32_t *count;                              // [batch * heads] moves
-    int32_t *moves;                              // [batch * heads][2][most]: places to, places from
+    int32_t *moves;                              // [batch * heads][2 * most]: count places that tokens go to, then those they leave
     int64_t most, recent;
     int keep, capacity;
 };
@@ -35,131 +40,69 @@ __device__ __forceinline__ uint32_t worth_of(float sum, int pos, int64_t oldest)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a)
+// Inclusive scans over the lanes of a wavefront: shifts within rows of 16 lanes, then the rows' last lanes handed on.  What a
+// lane gets from outside its row is the identity 0.
+struct Add {
+    __device__ uint32_t operator()(uint32_t x, uint32_t y) const { return x + y; }
+};
+struct Max {
+    __device__ uint32_t operator()(uint32_t x, uint32_t y) const { return max(x, y); }
+};
+template <int CTRL, int ROWS, class Op>
+__device__ __forceinline__ uint32_t take(uint32_t v, Op op)
 {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t found[2];
-    __shared__ int wave_top[kSelectWaves];
-    __shared__ uint32_t wave_count[3][kSelectWaves];
-
-    const int row = blockIdx.x, b = row / a.cache.heads, head = row % a.cache.heads;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n = min(max(a.lens[b], 0), a.capacity);
-    const float *sums = a.sums + b * a.sums_batch + head * a.sums_head;
-    const int32_t *pos = a.positions + b * a.positions_batch + head * a.positions_head;
-    float *new_sums = a.new_sums + (int64_t)row * a.capacity;
-    int32_t *new_pos = a.new_positions + (int64_t)row * a.capacity;
-    const int stay = min(n, a.keep);
-    if (head == 0 && tid == 0) a.new_lens[b] = stay;
-    for (int i = stay + tid; i < a.capacity; i += kSelectThreads) new_sums[i] = 0.0f, new_pos[i] = -1;
-    if (n <= a.keep || a.keep == 0) {
-        for (int i = tid; i < stay; i += kSelectThreads) new_sums[i] = sums[i], new_pos[i] = pos[i];
-        if (tid == 0) a.count[row] = 0;
-        return;
-    }
-
-    int newest = INT32_MIN;
-    for (int i = tid; i < n; i += kSelectThreads) newest = max(newest, pos[i]);
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) newest = max(newest, __shfl_xor(newest, off, 64));
-    if (lane == 0) wave_top[wave] = newest;
+    return op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false));
+}
+template <class Op>
+__device__ __forceinline__ uint32_t scan_row(uint32_t v, Op op)
+{
+    v = take<0x111, 0xf>(v, op);                 // row_shr:1
+    v = take<0x112, 0xf>(v, op);
+    v = take<0x114, 0xf>(v, op);
+    return take<0x118, 0xf>(v, op);
+}
+template <class Op>
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t v, Op op)
+{
+    v = take<0x142, 0xa>(scan_row(v, op), op);   // row_bcast:15 into rows 1 and 3
+    return take<0x143, 0xc>(v, op);              // row_bcast:31 into rows 2 and 3
+}
+// Scan over the workgroup, 16 wavefronts: what the threads before this one make together; `all` gets everybody's.  `lds`: one
+// word per wavefront, free again after the next barrier.
+static_assert(kSelectWaves == 16, "one row of lanes holds a word of every wavefront");
+template <class Op>
+__device__ __forceinline__ uint32_t scan_threads(uint32_t v, uint32_t *lds, uint32_t &all, Op op)
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const uint32_t scan = scan_lanes(v, op);
+    if (lane == 63) lds[wave] = scan;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSelectWaves; w++) newest = max(newest, wave_top[w]);
-    const int64_t oldest = (int64_t)newest - a.recent;
-
-    uint32_t prefix = 0, left = (uint32_t)a.keep;              // the left-th largest among the keys that start with prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += kSelectThreads) {
-            const uint32_t key = worth_of(sums[i], pos[i], oldest);
-            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255u], 1u);
-        }
-        __syncthreads();
-        if (wave == 0) {                                        // four digits per lane, lane 0 the largest ones
-            uint32_t c[4], sum = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) c[i] = hist[255 - (lane * 4 + i)], sum += c[i];
-            uint32_t scan = sum;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const uint32_t o = (uint32_t)__shfl_up((int)scan, off, 64);
-                if (lane >= off) scan += o;
-            }
-            uint32_t before = scan - sum;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (before < left && left <= before + c[i]) {   // one lane, one digit
-                    found[0] = 255 - (lane * 4 + i);
-                    found[1] = left - before;
-                }
-                before += c[i];
-            }
-        }
-        __syncthreads();
-        prefix |= found[0] << shift;
-        left = found[1];
-    }
-
-    // in the order of the places: which of the tokens with exactly the last key stay, the holes and what fills them
-    int32_t *to = a.moves + (int64_t)row * 2 * a.most, *from = to + a.most;
-    uint32_t ties = 0, holes = 0, fills = 0;
-    const uint64_t below = ((uint64_t)1 << lane) - 1;
-    for (int base = 0; base < n; base += kSelectThreads) {
-        const int i = base + tid;
-        const uint32_t key = i < n ? worth_of(sums[i], pos[i], oldest) : 0;
-        const bool tie = i < n && key == prefix;
-        const uint64_t tie_mask = __ballot(tie);
-        if (lane == 0) wave_count[0][wave] = (uint32_t)__popcll(tie_mask);
-        __syncthreads();
-        uint32_t rank = ties + (uint32_t)__popcll(tie_mask & below);
-        for (int w = 0; w < kSelectWaves; w++) {
-            if (w < wave) rank += wave_count[0][w];
-            ties += wave_count[0][w];
-        }
-        const bool kept = i < n && (key > prefix || (tie && rank < left));
-        const bool hole = i < n && i < a.keep && !kept, fill = kept && i >= a.keep;
-        const uint64_t hole_mask = __ballot(hole), fill_mask = __ballot(fill);
-        if (lane == 0) wave_count[1][wave] = (uint32_t)__popcll(hole_mask), wave_count[2][wave] = (uint32_t)__popcll(fill_mask);
-        __syncthreads();
-        uint32_t hole_rank = holes + (uint32_t)__popcll(hole_mask & below), fill_rank = fills + (uint32_t)__popcll(fill_mask & below);
-        for (int w = 0; w < kSelectWaves; w++) {
-            if (w < wave) hole_rank += wave_count[1][w], fill_rank += wave_count[2][w];
-            holes += wave_count[1][w];
-            fills += wave_count[2][w];
-        }
-        if (hole) to[hole_rank] = i;
-        if (fill) from[fill_rank] = i;
-        if (kept && i < a.keep) new_sums[i] = sums[i], new_pos[i] = pos[i];
-    }
-    __syncthreads();
-    for (uint32_t i = tid; i < holes; i += kSelectThreads) {
-        new_sums[to[i]] = sums[from[i]];
-        new_pos[to[i]] = pos[from[i]];
-    }
-    if (tid == 0) a.count[row] = (int32_t)holes;
+    const uint32_t waves = scan_row(lds[lane & 15], op);
+    all = (uint32_t)__builtin_amdgcn_readlane((int)waves, 15);
+    const uint32_t others = wave ? (uint32_t)__builtin_amdgcn_readlane((int)waves, wave - 1) : 0;
+    const uint32_t left_lane = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)scan, 0x138, 0xf, 0xf, false);       // wave_shr:1
+    return op(others, left_lane);
 }
 
-// Rows of keys and values, W bytes per access: 16 where every row starts on 16 bytes and has a multiple of them.
+// Moves rows of keys and values (and their scales) within one (sequence, head), W bytes per access: pieces first,
+// first + step, ... of all of them.  per_row = pieces of a row of keys, then of the row of values.
 template <int W>
-__global__ __launch_bounds__(256) void paged_move_kernel(EvictArgs a, int elem, int pieces, FastDiv per_row)
+__device__ __forceinline__ void move_pieces(const EvictArgs &a, int row, uint32_t count, uint32_t first, uint32_t step, int elem, const FastDiv &per_row)
 {
     typedef uint32_t word __attribute__((ext_vector_type(W >= 4 ? W / 4 : 1)));
-    const int row = blockIdx.y, b = row / a.cache.heads, head = row % a.cache.heads;
-    const int count = a.count[row];
-    const int32_t *to = a.moves + (int64_t)row * 2 * a.most, *from = to + a.most;
+    const int b = row / a.cache.heads, head = row % a.cache.heads;
+    const int32_t *to = a.moves + (int64_t)row * 2 * a.most, *from = to + count;
     const int32_t *table = a.table + b * a.table_stride;
-    const uint32_t all = (uint32_t)count * (uint32_t)pieces * 2;         // below 2^31: the host checks
-    for (uint32_t e = blockIdx.x * 256 + threadIdx.x; e < all; e += gridDim.x * 256) {
-        const uint32_t r = div_by(e, per_row), piece = e - r * per_row.d;   // per_row = pieces of keys, then of values
+    const uint32_t pieces = per_row.d / 2, all = count * per_row.d;      // below 2^31: the host checks
+    for (uint32_t e = first; e < all; e += step) {
+        const uint32_t r = div_by(e, per_row), piece = e - r * per_row.d;
         const uint32_t dst = (uint32_t)to[r], src = (uint32_t)from[r];
         const uint32_t dst_block = div_by(dst, a.cache.page), src_block = div_by(src, a.cache.page);
         const int dst_id = table[dst_block], src_id = table[src_block];
         if ((uint32_t)dst_id >= (uint32_t)a.cache.num_blocks || (uint32_t)src_id >= (uint32_t)a.cache.num_blocks) continue;
         const uint32_t dst_slot = (uint32_t)dst_id * a.cache.page.d + (dst - dst_block * a.cache.page.d);
         const uint32_t src_slot = (uint32_t)src_id * a.cache.page.d + (src - src_block * a.cache.page.d);
-        const bool value = piece >= (uint32_t)pieces;
+        const bool value = piece >= pieces;
         const PagedArray &x = value ? a.cache.value : a.cache.key;
         const uint32_t at = (value ? piece - pieces : piece) * W;
         char *d = x.base + a.cache.offset(x, dst_slot, head) + at;
@@ -173,6 +116,190 @@ __global__ __launch_bounds__(256) void paged_move_kernel(EvictArgs a, int elem, 
                 *reinterpret_cast<const float *>(sc.base + a.cache.offset(sc, src_slot, head));
         }
     }
+}
+
+// KPT: rounds of 1024 places whose keys are held, KPT * 1024 >= capacity; 0: any number, read again for every digit.
+// W: bytes per access of the moves that this kernel makes itself; 0: it leaves them to paged_move_kernel.
+template <int KPT, int W>
+__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a, int elem, FastDiv per_row)
+{
+    // places per scan of the counts below: 64 rounds with one count per thread
+    constexpr int kBatch = KPT ? KPT : 64;
+    __shared__ uint32_t hist[2048];
+    __shared__ uint32_t found[3];
+    __shared__ uint32_t wave_top[kSelectWaves], wave_sum[kSelectWaves];
+    __shared__ uint32_t count[kBatch * kSelectWaves];           // per round and wavefront: the ballot's ones, then those before
+
+    const int row = blockIdx.x, b = row / a.cache.heads, head = row % a.cache.heads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float *sums = a.sums + b * a.sums_batch + head * a.sums_head;
+    const int32_t *pos = a.positions + b * a.positions_batch + head * a.positions_head;
+    float *new_sums = a.new_sums + (int64_t)row * a.capacity;
+    int32_t *new_pos = a.new_positions + (int64_t)row * a.capacity;
+    constexpr int kHeld = KPT ? KPT : 1;
+    float sum[kHeld];
+    int32_t at[kHeld];
+    uint32_t key[kHeld];
+    if constexpr (KPT > 0) {                                    // requested before the length is known
+#pragma unroll
+        for (int j = 0; j < KPT; j++) {
+            const int i = min(j * kSelectThreads + tid, a.capacity - 1);
+            sum[j] = i >= 0 ? sums[i] : 0.0f, at[j] = i >= 0 ? pos[i] : 0;
+        }
+    }
+    const int n = min(max(a.lens[b], 0), a.capacity);
+    const int stay = min(n, a.keep);
+    if (head == 0 && tid == 0) a.new_lens[b] = stay;
+    if (n <= a.keep || a.keep == 0) {
+        for (int i = tid; i < a.capacity; i += kSelectThreads) new_sums[i] = i < stay ? sums[i] : 0.0f, new_pos[i] = i < stay ? pos[i] : -1;
+        if (tid == 0) a.count[row] = 0;
+        return;
+    }
+    for (int i = stay + tid; i < a.capacity; i += kSelectThreads) new_sums[i] = 0.0f, new_pos[i] = -1;
+    hist[tid] = 0, hist[tid + 1024] = 0;
+    int newest = INT32_MIN;
+    if constexpr (KPT > 0) {
+#pragma unroll
+        for (int j = 0; j < KPT; j++) newest = j * kSelectThreads + tid < n ? max(newest, at[j]) : newest;
+    } else {
+        for (int i = tid; i < n; i += kSelectThreads) newest = max(newest, pos[i]);
+    }
+    uint32_t top;                                               // positions as unsigned numbers in their order
+    scan_threads((uint32_t)newest ^ 0x80000000u, wave_top, top, Max());
+    newest = (int)(top ^ 0x80000000u);
+    const int64_t oldest = (int64_t)newest - a.recent;
+#pragma unroll
+    for (int j = 0; j < KPT; j++) key[j] = worth_of(sum[j], at[j], oldest);
+    const int rounds = KPT ? KPT : (n + kSelectThreads - 1) / kSelectThreads;
+    // calls each(j, place, key) for the thread's places, rounds [j0, j1)
+    const auto walk = [&](int j0, int j1, auto &&each) {
+        if constexpr (KPT > 0) {
+#pragma unroll
+            for (int j = 0; j < KPT; j++) each(j, j * kSelectThreads + tid, key[j]);
+        } else {
+            for (int j = j0; j < j1; j++) {
+                const int i = j * kSelectThreads + tid;
+                each(j, i, i < n ? worth_of(sums[i], pos[i], oldest) : 0u);
+            }
+        }
+    };
+
+    uint32_t prefix = 0, left = (uint32_t)a.keep, all;          // the left-th largest among the keys that start with prefix
+#pragma unroll
+    for (int digit = 0; digit < 3; digit++) {
+        const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, above = digit == 2 ? 10 : 21;
+        const uint32_t mask = digit == 2 ? 1023 : 2047;
+        walk(0, rounds, [&](int, int i, uint32_t k) {
+            if (i < n && (digit == 0 || (k >> above) == (prefix >> above))) atomicAdd(&hist[(k >> shift) & mask], 1u);
+        });
+        __syncthreads();
+        const uint32_t c0 = hist[2047 - 2 * tid], c1 = hist[2046 - 2 * tid];       // thread 0 has the largest digits
+        const uint32_t before = scan_threads(c0 + c1, wave_sum, all, Add());
+        if (before < left && left <= before + c0 + c1) {                           // one thread
+            const bool second = left > before + c0;
+            found[0] = 2047 - 2 * tid - second;
+            found[1] = left - before - (second ? c0 : 0);
+            found[2] = second ? c1 : c0;
+        }
+        hist[2047 - 2 * tid] = 0, hist[2046 - 2 * tid] = 0;                        // nobody else's
+        __syncthreads();
+        prefix |= found[0] << shift;
+        left = found[1];
+    }
+    const bool some = found[2] > left;                          // of the tokens with exactly the last key only some stay
+
+    // Counts, per round and wavefront, become the ones before; every thread of the workgroup calls it with its part.
+    const auto before_each = [&](uint32_t carry) {
+        __syncthreads();
+        const uint32_t mine = tid < kBatch * kSelectWaves ? count[tid] : 0;        // (kBatch * kSelectWaves <= 1024)
+        const uint32_t before = scan_threads(mine, wave_sum, all, Add());
+        if (tid < kBatch * kSelectWaves) count[tid] = carry + before;
+        __syncthreads();
+    };
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+    // the holes, then as many fills
+    int32_t *list = a.moves + (int64_t)row * 2 * a.most;
+    uint32_t ties = 0, ranks = 0;                               // before the batch of rounds
+    for (int j0 = 0; j0 < rounds; j0 += kBatch) {
+        const int j1 = min(j0 + kBatch, rounds);
+        uint64_t stays = 0;                                     // one bit per round
+        static_assert(kBatch <= 64, "one bit per round");
+        if (some) {
+            walk(j0, j1, [&](int j, int i, uint32_t k) {
+                const uint64_t tie = __ballot(i < n && k == prefix);
+                if (lane == 0) count[(j - j0) * kSelectWaves + wave] = (uint32_t)__popcll(tie);
+            });
+            if (tid >= (j1 - j0) * kSelectWaves && tid < kBatch * kSelectWaves) count[tid] = 0;
+            before_each(ties);
+            ties += all;
+        }
+        walk(j0, j1, [&](int j, int i, uint32_t k) {
+            bool kept = k > prefix || (k == prefix && !some);
+            if (some) {
+                const bool tie = i < n && k == prefix;
+                const uint32_t rank = count[(j - j0) * kSelectWaves + wave] + (uint32_t)__popcll(__ballot(tie) & below);
+                kept = kept || (tie && rank < left);
+            }
+            stays |= (uint64_t)(kept && i < n) << (j - j0);
+        });
+        if (some) __syncthreads();                              // the counts are used again
+        // a hole before `keep`, a fill behind it: holes come before all fills
+        const auto moves = [&](int i, int j) { return i < n && ((stays >> (j - j0)) & 1) == (uint64_t)(i >= a.keep); };
+        for (int j = j0; j < j1; j++) {
+            const uint64_t m = __ballot(moves(j * kSelectThreads + tid, j));
+            if (lane == 0) count[(j - j0) * kSelectWaves + wave] = (uint32_t)__popcll(m);
+        }
+        if (tid >= (j1 - j0) * kSelectWaves && tid < kBatch * kSelectWaves) count[tid] = 0;
+        before_each(ranks);
+        ranks += all;
+        walk(j0, j1, [&](int j, int i, uint32_t) {
+            const bool move = moves(i, j);
+            const uint64_t m = __ballot(move);
+            if (move) {
+                list[count[(j - j0) * kSelectWaves + wave] + (uint32_t)__popcll(m & below)] = i;
+            } else if (i < a.keep) {
+                new_sums[i] = KPT ? sum[KPT ? j : 0] : sums[i];
+                new_pos[i] = KPT ? at[KPT ? j : 0] : pos[i];
+            }
+        });
+        __syncthreads();
+    }
+    const uint32_t holes = ranks / 2;
+    for (uint32_t r = tid; r < holes; r += kSelectThreads) {
+        const int place = list[r], src = list[holes + r];
+        new_sums[place] = sums[src];
+        new_pos[place] = pos[src];
+    }
+    if constexpr (W > 0) move_pieces<W>(a, row, holes, tid, kSelectThreads, elem, per_row);
+    else if (tid == 0) a.count[row] = (int32_t)holes;
+}
+
+template <int W>
+__global__ __launch_bounds__(256) void paged_move_kernel(EvictArgs a, int elem, FastDiv per_row)
+{
+    move_pieces<W>(a, blockIdx.y, (uint32_t)a.count[blockIdx.y], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, elem, per_row);
+}
+
+// A workgroup that chooses moves its rows itself where there can be few: up to this many bytes of keys.
+constexpr int64_t kMovedBySelect = 16384;
+
+template <int KPT>
+void launch_select(const EvictArgs &a, unsigned rows, int width, int elem, const FastDiv &per_row, hipStream_t s)
+{
+    const dim3 grid(rows), block(kSelectThreads);
+    if (width == 16) hipLaunchKernelGGL((paged_select_kernel<KPT, 16>), grid, block, 0, s, a, elem, per_row);
+    else if (width == 2) hipLaunchKernelGGL((paged_select_kernel<KPT, 2>), grid, block, 0, s, a, elem, per_row);
+    else if (width == 1) hipLaunchKernelGGL((paged_select_kernel<KPT, 1>), grid, block, 0, s, a, elem, per_row);
+    else hipLaunchKernelGGL((paged_select_kernel<KPT, 0>), grid, block, 0, s, a, elem, per_row);
+}
+void launch_select(const EvictArgs &a, unsigned rows, int width, int elem, const FastDiv &per_row, hipStream_t s)
+{
+    if (a.capacity <= 2 * kSelectThreads) launch_select<2>(a, rows, width, elem, per_row, s);
+    else if (a.capacity <= 5 * kSelectThreads) launch_select<5>(a, rows, width, elem, per_row, s);
+    else if (a.capacity <= 8 * kSelectThreads) launch_select<8>(a, rows, width, elem, per_row, s);
+    else if (a.capacity <= 16 * kSelectThreads) launch_select<16>(a, rows, width, elem, per_row, s);
+    else if (a.capacity <= 32 * kSelectThreads) launch_select<32>(a, rows, width, elem, per_row, s);
+    else launch_select<0>(a, rows, width, elem, per_row, s);
 }
 
 // moves of one row at most
@@ -227,24 +354,22 @@ extern "C" int mi355_paged_cache_evict(const mi355_paged_cache *cache, const int
     a.count = static_cast<int32_t *>(workspace);
     a.moves = reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + (rows * 4 + 255) / 256 * 256);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)rows), dim3(kSelectThreads), 0, s, a);
-    if (a.most > 0) {
-        const int elem = cache_elem_bytes(cache->dtype), bytes = (int)cache->head_dim * elem;
-        const bool wide = bytes % 16 == 0 && rows_aligned(a.cache.key, 16) && rows_aligned(a.cache.value, 16);
-        const int width = wide ? 16 : elem, pieces = bytes / width;
-        const int64_t most = (a.most * pieces * 2 + 255) / 256;
-        const dim3 grid((unsigned)(most < 64 ? most : 64), 1);
-        for (int64_t r0 = 0; r0 < rows; r0 += 65535 / cache->kv_heads * cache->kv_heads) {   // a grid's second dimension has 16 bits
+    const int elem = cache_elem_bytes(cache->dtype), bytes = (int)cache->head_dim * elem;
+    const bool wide = bytes % 16 == 0 && rows_aligned(a.cache.key, 16) && rows_aligned(a.cache.value, 16);
+    const FastDiv per_row = fast_div((uint32_t)(bytes / (wide ? 16 : elem)) * 2);
+    const bool here = a.most * bytes <= kMovedBySelect;
+    launch_select(a, (unsigned)rows, here ? (wide ? 16 : elem) : 0, elem, per_row, s);
+    if (!here) {
+        const int64_t chunks = (a.most * per_row.d + 255) / 256, n = 65535 / cache->kv_heads * cache->kv_heads;
+        for (int64_t r0 = 0; r0 < rows; r0 += n) {               // a grid's second dimension has 16 bits
             EvictArgs c = a;
-            const int64_t n = 65535 / cache->kv_heads * cache->kv_heads;
             c.count += r0;
             c.moves += r0 * 2 * a.most;
             c.table += r0 / cache->kv_heads * table_stride;
-            const dim3 g(grid.x, (unsigned)(rows - r0 < n ? rows - r0 : n));
-            const FastDiv per_row = fast_div((uint32_t)pieces * 2);
-            if (wide) hipLaunchKernelGGL(paged_move_kernel<16>, g, dim3(256), 0, s, c, elem, pieces, per_row);
-            else if (elem == 2) hipLaunchKernelGGL(paged_move_kernel<2>, g, dim3(256), 0, s, c, elem, pieces, per_row);
-            else hipLaunchKernelGGL(paged_move_kernel<1>, g, dim3(256), 0, s, c, elem, pieces, per_row);
+            const dim3 grid((unsigned)(chunks < 64 ? chunks : 64), (unsigned)(rows - r0 < n ? rows - r0 : n));
+            if (wide) hipLaunchKernelGGL(paged_move_kernel<16>, grid, dim3(256), 0, s, c, elem, per_row);
+            else if (elem == 2) hipLaunchKernelGGL(paged_move_kernel<2>, grid, dim3(256), 0, s, c, elem, per_row);
+            else hipLaunchKernelGGL(paged_move_kernel<1>, grid, dim3(256), 0, s, c, elem, per_row);
         }
     }
     return check_launch();
