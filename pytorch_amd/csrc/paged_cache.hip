@@ -18,9 +18,19 @@ struct RowArgs {
     int64_t tok[2], head[2];           // their element strides
     const void *slot_ids;
     int slots64;                       // slot ids are int64, else int32
-    FastDiv heads;
-    uint32_t rows;                     // tokens * heads
+    FastDiv parts;                     // groups of heads of a token: heads / N
+    uint32_t tokens, groups;           // groups = tokens, rounded up to the run, * parts
+    int run;                           // log2 of the tokens of one head that follow each other
 };
+
+// Groups of N heads of a token are numbered so that neighbours lie side by side in the cache: the heads of a token, or 16
+// tokens of the same heads.
+__device__ __forceinline__ void group_at(const RowArgs &a, uint32_t group, uint32_t &t, uint32_t &part)
+{
+    const uint32_t q = group >> a.run, block = div_by(q, a.parts);
+    part = q - block * a.parts.d;
+    t = (block << a.run) + (group & ((1u << a.run) - 1));
+}
 
 __device__ __forceinline__ int64_t load_slot(const RowArgs &a, uint32_t t)
 {
@@ -59,38 +69,41 @@ struct RowQuant {
     }
 };
 
-// GL lanes per row, eight elements per lane: rows that start on 16-byte boundaries, dim % 8 == 0 and <= 8 GL.
-// QUANT: int8 cache; FP16: the 16-bit type (read by the conversions alone).
-template <int GL, bool QUANT, bool FP16>
+// GL lanes per row, eight elements per lane: rows that start on 16-byte boundaries, dim % 8 == 0 and <= 8 GL.  N heads of a
+// token per group of lanes: slot and addresses are worked out once (they were half of the instructions, and the int8 writer
+// is bound by those), the rows requested together.  QUANT: int8 cache; FP16: the 16-bit type (for the conversions alone).
+template <int GL, int N, bool QUANT, bool FP16>
 __global__ __launch_bounds__(256) void paged_write_kernel(RowArgs a)
 {
     const int plane = blockIdx.y, lane = threadIdx.x % GL;
-    const uint32_t row = blockIdx.x * (256 / GL) + threadIdx.x / GL;
-    const uint32_t t = div_by(row, a.heads), h = row - t * a.heads.d;
-    if (row >= a.rows) return;                                   // whole groups of GL lanes leave together
-    const int64_t slot = load_slot(a, t);
+    const uint32_t group = blockIdx.x * (256 / GL) + threadIdx.x / GL;
+    uint32_t t, part;
+    group_at(a, group, t, part);
+    if (group >= a.groups || t >= a.tokens) return;              // whole groups of lanes leave together
     const bool mine = lane * 8 < a.cache.dim;
-    u32x4 v = u32x4{0, 0, 0, 0};
-    if (mine) v = *reinterpret_cast<const u32x4 *>(a.plane[plane] + t * a.tok[plane] + h * a.head[plane] + lane * 8);
-    if (slot < 0 || slot >= a.cache.slots) return;
-    const PagedArray &to = plane ? a.cache.value : a.cache.key;
-    char *dst = to.base + a.cache.offset(to, (uint32_t)slot, (int)h);
-    if constexpr (!QUANT) {
-        if (mine) *reinterpret_cast<u32x4 *>(dst + lane * 16) = v;
-    } else {
-        uint32_t m = absmax8(v);
+    const PagedArray &to = plane ? a.cache.value : a.cache.key, &sc = plane ? a.cache.value_scale : a.cache.key_scale;
+    const int64_t slot = load_slot(a, t);
+    const uint16_t *src = a.plane[plane] + t * a.tok[plane] + (part * N) * a.head[plane] + lane * 8;
+    u32x4 v[N];
 #pragma unroll
-        for (int off = GL / 2; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, GL));
-        const RowQuant q(act_1<FP16>((uint16_t)m));
-        if (mine) {
+    for (int i = 0; i < N; i++) v[i] = mine ? *reinterpret_cast<const u32x4 *>(src + i * a.head[plane]) : u32x4{0, 0, 0, 0};
+    if (slot < 0 || slot >= a.cache.slots) return;
+    char *dst = to.base + a.cache.offset(to, (uint32_t)slot, (int)(part * N)) + lane * (QUANT ? 8 : 16);
+    char *scale = QUANT ? sc.base + a.cache.offset(sc, (uint32_t)slot, (int)(part * N)) : nullptr;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if constexpr (!QUANT) {
+            if (mine) *reinterpret_cast<u32x4 *>(dst + i * to.head) = v[i];
+        } else {
+            uint32_t m = absmax8(v[i]);
+#pragma unroll
+            for (int off = GL / 2; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, GL));
+            const RowQuant q(act_1<FP16>((uint16_t)m));
             u32x2 o;
-            o.x = pack4(q(act_lo<FP16>(v.x)), q(act_hi<FP16>(v.x)), q(act_lo<FP16>(v.y)), q(act_hi<FP16>(v.y)));
-            o.y = pack4(q(act_lo<FP16>(v.z)), q(act_hi<FP16>(v.z)), q(act_lo<FP16>(v.w)), q(act_hi<FP16>(v.w)));
-            *reinterpret_cast<u32x2 *>(dst + lane * 8) = o;
-        }
-        if (lane == 0) {
-            const PagedArray &s = plane ? a.cache.value_scale : a.cache.key_scale;
-            *reinterpret_cast<float *>(s.base + a.cache.offset(s, (uint32_t)slot, (int)h)) = q.scale;
+            o.x = pack4(q(act_lo<FP16>(v[i].x)), q(act_hi<FP16>(v[i].x)), q(act_lo<FP16>(v[i].y)), q(act_hi<FP16>(v[i].y)));
+            o.y = pack4(q(act_lo<FP16>(v[i].z)), q(act_hi<FP16>(v[i].z)), q(act_lo<FP16>(v[i].w)), q(act_hi<FP16>(v[i].w)));
+            if (mine) *reinterpret_cast<u32x2 *>(dst + i * to.head) = o;
+            if (lane == 0) *reinterpret_cast<float *>(scale + i * sc.head) = q.scale;
         }
     }
 }
@@ -101,8 +114,9 @@ __global__ __launch_bounds__(256) void paged_write_any_kernel(RowArgs a, int fp1
 {
     const int plane = blockIdx.y, lane = threadIdx.x % 64;
     const uint32_t row = blockIdx.x * 4 + threadIdx.x / 64;
-    if (row >= a.rows) return;
-    const uint32_t t = div_by(row, a.heads), h = row - t * a.heads.d;
+    uint32_t t, h;
+    group_at(a, row, t, h);
+    if (row >= a.groups || t >= a.tokens) return;
     const int64_t slot = load_slot(a, t);
     if (slot < 0 || slot >= a.cache.slots) return;
     const uint16_t *x = a.plane[plane] + t * a.tok[plane] + h * a.head[plane];
@@ -124,31 +138,43 @@ __global__ __launch_bounds__(256) void paged_write_any_kernel(RowArgs a, int fp1
     }
 }
 
-template <int GL, bool QUANT, bool FP16>
+template <int GL, int N, bool QUANT, bool FP16>
 __global__ __launch_bounds__(256) void paged_read_kernel(RowArgs a)
 {
     const int plane = blockIdx.y, lane = threadIdx.x % GL;
-    const uint32_t row = blockIdx.x * (256 / GL) + threadIdx.x / GL;
-    const uint32_t t = div_by(row, a.heads), h = row - t * a.heads.d;
-    if (row >= a.rows || lane * 8 >= a.cache.dim) return;
+    const uint32_t group = blockIdx.x * (256 / GL) + threadIdx.x / GL;
+    uint32_t t, part;
+    group_at(a, group, t, part);
+    if (group >= a.groups || t >= a.tokens || lane * 8 >= a.cache.dim) return;
+    const PagedArray &from = plane ? a.cache.value : a.cache.key, &sc = plane ? a.cache.value_scale : a.cache.key_scale;
     const int64_t slot = load_slot(a, t);
-    u32x4 v = u32x4{0, 0, 0, 0};
+    u32x4 v[N] = {};
     if (slot >= 0 && slot < a.cache.slots) {
-        const PagedArray &from = plane ? a.cache.value : a.cache.key;
-        const char *src = from.base + a.cache.offset(from, (uint32_t)slot, (int)h);
-        if constexpr (!QUANT) {
-            v = *reinterpret_cast<const u32x4 *>(src + lane * 16);
+        const char *src = from.base + a.cache.offset(from, (uint32_t)slot, (int)(part * N)) + lane * (QUANT ? 8 : 16);
+        if constexpr (QUANT) {
+            const char *at = sc.base + a.cache.offset(sc, (uint32_t)slot, (int)(part * N));
+            u32x2 c[N];
+            float scale[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                c[i] = *reinterpret_cast<const u32x2 *>(src + i * from.head);
+                scale[i] = *reinterpret_cast<const float *>(at + i * sc.head);
+            }
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                v[i].x = pack_act2<FP16>(sbyte_f32(c[i].x, 0) * scale[i], sbyte_f32(c[i].x, 1) * scale[i]);
+                v[i].y = pack_act2<FP16>(sbyte_f32(c[i].x, 2) * scale[i], sbyte_f32(c[i].x, 3) * scale[i]);
+                v[i].z = pack_act2<FP16>(sbyte_f32(c[i].y, 0) * scale[i], sbyte_f32(c[i].y, 1) * scale[i]);
+                v[i].w = pack_act2<FP16>(sbyte_f32(c[i].y, 2) * scale[i], sbyte_f32(c[i].y, 3) * scale[i]);
+            }
         } else {
-            const PagedArray &s = plane ? a.cache.value_scale : a.cache.key_scale;
-            const float scale = *reinterpret_cast<const float *>(s.base + a.cache.offset(s, (uint32_t)slot, (int)h));
-            const u32x2 c = *reinterpret_cast<const u32x2 *>(src + lane * 8);
-            v.x = pack_act2<FP16>(sbyte_f32(c.x, 0) * scale, sbyte_f32(c.x, 1) * scale);
-            v.y = pack_act2<FP16>(sbyte_f32(c.x, 2) * scale, sbyte_f32(c.x, 3) * scale);
-            v.z = pack_act2<FP16>(sbyte_f32(c.y, 0) * scale, sbyte_f32(c.y, 1) * scale);
-            v.w = pack_act2<FP16>(sbyte_f32(c.y, 2) * scale, sbyte_f32(c.y, 3) * scale);
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = *reinterpret_cast<const u32x4 *>(src + i * from.head);
         }
     }
-    *reinterpret_cast<u32x4 *>(a.plane[plane] + t * a.tok[plane] + h * a.head[plane] + lane * 8) = v;
+    uint16_t *dst = a.plane[plane] + t * a.tok[plane] + (part * N) * a.head[plane] + lane * 8;
+#pragma unroll
+    for (int i = 0; i < N; i++) __builtin_nontemporal_store(v[i], reinterpret_cast<u32x4 *>(dst + i * a.head[plane]));
 }
 
 template <bool QUANT>
@@ -156,8 +182,9 @@ __global__ __launch_bounds__(256) void paged_read_any_kernel(RowArgs a, int fp16
 {
     const int plane = blockIdx.y, lane = threadIdx.x % 64;
     const uint32_t row = blockIdx.x * 4 + threadIdx.x / 64;
-    if (row >= a.rows) return;
-    const uint32_t t = div_by(row, a.heads), h = row - t * a.heads.d;
+    uint32_t t, h;
+    group_at(a, row, t, h);
+    if (row >= a.groups || t >= a.tokens) return;
     const int64_t slot = load_slot(a, t);
     uint16_t *y = a.plane[plane] + t * a.tok[plane] + h * a.head[plane];
     const bool there = slot >= 0 && slot < a.cache.slots;
@@ -179,18 +206,38 @@ __global__ __launch_bounds__(256) void paged_read_any_kernel(RowArgs a, int fp16
     }
 }
 
-template <bool WRITE, int GL>
-void launch_rows(const RowArgs &a, bool quant, bool fp16, dim3 grid, hipStream_t s)
+// Groups of n heads (a divisor of the heads); RowArgs is complete after it.
+void number_groups(RowArgs &a, int n)
 {
+    const uint32_t parts = (uint32_t)(a.cache.heads / n);
+    a.parts = fast_div(parts);
+    a.groups = ((a.tokens + (1u << a.run) - 1) >> a.run << a.run) * parts;
+}
+
+template <bool WRITE, int GL, int N>
+void launch_rows(RowArgs &a, bool quant, bool fp16, hipStream_t s)
+{
+    number_groups(a, N);
+    const dim3 grid((a.groups + 256 / GL - 1) / (256 / GL), 2);
     if constexpr (WRITE) {
-        if (!quant) hipLaunchKernelGGL((paged_write_kernel<GL, false, false>), grid, dim3(256), 0, s, a);
-        else if (fp16) hipLaunchKernelGGL((paged_write_kernel<GL, true, true>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((paged_write_kernel<GL, true, false>), grid, dim3(256), 0, s, a);
+        if (!quant) hipLaunchKernelGGL((paged_write_kernel<GL, N, false, false>), grid, dim3(256), 0, s, a);
+        else if (fp16) hipLaunchKernelGGL((paged_write_kernel<GL, N, true, true>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((paged_write_kernel<GL, N, true, false>), grid, dim3(256), 0, s, a);
     } else {
-        if (!quant) hipLaunchKernelGGL((paged_read_kernel<GL, false, false>), grid, dim3(256), 0, s, a);
-        else if (fp16) hipLaunchKernelGGL((paged_read_kernel<GL, true, true>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((paged_read_kernel<GL, true, false>), grid, dim3(256), 0, s, a);
+        if (!quant) hipLaunchKernelGGL((paged_read_kernel<GL, N, false, false>), grid, dim3(256), 0, s, a);
+        else if (fp16) hipLaunchKernelGGL((paged_read_kernel<GL, N, true, true>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((paged_read_kernel<GL, N, true, false>), grid, dim3(256), 0, s, a);
     }
+}
+template <bool WRITE, int GL>
+void launch_rows(RowArgs &a, bool quant, bool fp16, hipStream_t s)
+{
+    // One row per group of lanes while that leaves the card short of workgroups.  Beyond: 8192 tokens to int8, 8 heads of 128,
+    // 14.3 us with one row per group, 13.2 with two, 13.9 with four; 32768 tokens from int8 33.6, 31.3 and 31.2.
+    const bool many = (int64_t)a.tokens * a.cache.heads * 2 / (256 / GL) >= kNumCU * 16;
+    if (many && !WRITE && a.cache.heads % 4 == 0) launch_rows<WRITE, GL, 4>(a, quant, fp16, s);
+    else if (many && a.cache.heads % 2 == 0) launch_rows<WRITE, GL, 2>(a, quant, fp16, s);
+    else launch_rows<WRITE, GL, 1>(a, quant, fp16, s);
 }
 
 template <bool WRITE>
@@ -204,7 +251,7 @@ int move_rows(const mi355_paged_cache *cache, int dtype, void *key, const int64_
     if (slots_dtype != MI355_DTYPE_INT32 && slots_dtype != MI355_DTYPE_INT64) return MI355_ERR_BAD_ARGUMENT;
     if (tokens == 0) return MI355_OK;
     if (!key || !value || !slots || !key_stride || !value_stride) return MI355_ERR_BAD_ARGUMENT;
-    if (tokens > 0x7fffffff / cache->kv_heads) return MI355_ERR_UNSUPPORTED;
+    if (tokens > 0x7fffff00 / cache->kv_heads - 16) return MI355_ERR_UNSUPPORTED;
     if (!aligned(key, 2) || !aligned(value, 2) || !aligned(slots, slots_dtype == MI355_DTYPE_INT64 ? 8 : 4)) return MI355_ERR_ALIGNMENT;
     a.plane[0] = static_cast<uint16_t *>(key);
     a.plane[1] = static_cast<uint16_t *>(value);
@@ -217,25 +264,26 @@ int move_rows(const mi355_paged_cache *cache, int dtype, void *key, const int64_
     }
     a.slot_ids = slots;
     a.slots64 = slots_dtype == MI355_DTYPE_INT64;
-    a.heads = fast_div((uint32_t)cache->kv_heads);
-    a.rows = (uint32_t)(tokens * cache->kv_heads);
+    a.run = a.cache.key.token < a.cache.key.head ? 4 : 0;
+    a.tokens = (uint32_t)tokens;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool fp16 = dtype == MI355_DTYPE_FP16;
-    const auto grid = [&](int per) { return dim3((a.rows + per - 1) / per, 2); };
     if (!vec) {
+        number_groups(a, 1);
+        const dim3 grid((a.groups + 3) / 4, 2);
         if constexpr (WRITE) {
-            if (quant) hipLaunchKernelGGL(paged_write_any_kernel<true>, grid(4), dim3(256), 0, s, a, fp16);
-            else hipLaunchKernelGGL(paged_write_any_kernel<false>, grid(4), dim3(256), 0, s, a, fp16);
+            if (quant) hipLaunchKernelGGL(paged_write_any_kernel<true>, grid, dim3(256), 0, s, a, fp16);
+            else hipLaunchKernelGGL(paged_write_any_kernel<false>, grid, dim3(256), 0, s, a, fp16);
         } else {
-            if (quant) hipLaunchKernelGGL(paged_read_any_kernel<true>, grid(4), dim3(256), 0, s, a, fp16);
-            else hipLaunchKernelGGL(paged_read_any_kernel<false>, grid(4), dim3(256), 0, s, a, fp16);
+            if (quant) hipLaunchKernelGGL(paged_read_any_kernel<true>, grid, dim3(256), 0, s, a, fp16);
+            else hipLaunchKernelGGL(paged_read_any_kernel<false>, grid, dim3(256), 0, s, a, fp16);
         }
     } else if (a.cache.dim <= 64) {
-        launch_rows<WRITE, 8>(a, quant, fp16, grid(32), s);
+        launch_rows<WRITE, 8>(a, quant, fp16, s);
     } else if (a.cache.dim <= 128) {
-        launch_rows<WRITE, 16>(a, quant, fp16, grid(16), s);
+        launch_rows<WRITE, 16>(a, quant, fp16, s);
     } else {
-        launch_rows<WRITE, 32>(a, quant, fp16, grid(8), s);
+        launch_rows<WRITE, 32>(a, quant, fp16, s);
     }
     return check_launch();
 }
