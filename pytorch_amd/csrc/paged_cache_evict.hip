@@ -40,33 +40,6 @@ __device__ __forceinline__ uint32_t worth_of(float sum, int pos, int64_t oldest)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Inclusive scans over the lanes of a wavefront: shifts within rows of 16 lanes, then the rows' last lanes handed on.  What a
-// lane gets from outside its row is the identity 0.
-struct Add {
-    __device__ uint32_t operator()(uint32_t x, uint32_t y) const { return x + y; }
-};
-struct Max {
-    __device__ uint32_t operator()(uint32_t x, uint32_t y) const { return max(x, y); }
-};
-template <int CTRL, int ROWS, class Op>
-__device__ __forceinline__ uint32_t take(uint32_t v, Op op)
-{
-    return op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false));
-}
-template <class Op>
-__device__ __forceinline__ uint32_t scan_row(uint32_t v, Op op)
-{
-    v = take<0x111, 0xf>(v, op);                 // row_shr:1
-    v = take<0x112, 0xf>(v, op);
-    v = take<0x114, 0xf>(v, op);
-    return take<0x118, 0xf>(v, op);
-}
-template <class Op>
-__device__ __forceinline__ uint32_t scan_lanes(uint32_t v, Op op)
-{
-    v = take<0x142, 0xa>(scan_row(v, op), op);   // row_bcast:15 into rows 1 and 3
-    return take<0x143, 0xc>(v, op);              // row_bcast:31 into rows 2 and 3
-}
 // Scan over the workgroup, 16 wavefronts: what the threads before this one make together; `all` gets everybody's.  `lds`: one
 // word per wavefront, free again after the next barrier.
 static_assert(kSelectWaves == 16, "one row of lanes holds a word of every wavefront");

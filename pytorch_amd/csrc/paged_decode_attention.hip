@@ -20,9 +20,9 @@
 // values multiplies its probability, in float32.
 //
 // Work is dealt out on the device, because the lengths are known only there: the positions of every (sequence, head) pair
-// are cut into halves of a tile, 16 positions of one block (fewer at a block's end), eight halves make a unit, all units are
-// numbered, and every workgroup takes the same number of consecutive ones.  A pair that lies within one workgroup is
-// finished there; of a pair that is cut, every workgroup leaves (sums, m, l) in the workspace, and the last one to arrive adds
+// are cut into halves of a tile, 16 positions of one block (fewer at a block's end), eight halves make a unit, and a pair
+// of more units than the card's fair share is cut into equal pieces of at most that.  A workgroup takes a piece at a time; a
+// pair of one piece is finished there, else the workgroup leaves (sums, m, l) in the workspace, and the last one to arrive adds
 // them in their order.
 #include "paged_cache.h"
 #include "weight_quant_common.h"
@@ -46,18 +46,18 @@ struct AttnArgs {
     int64_t table_stride;
     const uint8_t *mask;
     int64_t mask_stride;
-    uint32_t *arrived;                       // [workgroups] zero before and after
-    float *part;                             // [workgroups][2][rows][DP]
-    float *part_ml;                          // [workgroups][2][kHeads][2]: maximum, sum
+    uint32_t *arrived;                       // [2][cut pieces] zero before and after
+    float *part;                             // [cut pieces][rows][DP]
+    float *part_ml;                          // [cut pieces][kHeads][2]: maximum, sum
     float *scores;                           // [batch * heads][score_pitch] z_j, or null
     float *lse2;                             // [batch * heads] m + log2 l, with scores
     float *sums;
     int64_t score_pitch, sums_batch, sums_head;
-    FastDiv by_pairs, by_workgroups;
+    FastDiv by_pairs, by_shares;
     FastDiv span, halves;                    // positions that are cut into halves together (a block, or 16), and their halves
-    int batch, heads, group, rows, tiles, pairs, workgroups;    // pairs = key/value heads * tiles, of one sequence
+    int batch, heads, group, rows, tiles, pairs, shares;        // pairs = key/value heads * tiles, of one sequence
     int capacity, max_blocks;                // capacity = max_blocks * block_size
-    uint32_t part_bytes;
+    uint32_t part_bytes, part_ml_bytes;
     float scale2;                            // scale * log2(e)
 };
 
@@ -106,39 +106,59 @@ __device__ __forceinline__ uint32_t halves_of(Args a, int len)
 }
 __device__ __forceinline__ uint32_t units_of(Args a, int len) { return (halves_of(a, len) + kUnit - 1) / kUnit; }
 
-// The numbering of units: sequence by sequence, in it pair by pair.  Every wavefront counts for itself, lane i a run of
-// consecutive sequences; no barrier, no LDS.
-struct Numbering {
-    uint32_t before, sum, total;             // units of one pair: in the runs before this lane's, in it, in all
+// How the work is cut up, and the numbering of the pieces: sequence by sequence, in it pair by pair.  Every wavefront counts for
+// itself, lane i a run of consecutive sequences; no barrier, no LDS.
+struct Pieces {
+    uint32_t share;                          // units of a piece at most
+    uint32_t before, count, total;           // pieces of one pair: in the runs before this lane's, in it, in all
+    uint32_t cut_before;                     // those of pairs with several pieces, before this lane's run
     int run, len;                            // sequences per lane; the length of the first
+    bool empty;                              // there is a sequence without positions
 
-    __device__ explicit Numbering(Args a)
+    __device__ uint32_t of(uint32_t units) const { return (units + share - 1) / share; }
+    __device__ explicit Pieces(Args a)
     {
         const int lane = threadIdx.x & 63, batch = a->batch;
         run = (batch + 63) / 64;
-        sum = 0;
-        len = lane * run < batch ? clamp_len(a, at(a->lens)[lane * run]) : 0;
-        sum = units_of(a, len);
-        for (int i = lane * run + 1; i < min((lane + 1) * run, batch); i++) sum += units_of(a, clamp_len(a, at(a->lens)[i]));
-        uint32_t scan = sum;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t o = (uint32_t)__shfl_up((int)scan, off, 64);
-            if (lane >= off) scan += o;
+        const int first = lane * run, end = min(first + run, batch);
+        len = first < batch ? clamp_len(a, at(a->lens)[first]) : 0;
+        const uint32_t mine = units_of(a, len);
+        uint32_t sum = mine;
+        bool none = first < batch && mine == 0;
+        for (int i = first + 1; i < end; i++) {
+            const uint32_t units = units_of(a, clamp_len(a, at(a->lens)[i]));
+            none = none || units == 0;
+            sum += units;
         }
-        before = scan - sum;
+        empty = __any(none);
+        const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)scan_lanes(sum, Add()), 63) * (uint32_t)a->pairs;
+        share = max(divide(all + a->shares - 1, a->by_shares), 1u);
+        count = of(mine);
+        uint32_t cut = count > 1 ? count : 0;
+        for (int i = first + 1; i < end; i++) {
+            const uint32_t pieces = of(units_of(a, clamp_len(a, at(a->lens)[i])));
+            count += pieces;
+            cut += pieces > 1 ? pieces : 0;
+        }
+        const uint32_t scan = scan_lanes(count, Add());
+        before = scan - count;
         total = (uint32_t)__builtin_amdgcn_readlane((int)scan, 63);
+        cut_before = scan_lanes(cut, Add()) - cut;
     }
-    // the sequence that holds unit y of one pair, how many units come before it, and its own
-    __device__ void find(Args a, uint32_t y, int &b, uint32_t &units_before, uint32_t &units) const
+    // the sequence that holds piece y of one pair: its length and pieces, and how many (of them cut) come before it
+    __device__ void find(Args a, uint32_t y, int &b, int &length, uint32_t &pieces, uint32_t &pieces_before, uint32_t &cut_pieces_before) const
     {
-        const int lane = __builtin_ctzll(__ballot(y >= before && y - before < sum));
+        const int lane = __builtin_ctzll(__ballot(y >= before && y - before < count));
         b = lane * run;
-        units_before = (uint32_t)__builtin_amdgcn_readlane((int)before, lane);
-        units = units_of(a, __builtin_amdgcn_readlane(len, lane));
-        while (y - units_before >= units) {
-            units_before += units;
-            units = units_of(a, clamp_len(a, scalar_load(a->lens + ++b)));
+        pieces_before = (uint32_t)__builtin_amdgcn_readlane((int)before, lane);
+        cut_pieces_before = (uint32_t)__builtin_amdgcn_readlane((int)cut_before, lane);
+        length = __builtin_amdgcn_readlane(len, lane);
+        pieces = uniform(of(units_of(a, length)));
+        while (y - pieces_before >= pieces) {
+            pieces_before += pieces;
+            cut_pieces_before += pieces > 1 ? pieces : 0;
+            length = clamp_len(a, scalar_load(a->lens + ++b));
+            pieces = uniform(of(units_of(a, length)));
         }
     }
 };
@@ -577,108 +597,209 @@ __device__ __forceinline__ void store_lse(Args a, int64_t row, float m, float l,
     if (a->lse2) at(a->lse2)[row] = lse2;
 }
 
-// Adds the partial sums that workgroups w0 .. w1 left for one pair, in their order, and finishes the pair.  Every thread
-// takes quads of consecutive d; two halves of the workgroup take the even and the odd partials when there are few quads.
+// Sums of one stretch of positions over the 16 query heads: what a workgroup has in LDS, what it leaves in the workspace and
+// what comes of adding those.
+template <int DP>
+struct Sums {
+    static constexpr int QPR = DP / 4;                           // quads of consecutive d in a row
+    static constexpr int RP = (DP > 128 ? DP : 128) + 4;         // row pitch, 4 words past a bank cycle
+    float (*row)[RP];
+    float (*ml)[2];                                              // maximum, sum of probabilities
+    __device__ __forceinline__ f32x4 &quad(int r, int d) const { return *reinterpret_cast<f32x4 *>(&row[r][d]); }
+};
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_of(Args a) { return make_rsrc(a->part, a->part_bytes); }
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_ml_of(Args a) { return make_rsrc(a->part_ml, a->part_ml_bytes); }
+
+// Leaves the sums in the workspace, as those of cut piece `place`, written through to where every XCD sees them.
+template <int DP>
+__device__ void publish(Args a, const Sums<DP> &own, uint32_t place, int rows)
+{
+    const __amdgpu_buffer_rsrc_t part = part_of(a);
+    const int thread = thread_now();
+    for (int e = thread; e < rows * (DP / 4); e += 256) {
+        const int r = e / (DP / 4), d = (e % (DP / 4)) * 4;
+        buffer_store_b128<kSC1>(__builtin_bit_cast(u32x4, own.quad(r, d)), part, ((place * (uint32_t)a->rows + r) * DP + d) * 4, 0);
+    }
+    if (thread < rows) {
+        const u32x2 w = {__float_as_uint(own.ml[thread][0]), __float_as_uint(own.ml[thread][1])};
+        __builtin_amdgcn_raw_buffer_store_b64(w, part_ml_of(a), (place * kHeads + thread) * 8, 0, kSC1);
+    }
+}
 template <int DP, int QT>
-__device__ void join(Args a, int b, int head0, int rows, int w0, int w1, bool first_at_0, float shift, float (*lds)[4])
+__device__ void finish(Args a, const Sums<DP> &own, int64_t out_row, int rows, float shift)
+{
+    const int thread = thread_now();
+    for (int e = thread; e < rows * (DP / 4); e += 256) {
+        const int r = e / (DP / 4), d = (e % (DP / 4)) * 4;
+        const float l = own.ml[r][1], inv = l == 0.0f ? 0.0f : 1.0f / l;
+        store_out<QT>(a, out_row + r, d, own.quad(r, d) * inv);
+    }
+    if (thread < rows) store_lse(a, out_row + thread, own.ml[thread][0], own.ml[thread][1], shift);
+}
+
+// Over the 16 lanes of a row of lanes, in all of them.
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float v, float outside)
+{
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)__float_as_uint(outside), (int)__float_as_uint(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float row_max(float v)
+{
+    v = fmaxf(v, from_lane<0x111>(v, -INFINITY));                // row_shr:1, 2, 4, 8: the last lane has it
+    v = fmaxf(v, from_lane<0x112>(v, -INFINITY));
+    v = fmaxf(v, from_lane<0x114>(v, -INFINITY));
+    v = fmaxf(v, from_lane<0x118>(v, -INFINITY));
+    return __shfl(v, 15, 16);
+}
+__device__ __forceinline__ float row_sum(float v)
+{
+    v += from_lane<0x111>(v, 0.0f);
+    v += from_lane<0x112>(v, 0.0f);
+    v += from_lane<0x114>(v, 0.0f);
+    v += from_lane<0x118>(v, 0.0f);
+    return __shfl(v, 15, 16);
+}
+
+// Adds the sums of n cut pieces, first, first + step, ..., in this order, into `own`, which already holds those of number
+// `mine`.  A thread adds one quad, eight partials in flight; where there are fewer quads than threads, several share the
+// partials of a quad.  What the partials weigh is worked out meanwhile, 16 lanes to a head.
+constexpr int kFlight = 8;
+constexpr int kJoin = 64;                                        // sums of one call at most
+constexpr size_t kJoinLds = (kJoin * kHeads + 256 * 4) * sizeof(float);
+template <int DP>
+__device__ void join(Args a, const Sums<DP> &own, int mine, uint32_t first, uint32_t step, int n, int rows, float *lds)
 {
     constexpr int QPR = DP / 4;
-    const __amdgpu_buffer_rsrc_t part = make_rsrc(a->part, a->part_bytes);
-    const __amdgpu_buffer_rsrc_t mls = make_rsrc(a->part_ml, (uint32_t)a->workgroups * 2 * kHeads * 2 * 4);
     const int thread = thread_now();
-    for (int e0 = 0; e0 < rows * QPR; e0 += 128) {
-        const int e = e0 + (thread & 127), row = min(e / QPR, rows - 1), d = (e % QPR) * 4, odd = thread >> 7;
-        float m = -INFINITY, l = 0.0f;
+    const uint32_t row_bytes = DP * 4, place_bytes = (uint32_t)a->rows * row_bytes;
+    const auto place = [&](int i) { return first + (uint32_t)i * step; };
+    // ends with the last of them: a request for number n or a later one reads zeros
+    const __amdgpu_buffer_rsrc_t part = make_rsrc(a->part, uniform((place(n - 1) + 1) * place_bytes));
+    const __amdgpu_buffer_rsrc_t mls = make_rsrc(a->part_ml, uniform((place(n - 1) + 1) * kHeads * 8));
+    float(*weight)[kHeads] = reinterpret_cast<float(*)[kHeads]>(lds);
+    f32x4 *shared = reinterpret_cast<f32x4 *>(lds + kJoin * kHeads);
+    int threads = QPR;                                           // of all quads, a power of two
+    while (threads < rows * QPR && threads < 256) threads *= 2;
+    const int split = 256 / threads, part_no = thread / threads;
+#pragma unroll 1
+    for (int e0 = 0; e0 < rows * QPR; e0 += threads) {
+        const int e = e0 + (thread & (threads - 1)), row = min(e / QPR, rows - 1), d = (e % QPR) * 4;
+        f32x4 v[kFlight];
+        const auto request = [&](int i0) {
+            const uint32_t from = (uint32_t)row * row_bytes + d * 4;
+#pragma unroll
+            for (int k = 0; k < kFlight; k++)
+                v[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, place(i0 + k * split) * place_bytes + from, 0, kSC1));
+        };
+        request(part_no);
+        if (e0 == 0) {
+            const int r = thread / 16, lane = thread % 16;
+            float m[kJoin / 16], l[kJoin / 16], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kJoin / 16; k++) {
+                const int i = lane + 16 * k;
+                const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(mls, (place(i) * kHeads + r) * 8, 0, kSC1);
+                m[k] = i < n ? __uint_as_float(w.x) : -INFINITY, l[k] = __uint_as_float(w.y);
+                if (i == mine) m[k] = own.ml[r][0], l[k] = own.ml[r][1];
+                top = fmaxf(top, m[k]);
+            }
+            top = row_max(top);
+#pragma unroll
+            for (int k = 0; k < kJoin / 16; k++) {
+                const float f = weight_of(m[k], top);
+                weight[lane + 16 * k][r] = f;                    // 0 behind the last one
+                sum += l[k] * f;
+            }
+            sum = row_sum(sum);
+            if (lane == 0) own.ml[r][0] = top, own.ml[r][1] = sum;          // (this row's lanes have read it)
+            __syncthreads();
+        }
+        const f32x4 here = own.quad(row, d);
         f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int w = w0 + odd; w <= w1; w += 16) {
-            f32x4 v[8];
-            u32x2 ml[8];
+#pragma unroll 1
+        for (int i0 = part_no; i0 < n; i0 += kFlight * split) {
+            if (i0 != part_no) request(i0);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {                        // eight in flight; past the end they read zeros
-                const int wi = w + 2 * i;
-                const uint32_t at = (uint32_t)wi * 2 + (wi > w0 || first_at_0 ? 0 : 1);
-                const uint32_t po = (at * (uint32_t)a->rows + row) * (DP * 4) + d * 4, mo = (at * kHeads + row) * 8;
-                v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, wi <= w1 ? po : kOutOfRange, 0, kSC1));
-                ml[i] = __builtin_amdgcn_raw_buffer_load_b64(mls, wi <= w1 ? mo : kOutOfRange, 0, kSC1);
-            }
-            float top = m;
+            for (int k = 0; k < kFlight; k++) {
+                const int i = i0 + k * split;
+                const float f = weight[min(i, kJoin - 1)][row];
 #pragma unroll
-            for (int i = 0; i < 8; i++) top = w + 2 * i <= w1 ? fmaxf(top, __uint_as_float(ml[i].x)) : top;
-            const float f = weight_of(m, top);
-            m = top;
-            l *= f;
-            sum *= f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if (w + 2 * i > w1) break;
-                const float fi = weight_of(__uint_as_float(ml[i].x), top);
-                l += __uint_as_float(ml[i].y) * fi;
-                sum += v[i] * fi;
+                for (int c = 0; c < 4; c++) sum[c] = __builtin_fmaf(i == mine ? here[c] : v[k][c], f, sum[c]);
             }
         }
-        __syncthreads();
-        if (odd) {
-            const int t = thread & 127;
-            lds[2 * t][0] = m, lds[2 * t][1] = l;
-            *reinterpret_cast<f32x4 *>(lds[2 * t + 1]) = sum;
+        if (split > 1) {                                         // (one round: every quad has its threads)
+            shared[thread] = sum;
+            __syncthreads();
+            if (part_no) continue;
+            for (int k = 1; k < split; k++) sum += shared[thread + k * threads];
         }
-        __syncthreads();
-        if (odd || e >= rows * QPR) continue;
-        const int t = thread;
-        const float top = fmaxf(m, lds[2 * t][0]), f0 = weight_of(m, top), f1 = weight_of(lds[2 * t][0], top);
-        l = l * f0 + lds[2 * t][1] * f1;
-        sum = sum * f0 + *reinterpret_cast<const f32x4 *>(lds[2 * t + 1]) * f1;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        store_out<QT>(a, (int64_t)b * a->heads + head0 + row, d, sum * inv);
-        if (d == 0) store_lse(a, (int64_t)b * a->heads + head0 + row, top, l, shift);
+        if (e < rows * QPR) own.quad(row, d) = sum;
     }
+    __syncthreads();
+}
+
+// Says that this workgroup's sums are in the workspace; true for the last of `n` to say so.  The counter is 0 again then.
+__device__ __forceinline__ bool arrive(Global<uint32_t> *counter, int n, int *lds)
+{
+    wait_vmcnt<0>();                                             // they have reached the coherence point
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t old = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *lds = old == (uint32_t)(n - 1);
+        if (*lds) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);     // for the next launch
+    }
+    __syncthreads();
+    return uniform(*lds) != 0;
 }
 
 template <int DP, bool QUANT, int QT, Addressing AD>
 __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void paged_decode_kernel(AttnArgs)
 {
     using W = Decode<DP, QUANT, QT, AD>;
-    constexpr int RP = 128 + 4;                                  // row pitch of the sums in LDS, 4 words past a bank cycle
+    constexpr int RP = 128 + 4;                                  // row pitch of a wavefront's sums in LDS
     __shared__ float red[4][kHeads][RP];
     __shared__ float ml[4][kHeads][2];
+    __shared__ float all_wide[W::NP > 1 ? kHeads : 1][Sums<DP>::RP];     // the workgroup's sums: the first wavefront's place, if they fit
+    __shared__ float all_ml[kHeads][2];
+    __shared__ int counted[2];
+    static_assert(W::NP > 1 || Sums<DP>::RP == RP, "the workgroup's sums lie where a wavefront's were");
+    static_assert(sizeof(red) - sizeof(red[0]) >= kJoinLds, "join works behind the workgroup's sums");
     __shared__ int last_here;
 
-    uint32_t x, x_begin, x_end, share;                           // all units are fewer than 2^31 - workgroups: the host checks
-    int b = 0, pair = 0, unit = 0;
-    {
+    const Pieces pieces = [] {
         const Args a = args_now();
-        const Numbering n(a);
-        const uint32_t all = n.total * (uint32_t)a->pairs;
-        share = divide(all + a->workgroups - 1, a->by_workgroups);
-        x = x_begin = min(blockIdx.x * share, all);
-        x_end = min(x + share, all);
-        if (x < x_end) {
-            uint32_t before, units;
-            n.find(a, divide(x, a->by_pairs), b, before, units);
-            const uint32_t in = x - before * (uint32_t)a->pairs;
-            pair = (int)(in / units);
-            unit = (int)(in - pair * units);
-        }
-    }
+        uint32_t lines = 0;                                      // the arguments' cache lines, for the phases that follow
+#pragma unroll
+        for (size_t i = 0; i < sizeof(AttnArgs); i += 64) lines |= *(const __attribute__((address_space(4))) uint32_t *)((const __attribute__((address_space(4))) char *)a + i);
+        const Pieces p(a);
+        asm volatile("" ::"s"(lines));
+        return p;
+    }();
+    const uint32_t all_pieces = uniform(pieces.total * (uint32_t)args_now()->pairs);
 
-    while (x < x_end) {
-        int head0, rows, units, last;
+    for (uint32_t piece = blockIdx.x; piece < all_pieces; piece += gridDim.x) {
+        int b, head0, rows, n, number;                           // piece `number` of the pair's n
+        uint32_t first_cut;                                      // the pair's first cut piece
         float l, m;
         f32x4 acc[W::NP][W::PE];
         {
-            W w(args_now());
-            b = uniform(b), pair = uniform(pair), unit = uniform(unit);
-            int len = clamp_len(w.a, scalar_load(w.a->lens + b));
-            while (len == 0) len = clamp_len(w.a, scalar_load(w.a->lens + ++b));     // the next sequence that has positions
-            const int halves = (int)halves_of(w.a, len);
-            units = (halves + kUnit - 1) / kUnit;
-            last = min(units, unit + (int)(x_end - x));      // units [unit, last) of this pair
-            const int kvh = pair / w.a->tiles;
-            head0 = kvh * w.a->group + (pair % w.a->tiles) * kHeads;
-            rows = min(kHeads, (kvh + 1) * w.a->group - head0);
-            last = uniform(last);
-            w.start(b, kvh, head0, rows, len, min(halves, last * kUnit));
-            w.run(unit * (kUnit / 2) + w.wave, last * (kUnit / 2), head0, rows);
+            const Args a = args_now();
+            W w(a);
+            int len;
+            uint32_t count, before, cut_before;
+            pieces.find(a, divide(piece, a->by_pairs), b, len, count, before, cut_before);
+            b = uniform(b), len = uniform(len), n = uniform((int)count);
+            const uint32_t in = piece - before * (uint32_t)a->pairs, pair = uniform(in / count);
+            number = uniform((int)(in - pair * count));
+            first_cut = cut_before * (uint32_t)a->pairs + pair * count;
+            const int kvh = (int)pair / a->tiles, halves = (int)halves_of(a, len), units = (halves + kUnit - 1) / kUnit;
+            head0 = kvh * a->group + ((int)pair - kvh * a->tiles) * kHeads;
+            rows = min(kHeads, (kvh + 1) * a->group - head0);
+            // the first units % n pieces have one more unit
+            const int each = uniform(units / n), more = units - each * n;
+            const int unit = number * each + min(number, more), end = unit + each + (number < more ? 1 : 0);
+            w.start(b, kvh, head0, rows, len, min(halves, end * kUnit));
+            w.run(unit * (kUnit / 2) + w.wave, end * (kUnit / 2), head0, rows);
             l = w.l, m = w.m;
 #pragma unroll
             for (int h = 0; h < W::NP; h++)
@@ -686,18 +807,38 @@ __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void paged_decode_kernel(At
                 for (int i = 0; i < W::PE; i++) acc[h][i] = w.acc[h][i];
         }
 
-        // the four wavefronts' sums on a common maximum
         const Args a = args_now();
+        const int64_t out_row = (int64_t)b * a->heads + head0;
+        Global<uint32_t> *arrived = at(a->arrived);
+        // Of a pair that is cut, the last of its workgroups to arrive adds everybody's sums.  Where those are more than some
+        // hundred kilobytes, groups of about the root of their number are added first, so that no workgroup has many to read.  The
+        // counter of a group is its first piece's, that of the groups lies behind all of these.
+        int size = n;
+        if (n >= kJoin || n * rows * (DP / 4) > 512 * kFlight) {
+            size = 8;
+            while (size * size < n) size += 4;
+        }
+        const int group = number / size, groups = (n + size - 1) / size, members = min(size, n - group * size);
+        const uint32_t first = first_cut + group * size, behind = 2 * (uint32_t)a->shares;
+        uint32_t seen = 0;                                       // how many have arrived: requested here, looked at behind what follows
+        if (n > 1 && threadIdx.x < 2)
+            seen = __hip_atomic_load(arrived + (threadIdx.x ? behind + first_cut : first), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+
+        // the four wavefronts' sums on a common maximum
         const int thread = thread_now(), lane = thread & 63, wave = thread >> 6, col = lane & 15, g = lane >> 4;
+        const Sums<DP> own = {W::NP > 1 ? all_wide : reinterpret_cast<float (*)[Sums<DP>::RP]>(red[0]), all_ml};
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (g == 0) ml[wave][col][0] = m, ml[wave][col][1] = l;
         __syncthreads();
         const float top = fmaxf(fmaxf(ml[0][col][0], ml[1][col][0]), fmaxf(ml[2][col][0], ml[3][col][0]));
         const float f = weight_of(m, top);
-        const bool whole = unit == 0 && last == units;
-        const int slot = x == x_begin ? 0 : 1;
-        const uint32_t part_at = (blockIdx.x * 2 + slot) * (uint32_t)a->rows;
+        if (thread < kHeads) {
+            float total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) total += ml[i][col][1] * weight_of(ml[i][col][0], top);
+            all_ml[col][0] = top, all_ml[col][1] = total;
+        }
 #pragma unroll
         for (int h = 0; h < W::NP; h++) {
             if (h) __syncthreads();
@@ -714,53 +855,35 @@ __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void paged_decode_kernel(At
                 f32x4 sum = *reinterpret_cast<const f32x4 *>(&red[0][row][d]);
 #pragma unroll
                 for (int i = 1; i < 4; i++) sum += *reinterpret_cast<const f32x4 *>(&red[i][row][d]);
-                if (whole) {
-                    const float rt = fmaxf(fmaxf(ml[0][row][0], ml[1][row][0]), fmaxf(ml[2][row][0], ml[3][row][0]));
-                    float total = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) total += ml[i][row][1] * weight_of(ml[i][row][0], rt);
-                    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-                    store_out<QT>(a, (int64_t)b * a->heads + head0 + row, h * 128 + d, sum * inv);
-                } else {
-                    const __amdgpu_buffer_rsrc_t part = make_rsrc(a->part, a->part_bytes);
-                    buffer_store_b128<kSC1>(__builtin_bit_cast(u32x4, sum), part, ((part_at + row) * DP + h * 128 + d) * 4, 0);
-                }
+                own.quad(row, h * 128 + d) = sum;
             }
         }
-        if (wave == 0 && g == 0 && col < rows) {
-            float total = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) total += ml[i][col][1] * weight_of(ml[i][col][0], top);
-            if (whole) {
-                store_lse(a, (int64_t)b * a->heads + head0 + col, top, total, W::kShift);
-            } else {
-                const __amdgpu_buffer_rsrc_t mls = make_rsrc(a->part_ml, (uint32_t)a->workgroups * 2 * kHeads * 2 * 4);
-                const u32x2 two = {__float_as_uint(top), __float_as_uint(total)};
-                __builtin_amdgcn_raw_buffer_store_b64(two, mls, ((blockIdx.x * 2 + slot) * kHeads + col) * 8, 0, kSC1);
+        if (thread < 2) counted[thread] = (int)seen;
+        __syncthreads();
+
+        bool done = true;
+        const auto last_of = [&](Global<uint32_t> *counter, int of, int seen, uint32_t place) {
+            if (of == 1) return true;
+            if (seen == of - 1) {                                // everybody else was there already: nobody waits for these sums
+                if (thread == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                return true;
             }
+            publish<DP>(a, own, place, rows);
+            return arrive(counter, of, &last_here);
+        };
+        const int seen0 = uniform(counted[0]), seen1 = uniform(counted[1]);
+#pragma unroll 1
+        for (int level = 0; level < 2 && done; level++) {        // within the group, among the groups
+            const int of = level ? groups : members;
+            done = last_of(arrived + (level ? behind + first_cut : first), of, level ? seen1 : seen0, first + (level ? 0 : number - group * size));
+            if (done && of > 1)
+                join<DP>(a, own, level ? group : number - group * size, level ? first_cut : first, level ? (uint32_t)size : 1u, of, rows, &red[1][0][0]);
         }
-        if (!whole) {
-            // the last of the pair's workgroups to arrive adds everybody's sums; the first one's counter counts them
-            const uint32_t x0 = x - unit;
-            const int w0 = (int)(x0 / share), w1 = (int)((x0 + units - 1) / share);
-            wait_vmcnt<0>();                                     // this wavefront's sums have reached the coherence point
-            __syncthreads();
-            if (thread == 0) {
-                const uint32_t old = __hip_atomic_fetch_add(at(a->arrived) + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                last_here = old == (uint32_t)(w1 - w0);
-                if (last_here) __hip_atomic_store(at(a->arrived) + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);     // for the next launch
-            }
-            __syncthreads();
-            if (last_here)
-                join<DP, QT>(args_now(), b, head0, rows, w0, w1, w0 * share == x0, W::kShift, reinterpret_cast<float (*)[4]>(&red[0][0][0]));
-        }
+        if (done) finish<DP, QT>(args_now(), own, out_row, rows, W::kShift);
         __syncthreads();                                         // ml and red are free again
-        x += last - unit;
-        unit = 0;
-        if (last == units && ++pair == a->pairs) pair = 0, b++;
     }
 
-    // sequences without positions
+    if (!pieces.empty) return;
     const Args a = args_now();
     for (int e = blockIdx.x; e < a->batch; e += gridDim.x) {
         if (clamp_len(a, scalar_load(a->lens + e)) != 0) continue;
@@ -793,9 +916,9 @@ __global__ __launch_bounds__(256) void paged_sums_kernel(AttnArgs a)
 }
 
 struct AttnSizes {
-    int64_t rows, tiles, pairs, units, workgroups, dp, score_pitch;
+    int64_t rows, tiles, pairs, units, shares, workgroups, dp, score_pitch;
     size_t part, part_ml, lse2, scores, bytes;                    // offsets in the workspace, and its size
-    uint32_t part_bytes;
+    uint32_t part_bytes, part_ml_bytes;
 };
 
 constexpr size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -816,25 +939,31 @@ bool plan_attention(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head
     p->units = (halves + kUnit - 1) / kUnit;
     if (batch * p->pairs > 0x7ffff000 / p->units) return false;
     p->dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-    p->workgroups = kNumCU * (p->dp == 256 ? 2 : 3);              // as many as the card holds at once
-    if (batch * p->units * p->pairs < p->workgroups) p->workgroups = batch * p->units * p->pairs;
+    // Pieces: as many as the card holds workgroups at once, and up to one more for every pair, whose last piece is smaller.
+    p->shares = kNumCU * (p->dp == 256 ? 2 : 3); if (const char *e = getenv("PW")) p->shares = atoi(e);
+    const int64_t pieces = batch * p->pairs * p->units < p->shares ? batch * p->pairs * p->units : p->shares + batch * p->pairs;
+    p->workgroups = pieces < 2048 ? pieces : 2048;
     p->score_pitch = (capacity + 3) / 4 * 4;
     size_t at = MI355_WORKSPACE_ZERO_BYTES;                       // the arrival counters lie at its start
     const auto take = [&](size_t bytes) { const size_t o = at; at += round256(bytes); return o; };
-    p->part_bytes = (uint32_t)(p->workgroups * 2 * p->rows * p->dp * 4);
+    // of pairs that are cut there are fewer than twice as many pieces as shares: a pair of u units, u more than a share of s, has
+    // fewer than u / s + 1 < 2 u / s
+    p->part_bytes = (uint32_t)(p->shares * 2 * p->rows * p->dp * 4);
+    p->part_ml_bytes = (uint32_t)(p->shares * 2 * kHeads * 2 * 4);
     p->part = take(p->part_bytes);
-    p->part_ml = take((size_t)(p->workgroups * 2 * kHeads * 2) * 4);
+    p->part_ml = take(p->part_ml_bytes);
     p->lse2 = take(sums ? (size_t)(batch * heads) * 4 : 0);
     p->scores = take(sums ? (size_t)(batch * heads) * (size_t)p->score_pitch * 4 : 0);
     p->bytes = at;
     return true;
 }
-static_assert(kNumCU * 3 * sizeof(uint32_t) <= kWorkspaceCounterBytes, "arrival counters");
+static_assert(kNumCU * 3 * 4 * sizeof(uint32_t) <= kWorkspaceCounterBytes, "arrival counters");
+static_assert(kNumCU * 3 <= (kJoin / 2) * (kJoin / 2), "groups of pieces, and members of a group");
 
 template <int DP, bool QUANT, int QT>
-void launch_attention(const AttnArgs &a, Addressing ad, hipStream_t s)
+void launch_attention(const AttnArgs &a, Addressing ad, unsigned workgroups, hipStream_t s)
 {
-    const dim3 grid(a.workgroups), block(256);
+    const dim3 grid(workgroups), block(256);
     if (ad == kRows) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kRows>), grid, block, 0, s, a);
     else if (QUANT && ad == kBlockScales) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, QUANT ? kBlockScales : kBlock>), grid, block, 0, s, a);
     else if (ad == kBlockMask) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlockMask>), grid, block, 0, s, a);
@@ -842,14 +971,14 @@ void launch_attention(const AttnArgs &a, Addressing ad, hipStream_t s)
 }
 
 template <int DP>
-void launch_attention(const AttnArgs &a, bool quant, bool fp16, Addressing ad, hipStream_t s)
+void launch_attention(const AttnArgs &a, bool quant, bool fp16, Addressing ad, unsigned workgroups, hipStream_t s)
 {
     if (quant) {
-        if (fp16) launch_attention<DP, true, 1>(a, ad, s);
-        else launch_attention<DP, true, 0>(a, ad, s);
+        if (fp16) launch_attention<DP, true, 1>(a, ad, workgroups, s);
+        else launch_attention<DP, true, 0>(a, ad, workgroups, s);
     } else {
-        if (fp16) launch_attention<DP, false, 1>(a, ad, s);
-        else launch_attention<DP, false, 0>(a, ad, s);
+        if (fp16) launch_attention<DP, false, 1>(a, ad, workgroups, s);
+        else launch_attention<DP, false, 0>(a, ad, workgroups, s);
     }
 }
 
@@ -912,12 +1041,13 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     a.rows = (int)p.rows;
     a.tiles = (int)p.tiles;
     a.pairs = (int)p.pairs;
-    a.workgroups = (int)p.workgroups;
+    a.shares = (int)p.shares;
     a.by_pairs = fast_div((uint32_t)p.pairs);
-    a.by_workgroups = fast_div((uint32_t)p.workgroups);
+    a.by_shares = fast_div((uint32_t)p.shares);
     a.capacity = (int)(max_blocks * cache->block_size);
     a.max_blocks = (int)max_blocks;
     a.part_bytes = p.part_bytes;
+    a.part_ml_bytes = p.part_ml_bytes;
     a.scale2 = scale * kLog2e;
     const int es = quant ? 1 : 2;
     // pieces of 16 bytes: rows on 16-byte boundaries, and no piece reaching past a row's end
@@ -935,9 +1065,9 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     a.span = ad != kRows ? a.cache.page : fast_div(kHalf);
     a.halves = fast_div((a.span.d + kHalf - 1) / kHalf);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (p.dp == 64) launch_attention<64>(a, quant, fp16, ad, s);
-    else if (p.dp == 128) launch_attention<128>(a, quant, fp16, ad, s);
-    else launch_attention<256>(a, quant, fp16, ad, s);
+    if (p.dp == 64) launch_attention<64>(a, quant, fp16, ad, (unsigned)p.workgroups, s);
+    else if (p.dp == 128) launch_attention<128>(a, quant, fp16, ad, (unsigned)p.workgroups, s);
+    else launch_attention<256>(a, quant, fp16, ad, (unsigned)p.workgroups, s);
     if (attn_sums && a.capacity > 0) {
         const int64_t chunks = (a.capacity + 1023) / 1024;
         for (int64_t b0 = 0; b0 < batch; b0 += 65535) {           // a grid's third dimension has 16 bits
