@@ -195,13 +195,24 @@ __device__ __forceinline__ void buffer_load(uint32_t (&to)[W], __amdgpu_buffer_r
     }
 }
 
+// Over the four lanes that differ in their group of 16, in all of them: exchanges of neighbouring groups, then of halves.
+template <class Op>
+__device__ __forceinline__ float over_groups(float v, Op op)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
+
 // How the rows of half a tile are addressed.
 //   kRows   lane by lane: any block size, stride, width and alignment
 //   kBlock  the half lies in one block: a scalar descriptor that ends with the half's last row, constant lane offsets; rows in
 //           16-byte pieces.  Rows behind the end read as zero without traffic, so the loop needs no edge code.
-//   kBlockScales  the same, and (int8) the scales of four tokens of a head are 16 aligned bytes
+//   kBlockAlike  as kBlock; keys and values lie alike, so that one offset serves both - the loop has half the scalar
+//           instructions -, and so do the scales (int8), those of four tokens of a head in 16 aligned bytes
 //   kBlockMask  as kBlock, with a mask, whose bytes are read four at a time
-enum Addressing { kRows, kBlock, kBlockScales, kBlockMask };
+enum Addressing { kRows, kBlock, kBlockAlike, kBlockMask };
 
 // DP: head_dim rounded up to 64, 128 or 256.  QT: type of q and out (0 bf16, 1 fp16).
 template <int DP, bool QUANT, int QT, Addressing AD>
@@ -235,7 +246,9 @@ struct Decode {
     // of the pair that is being worked on
     int b, kvh, len, half_end;
     const int32_t *table;
-    const char *kbase, *vbase;
+    const char *kbase, *vbase, *ksbase, *vsbase;
+    uint64_t start[2], scale_start[2];                           // kBlockAlike: of the tile whose keys were requested last
+    uint32_t reach[2];
 
     __device__ explicit Decode(Args args)
         : Decode(args, thread_now())
@@ -273,12 +286,13 @@ struct Decode {
     // first d of the lane's key piece c; an int8 piece serves the chunks 2c and 2c + 1
     __device__ __forceinline__ int first_d(int c) const { return QUANT ? c * 64 + g * 16 : c * 32 + g * 8; }
 
-    __device__ __forceinline__ void start(int b_, int kvh_, int head0, int rows, int len_, int half_end_)
+    __device__ __forceinline__ void begin(int b_, int kvh_, int head0, int rows, int len_, int half_end_)
     {
         b = b_, kvh = kvh_, len = len_, half_end = half_end_;
         table = a->table + b * a->table_stride;
         kbase = a->cache.key.base + kvh * a->cache.key.head;
         vbase = a->cache.value.base + kvh * a->cache.value.head;
+        if constexpr (QUANT) ksbase = a->cache.key_scale.base + kvh * a->cache.key_scale.head, vsbase = a->cache.value_scale.base + kvh * a->cache.value_scale.head;
         const uint16_t *row = a->q + b * a->q_batch + (head0 + min(col, rows - 1)) * a->q_head;
 #pragma unroll
         for (int c = 0; c < NCH; c++) {
@@ -318,11 +332,22 @@ struct Decode {
                 if ((uint32_t)p.id[s] >= (uint32_t)a->cache.num_blocks) p.n[s] = 0, p.id[s] = 0;
         }
     }
+    // where half s begins within an array, and how far its rows reach
+    __device__ __forceinline__ uint64_t start_of(ArgArray &x, const Place &p, int s) const
+    {
+        return (uint64_t)(uint32_t)p.id[s] * (uint32_t)x.block + p.off[s] * (uint32_t)x.token;
+    }
+    __device__ __forceinline__ uint32_t reach_of(ArgArray &x, const Place &p, int s, int row_bytes) const
+    {
+        return uniform(p.n[s] > 0 ? (uint32_t)(p.n[s] - 1) * (uint32_t)x.token + row_bytes : 0);
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char *base, uint64_t start, uint32_t reach) const
+    {
+        return make_rsrc((const char *)uniform((int64_t)((uint64_t)base + start)), reach);
+    }
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char *base, ArgArray &x, const Place &p, int s, int row_bytes) const
     {
-        const uint64_t block = (uint64_t)(uint32_t)p.id[s] * (uint32_t)x.block, first = (uint64_t)base + block + p.off[s] * (uint32_t)x.token;
-        const uint32_t bytes = p.n[s] > 0 ? (uint32_t)(p.n[s] - 1) * (uint32_t)x.token + row_bytes : 0;
-        return make_rsrc((const char *)uniform((int64_t)first), uniform(bytes));
+        return rows_at(base, start_of(x, p, s), reach_of(x, p, s, row_bytes));
     }
     // positions of the tile, their keys, key scales and mask bytes
     __device__ __forceinline__ void load_keys(const Place &p)
@@ -330,10 +355,14 @@ struct Decode {
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             if constexpr (AD != kRows) {
-                const __amdgpu_buffer_rsrc_t r = rows_of(kbase, a->cache.key, p, s, D * ES);
+                if constexpr (AD == kBlockAlike) {
+                    start[s] = start_of(a->cache.key, p, s), reach[s] = reach_of(a->cache.key, p, s, D * ES);
+                    if constexpr (QUANT) scale_start[s] = start_of(a->cache.key_scale, p, s);
+                }
+                const __amdgpu_buffer_rsrc_t r = AD == kBlockAlike ? rows_at(kbase, start[s], reach[s]) : rows_of(kbase, a->cache.key, p, s, D * ES);
 #pragma unroll
                 for (int c = 0; c < KL; c++) buffer_load<4>(k[s][c], r, koff[c]);
-                if constexpr (QUANT) load_scales(ks[s], a->cache.key_scale, p, s, soff[0]);
+                if constexpr (QUANT) load_scales(ks[s], ksbase, a->cache.key_scale, p, s, soff[0]);
             } else {
                 const int key = p.key[s] + col;
                 const uint32_t block = divide((uint32_t)key, a->cache.page);
@@ -357,10 +386,11 @@ struct Decode {
             }
         }
     }
-    __device__ __forceinline__ void load_scales(float (&to)[4], ArgArray &x, const Place &p, int s, const uint32_t (&off)[4]) const
+    __device__ __forceinline__ void load_scales(float (&to)[4], const char *base, ArgArray &x, const Place &p, int s, const uint32_t (&off)[4]) const
     {
-        const __amdgpu_buffer_rsrc_t r = rows_of(x.base + kvh * x.head, x, p, s, 4);
-        if constexpr (AD == kBlockScales) {
+        // (alike: the four scales of a lane group, or none; of those behind the end nothing is used)
+        const __amdgpu_buffer_rsrc_t r = AD == kBlockAlike ? rows_at(base, scale_start[s], (uint32_t)(p.n[s] + 3 & ~3) * 4) : rows_of(base, x, p, s, 4);
+        if constexpr (AD == kBlockAlike) {
             const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(r, g * 16, 0, 0);
 #pragma unroll
             for (int i = 0; i < 4; i++) to[i] = __uint_as_float(w[i]);
@@ -374,12 +404,12 @@ struct Decode {
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             if constexpr (AD != kRows) {
-                const __amdgpu_buffer_rsrc_t r = rows_of(vbase, a->cache.value, p, s, D * ES);
+                const __amdgpu_buffer_rsrc_t r = AD == kBlockAlike ? rows_at(vbase, start[s], reach[s]) : rows_of(vbase, a->cache.value, p, s, D * ES);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
                     for (int h = 0; h < NP; h++) buffer_load<VW>(v[s][j][h], r, voff[j][h]);
-                if constexpr (QUANT) load_scales(vs[s], a->cache.value_scale, p, s, soff[1]);
+                if constexpr (QUANT) load_scales(vs[s], vsbase, a->cache.value_scale, p, s, soff[1]);
             } else {
                 const int64_t mine = lane_slot[s] == ~0u ? -1 : offset(a->cache.value, lane_slot[s]);
                 if constexpr (QUANT) {
@@ -447,11 +477,17 @@ struct Decode {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 z[s][r] = QUANT ? z[s][r] * (a->scale2 * ks[s][r]) : z[s][r] * a->scale2;
-                if (!full(p)) z[s][r] = (valid >> (4 * s + r)) & 1 ? z[s][r] : -INFINITY;
             }
+        if (!full(p)) {
+            no_select();
+#pragma unroll
+            for (int i = 0; i < 8; i++) z[i / 4][i % 4] = (valid >> i) & 1 ? z[i / 4][i % 4] : -INFINITY;
+        }
     }
+    // keeps a uniform branch a branch: the edge cases would cost selects in every tile
+    __device__ static __forceinline__ void no_select() { asm volatile(""); }
     // every position of the tile is seen, known without a look at the lanes
-    __device__ __forceinline__ bool full(const Place &p) const { return (AD == kBlock || AD == kBlockScales) && p.n[0] + p.n[1] == 2 * kHalf; }
+    __device__ __forceinline__ bool full(const Place &p) const { return (AD == kBlock || AD == kBlockAlike) && p.n[0] + p.n[1] == 2 * kHalf; }
     __device__ __forceinline__ void store_scores(const Place &p, const f32x4 (&z)[2], int head0, int rows) const
     {
         if (col >= rows) return;
@@ -474,8 +510,7 @@ struct Decode {
     __device__ __forceinline__ void add(const Place &place, uint32_t valid, const f32x4 (&z)[2], u32x4 &ph, u32x4 &pl)
     {
         float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])), fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
         if (__any(top > m)) {
             const float higher = fmaxf(m, top), f = weight_of(m, higher);
             m = higher;
@@ -494,17 +529,17 @@ struct Decode {
         }
         if constexpr (QUANT) {
             // probabilities times value scales in two bf16 terms: 16 significant bits of any magnitude
-            float hi[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                p[i] = p[i] * vs[i / 4][i % 4];
-                if (!full(place)) p[i] = (valid >> i) & 1 ? p[i] : 0.0f;
-                hi[i] = bf16_1(f32_to_bf16(p[i]));
+            for (int i = 0; i < 8; i++) p[i] = p[i] * vs[i / 4][i % 4];
+            if (!full(place)) {                                  // (a scale that is not seen may be anything)
+                no_select();
+#pragma unroll
+                for (int i = 0; i < 8; i++) p[i] = (valid >> i) & 1 ? p[i] : 0.0f;
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                ph[i] = pack_bf16x2(hi[2 * i], hi[2 * i + 1]);
-                pl[i] = pack_bf16x2(p[2 * i] - hi[2 * i], p[2 * i + 1] - hi[2 * i + 1]);
+                ph[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
+                pl[i] = pack_bf16x2(p[2 * i] - bf16_lo(ph[i]), p[2 * i + 1] - bf16_hi(ph[i]));
             }
         } else {
 #pragma unroll
@@ -556,7 +591,11 @@ struct Decode {
         __builtin_amdgcn_sched_barrier(0);
         Place next = place(tile + 4);
         for (; tile < tile_end; tile += 4) {
-            const uint32_t valid = seen(cur);
+            uint32_t valid = 0xff;
+            if (!full(cur)) {
+                no_select();
+                valid = seen(cur);
+            }
             f32x4 z[2];
             score(cur, valid, z);
             if (a->scores) store_scores(cur, z, head0, rows);
@@ -789,16 +828,16 @@ __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void paged_decode_kernel(At
             uint32_t count, before, cut_before;
             pieces.find(a, divide(piece, a->by_pairs), b, len, count, before, cut_before);
             b = uniform(b), len = uniform(len), n = uniform((int)count);
-            const uint32_t in = piece - before * (uint32_t)a->pairs, pair = uniform(in / count);
+            const uint32_t in = piece - before * (uint32_t)a->pairs, pair = n == 1 ? in : uniform(in / count);
             number = uniform((int)(in - pair * count));
             first_cut = cut_before * (uint32_t)a->pairs + pair * count;
             const int kvh = (int)pair / a->tiles, halves = (int)halves_of(a, len), units = (halves + kUnit - 1) / kUnit;
             head0 = kvh * a->group + ((int)pair - kvh * a->tiles) * kHeads;
             rows = min(kHeads, (kvh + 1) * a->group - head0);
             // the first units % n pieces have one more unit
-            const int each = uniform(units / n), more = units - each * n;
+            const int each = n == 1 ? units : uniform(units / n), more = units - each * n;
             const int unit = number * each + min(number, more), end = unit + each + (number < more ? 1 : 0);
-            w.start(b, kvh, head0, rows, len, min(halves, end * kUnit));
+            w.begin(b, kvh, head0, rows, len, min(halves, end * kUnit));
             w.run(unit * (kUnit / 2) + w.wave, end * (kUnit / 2), head0, rows);
             l = w.l, m = w.m;
 #pragma unroll
@@ -827,8 +866,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void paged_decode_kernel(At
         // the four wavefronts' sums on a common maximum
         const int thread = thread_now(), lane = thread & 63, wave = thread >> 6, col = lane & 15, g = lane >> 4;
         const Sums<DP> own = {W::NP > 1 ? all_wide : reinterpret_cast<float (*)[Sums<DP>::RP]>(red[0]), all_ml};
-        l += __shfl_xor(l, 16, 64);
-        l += __shfl_xor(l, 32, 64);
+        l = over_groups(l, [](float x, float y) { return x + y; });
         if (g == 0) ml[wave][col][0] = m, ml[wave][col][1] = l;
         __syncthreads();
         const float top = fmaxf(fmaxf(ml[0][col][0], ml[1][col][0]), fmaxf(ml[2][col][0], ml[3][col][0]));
@@ -940,7 +978,7 @@ bool plan_attention(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head
     if (batch * p->pairs > 0x7ffff000 / p->units) return false;
     p->dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
     // Pieces: as many as the card holds workgroups at once, and up to one more for every pair, whose last piece is smaller.
-    p->shares = kNumCU * (p->dp == 256 ? 2 : 3); if (const char *e = getenv("PW")) p->shares = atoi(e);
+    p->shares = kNumCU * (p->dp == 256 ? 2 : 3);
     const int64_t pieces = batch * p->pairs * p->units < p->shares ? batch * p->pairs * p->units : p->shares + batch * p->pairs;
     p->workgroups = pieces < 2048 ? pieces : 2048;
     p->score_pitch = (capacity + 3) / 4 * 4;
@@ -965,7 +1003,7 @@ void launch_attention(const AttnArgs &a, Addressing ad, unsigned workgroups, hip
 {
     const dim3 grid(workgroups), block(256);
     if (ad == kRows) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kRows>), grid, block, 0, s, a);
-    else if (QUANT && ad == kBlockScales) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, QUANT ? kBlockScales : kBlock>), grid, block, 0, s, a);
+    else if (ad == kBlockAlike) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlockAlike>), grid, block, 0, s, a);
     else if (ad == kBlockMask) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlockMask>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlock>), grid, block, 0, s, a);
 }
@@ -1055,13 +1093,15 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     // Halves that lie in one block: block by block, the last half of a block may be short, so blocks of fewer than 8 tokens
     // would leave most of a tile empty.  Offsets within a block have 31 bits, a block's own offset is a 32 x 32-bit product.
     const PagedArray *const arrays[] = {&a.cache.key, &a.cache.value, &a.cache.key_scale, &a.cache.value_scale};
-    bool blocks = pieces && cache->block_size >= 8, scales = cache->block_size % 4 == 0;
+    bool blocks = pieces && cache->block_size >= 8 && (!mask || cache->block_size % 4 == 0), scales = cache->block_size % 4 == 0;
     for (int i = 0; i < (quant ? 4 : 2); i++) {
         const PagedArray &x = *arrays[i];
-        blocks = blocks && (!mask || cache->block_size % 4 == 0) && x.block >= 0 && x.block <= 0xffffffffll && x.token >= 0 && x.token <= 0x7fffffff / (cache->block_size + 16);
+        blocks = blocks && x.block >= 0 && x.block <= 0xffffffffll && x.token >= 0 && x.token <= 0x7fffffff / (cache->block_size + 16);
         if (i >= 2) scales = scales && x.token == 4 && aligned(x.base, 16) && x.block % 16 == 0 && x.head % 16 == 0;
     }
-    const Addressing ad = !blocks ? kRows : mask ? kBlockMask : quant && scales ? kBlockScales : kBlock;
+    const auto alike = [](const PagedArray &x, const PagedArray &y) { return x.block == y.block && x.token == y.token && x.head == y.head; };
+    const bool same = alike(a.cache.key, a.cache.value) && (!quant || (scales && alike(a.cache.key_scale, a.cache.value_scale)));
+    const Addressing ad = !blocks ? kRows : mask ? kBlockMask : same ? kBlockAlike : kBlock;
     a.span = ad != kRows ? a.cache.page : fast_div(kHalf);
     a.halves = fast_div((a.span.d + kHalf - 1) / kHalf);
     hipStream_t s = static_cast<hipStream_t>(stream);
