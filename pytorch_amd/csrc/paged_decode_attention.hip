@@ -36,6 +36,13 @@ constexpr int kHeads = 16;                   // query heads of one tile
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 constexpr int kSC1 = 16;                     // cache-policy bit: agent scope, past the caches of one XCD
 
+// Workgroups that a compute unit holds, as their registers allow: one wavefront's keys, values and sums are 2 rows of 16 tokens
+// and 16 rows of outputs.  Rows of 512 bytes take more than 256 registers (16-bit heads of 256, one sequence of 65000, 532 MB:
+// 99 us with one workgroup and no spills, 190 with two that spill).  The work is cut for as many workgroups as the card holds:
+// a piece more or fewer for each leaves compute units waiting for the last (heads of 128, 32 sequences of up to 4095, 280 MB:
+// 62 us for 768 pieces, 66 for 512, 64 for 1024, 68 for 1536).
+constexpr int resident(int dp, bool quant) { return dp < 256 ? 3 : quant ? 2 : 1; }
+
 struct AttnArgs {
     PagedCache cache;
     const uint16_t *q;
@@ -792,7 +799,7 @@ __device__ __forceinline__ bool arrive(Global<uint32_t> *counter, int n, int *ld
 }
 
 template <int DP, bool QUANT, int QT, Addressing AD>
-__global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void paged_decode_kernel(AttnArgs)
+__global__ __launch_bounds__(256, resident(DP, QUANT)) void paged_decode_kernel(AttnArgs)
 {
     using W = Decode<DP, QUANT, QT, AD>;
     constexpr int RP = 128 + 4;                                  // row pitch of a wavefront's sums in LDS
@@ -962,8 +969,8 @@ struct AttnSizes {
 constexpr size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // false: outside what the kernels number in 32 bits
-bool plan_attention(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_blocks, int64_t block_size, bool sums,
-                    AttnSizes *p)
+bool plan_attention(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_blocks, int64_t block_size, bool quant,
+                    bool sums, AttnSizes *p)
 {
     if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || head_dim > 256 || max_blocks < 0 || block_size < 1)
         return false;
@@ -978,7 +985,7 @@ bool plan_attention(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head
     if (batch * p->pairs > 0x7ffff000 / p->units) return false;
     p->dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
     // Pieces: as many as the card holds workgroups at once, and up to one more for every pair, whose last piece is smaller.
-    p->shares = kNumCU * (p->dp == 256 ? 2 : 3);
+    p->shares = kNumCU * resident((int)p->dp, quant);
     const int64_t pieces = batch * p->pairs * p->units < p->shares ? batch * p->pairs * p->units : p->shares + batch * p->pairs;
     p->workgroups = pieces < 2048 ? pieces : 2048;
     p->score_pitch = (capacity + 3) / 4 * 4;
@@ -986,8 +993,9 @@ bool plan_attention(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head
     const auto take = [&](size_t bytes) { const size_t o = at; at += round256(bytes); return o; };
     // of pairs that are cut there are fewer than twice as many pieces as shares: a pair of u units, u more than a share of s, has
     // fewer than u / s + 1 < 2 u / s
-    p->part_bytes = (uint32_t)(p->shares * 2 * p->rows * p->dp * 4);
-    p->part_ml_bytes = (uint32_t)(p->shares * 2 * kHeads * 2 * 4);
+    const int64_t reserved = kNumCU * resident((int)p->dp, true);    // (the query of the size knows no type)
+    p->part_bytes = (uint32_t)(reserved * 2 * p->rows * p->dp * 4);
+    p->part_ml_bytes = (uint32_t)(reserved * 2 * kHeads * 2 * 4);
     p->part = take(p->part_bytes);
     p->part_ml = take(p->part_ml_bytes);
     p->lse2 = take(sums ? (size_t)(batch * heads) * 4 : 0);
@@ -995,6 +1003,7 @@ bool plan_attention(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head
     p->bytes = at;
     return true;
 }
+static_assert(resident(256, false) <= resident(256, true), "the workspace's size");
 static_assert(kNumCU * 3 * 4 * sizeof(uint32_t) <= kWorkspaceCounterBytes, "arrival counters");
 static_assert(kNumCU * 3 <= (kJoin / 2) * (kJoin / 2), "groups of pieces, and members of a group");
 
@@ -1027,7 +1036,7 @@ extern "C" size_t mi355_paged_decode_attention_workspace(int64_t batch, int64_t 
                                                          int64_t max_blocks, int64_t block_size, int with_sums)
 {
     mi355::AttnSizes p;
-    return mi355::plan_attention(batch, heads, kv_heads, head_dim, max_blocks, block_size, with_sums != 0, &p) ? p.bytes : 0;
+    return mi355::plan_attention(batch, heads, kv_heads, head_dim, max_blocks, block_size, true, with_sums != 0, &p) ? p.bytes : 0;
 }
 
 extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, const void *q, int q_dtype, int64_t q_stride_batch,
@@ -1047,7 +1056,7 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     if (batch == 0) return MI355_OK;
     if (!q || !out || !context_lens || (max_blocks > 0 && !block_table)) return MI355_ERR_BAD_ARGUMENT;
     AttnSizes p;
-    if (!plan_attention(batch, heads, cache->kv_heads, cache->head_dim, max_blocks, cache->block_size, attn_sums != nullptr, &p)) return MI355_ERR_UNSUPPORTED;
+    if (!plan_attention(batch, heads, cache->kv_heads, cache->head_dim, max_blocks, cache->block_size, quant, attn_sums != nullptr, &p)) return MI355_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < p.bytes) return MI355_ERR_WORKSPACE;
     if (!aligned(workspace, 16) || !aligned(q, 2) || !aligned(out, 2) || !aligned(lse, 4) || !aligned(block_table, 4) || !aligned(context_lens, 4) ||
         !aligned(attn_sums, 4))
