@@ -265,13 +265,15 @@ void launch_select(const EvictArgs &a, unsigned rows, int width, int elem, const
     else if (width == 1) hipLaunchKernelGGL((paged_select_kernel<KPT, 1>), grid, block, 0, s, a, elem, per_row);
     else hipLaunchKernelGGL((paged_select_kernel<KPT, 0>), grid, block, 0, s, a, elem, per_row);
 }
+// Rounds in steps of 2^k + 1: budgets are powers of two as a rule, and a cache that is kept at one has a block or two more.
 void launch_select(const EvictArgs &a, unsigned rows, int width, int elem, const FastDiv &per_row, hipStream_t s)
 {
     if (a.capacity <= 2 * kSelectThreads) launch_select<2>(a, rows, width, elem, per_row, s);
+    else if (a.capacity <= 3 * kSelectThreads) launch_select<3>(a, rows, width, elem, per_row, s);
     else if (a.capacity <= 5 * kSelectThreads) launch_select<5>(a, rows, width, elem, per_row, s);
-    else if (a.capacity <= 8 * kSelectThreads) launch_select<8>(a, rows, width, elem, per_row, s);
-    else if (a.capacity <= 16 * kSelectThreads) launch_select<16>(a, rows, width, elem, per_row, s);
-    else if (a.capacity <= 32 * kSelectThreads) launch_select<32>(a, rows, width, elem, per_row, s);
+    else if (a.capacity <= 9 * kSelectThreads) launch_select<9>(a, rows, width, elem, per_row, s);
+    else if (a.capacity <= 17 * kSelectThreads) launch_select<17>(a, rows, width, elem, per_row, s);
+    else if (a.capacity <= 33 * kSelectThreads) launch_select<33>(a, rows, width, elem, per_row, s);
     else launch_select<0>(a, rows, width, elem, per_row, s);
 }
 
