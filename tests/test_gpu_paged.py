@@ -325,6 +325,60 @@ def test_attention_on_another_stream_and_in_a_graph(pa):
     assert not torch.equal(one, out)
 
 
+@pytest.mark.parametrize("kind", [torch.bfloat16, "int8"])
+@pytest.mark.parametrize("page,d", [(16, 128), (24, 64), (64, 256)])
+def test_attention_keys_and_values_laid_out_differently(pa, kind, page, d):
+    """Keys token by token and values head by head, the scales the other way round."""
+    g = torch.Generator().manual_seed(page + d)
+    B, H, hkv = 5, 6, 3
+    kc, _, ks, _ = make_cache(g, 40, page, hkv, d, kind, "token", 16, "head")
+    _, vc, _, vs = make_cache(g, 40, page, hkv, d, kind, "head", 0, "token")
+    table, lens = tables(g, B, 7, 40, page), torch.tensor([0, 1, page, 5 * page + 3, 7 * page], dtype=torch.int32)
+    q = torch.randn(B, H, d, generator=g).to(torch.bfloat16)
+    check_attention(run_attention(pa, q, kc, vc, table, lens, ks, vs), attend_ref(q, kc, vc, table, lens, ks, vs), torch.bfloat16, kind == "int8")
+
+
+@pytest.mark.parametrize("kind", [torch.float16, "int8"])
+@pytest.mark.parametrize("hkv,group,d", [(1, 16, 128), (1, 3, 256), (2, 20, 64)])
+def test_attention_long_sequences_in_many_pieces(pa, kind, hkv, group, d):
+    """More pieces of a pair than are added at once, beside short sequences."""
+    g = torch.Generator().manual_seed(hkv * group)
+    lens = torch.tensor([23001, 40, 0, 9000], dtype=torch.int32)
+    width = 23040 // 64
+    kc, vc, ks, vs = make_cache(g, 4 * width, 64, hkv, d, kind)
+    table = tables(g, 4, width, 4 * width, 64)
+    q = torch.randn(4, hkv * group, d, generator=g).to(torch.float16)
+    check_attention(run_attention(pa, q, kc, vc, table, lens, ks, vs), attend_ref(q, kc, vc, table, lens, ks, vs), torch.float16, kind == "int8")
+
+
+@pytest.mark.parametrize("kind,d", [(torch.bfloat16, 80), (torch.float16, 40), ("int8", 64)])
+def test_attention_rows_of_several_heads_in_a_line(pa, kind, d):
+    g = torch.Generator().manual_seed(d)
+    B, hkv, page = 21, 7, 16
+    lens = torch.randint(0, 500, (B,), generator=g).to(torch.int32)
+    kc, vc, ks, vs = make_cache(g, B * 32, page, hkv, d, kind)
+    table = tables(g, B, 32, B * 32, page)
+    dt = torch.bfloat16 if kind == "int8" else kind
+    q = torch.randn(B, 2 * hkv, d, generator=g).to(dt)
+    check_attention(run_attention(pa, q, kc, vc, table, lens, ks, vs), attend_ref(q, kc, vc, table, lens, ks, vs), dt, kind == "int8")
+
+
+def test_attention_calls_leave_nothing_behind(pa):
+    """Calls of different shapes in turn, whose arrival counters lie at the same addresses: each gives the same bits every time."""
+    g = torch.Generator().manual_seed(77)
+    calls, first = [], []
+    for B, H, hkv, d, n in ((2, 16, 1, 128, 9000), (7, 8, 8, 64, 700), (1, 32, 2, 256, 20000), (130, 4, 2, 128, 300)):
+        width = -(-n // 64)
+        kc, vc, _, _ = make_cache(g, B * width, 64, hkv, d, torch.bfloat16)
+        lens = torch.randint(n // 2, n + 1, (B,), generator=g).to(torch.int32)
+        calls.append((torch.randn(B, H, d, generator=g).to(torch.bfloat16).cuda(), gpu(kc), gpu(vc), tables(g, B, width, B * width, 64).cuda(), lens.cuda()))
+        first.append(pa.npu_paged_decode_attention(*calls[-1], softmax_lse=True))
+    for _ in range(5):
+        for args, want in zip(calls, first):
+            got = pa.npu_paged_decode_attention(*args, softmax_lse=True)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 # ------------------------------------------------------------------------------------------------ write and read
 
 def codes_ref(x):
