@@ -163,7 +163,13 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
         const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, above = digit == 2 ? 10 : 21;
         const uint32_t mask = digit == 2 ? 1023 : 2047;
         walk(0, rounds, [&](int, int i, uint32_t k) {
-            if (i < n && (digit == 0 || (k >> above) == (prefix >> above))) atomicAdd(&hist[(k >> shift) & mask], 1u);
+            if (i < n && (digit == 0 || (k >> above) == (prefix >> above))) {
+                // the lanes with the first one's digit count as one: equal sums, all 0 after a prefill, would wait for each other
+                const uint32_t d = (k >> shift) & mask, d0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)d);
+                const uint64_t same = __ballot(d == d0);
+                if (d != d0) atomicAdd(&hist[d], 1u);
+                else if (lane == __builtin_ctzll(same)) atomicAdd(&hist[d], (uint32_t)__popcll(same));
+            }
         });
         __syncthreads();
         const uint32_t c0 = hist[2047 - 2 * tid], c1 = hist[2046 - 2 * tid];       // thread 0 has the largest digits
