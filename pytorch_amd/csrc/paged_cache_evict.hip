@@ -8,9 +8,10 @@
 // so all of them move at once, in place.
 //
 // One workgroup of 1024 threads chooses for one (sequence, head).  Thread t holds the places t, t + 1024, ..., whose keys stay
-// in registers over the three digits (rows of more than 32768 places are read again for each); ranks in the order of the places
+// in registers over the three digits (rows of more than 33 rounds are read again for each); ranks in the order of the places
 // come from ballots, counted per wavefront and 1024 places, and one scan over those counts.  Bound by latency: a dozen
-// barriers and three trips to memory.
+// barriers, three trips to memory, and 0.6 us per 1024 places.  One token over a budget of 4096, 128 rows of 128 elements:
+// 7.7 us in one launch, of 16384 17.7.  64 rows of 8192 places halved: 12 us, and 15.7 for the moves of 62 MB, 4.0 TB/s.
 #include "paged_cache.h"
 
 namespace mi355 {
@@ -91,7 +92,8 @@ __device__ __forceinline__ void move_pieces(const EvictArgs &a, int row, uint32_
     }
 }
 
-// KPT: rounds of 1024 places whose keys are held, KPT * 1024 >= capacity; 0: any number, read again for every digit.
+// KPT: rounds of 1024 places whose keys are held, KPT * 1024 >= capacity; 0: any number, read again for every digit (64 rows of
+// 16000 places halved: 52 us held, 82 read again; of 32000 114 and 157).
 // W: bytes per access of the moves that this kernel makes itself; 0: it leaves them to paged_move_kernel.
 template <int KPT, int W>
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a, int elem, FastDiv per_row)
@@ -164,10 +166,10 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
         const uint32_t mask = digit == 2 ? 1023 : 2047;
         walk(0, rounds, [&](int, int i, uint32_t k) {
             if (i < n && (digit == 0 || (k >> above) == (prefix >> above))) {
-                // the lanes with the first one's digit count as one: equal sums, all 0 after a prefill, would wait for each other
+                // a wavefront of equal digits counts as one: equal sums, all 0 after a prefill, would wait for each other
                 const uint32_t d = (k >> shift) & mask, d0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)d);
                 const uint64_t same = __ballot(d == d0);
-                if (d != d0) atomicAdd(&hist[d], 1u);
+                if (__ballot(d != d0)) atomicAdd(&hist[d], 1u);
                 else if (lane == __builtin_ctzll(same)) atomicAdd(&hist[d], (uint32_t)__popcll(same));
             }
         });
@@ -259,7 +261,9 @@ __global__ __launch_bounds__(256) void paged_move_kernel(EvictArgs a, int elem, 
     move_pieces<W>(a, blockIdx.y, (uint32_t)a.count[blockIdx.y], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, elem, per_row);
 }
 
-// A workgroup that chooses moves its rows itself where there can be few: up to this many bytes of keys.
+// A workgroup that chooses moves its rows itself where there can be few: up to this many bytes of keys.  (128 heads, rows of 256
+// bytes, 16 moves 9.7 us against 11.9 with a second launch, 64 moves 11.7 and 13.3, 256 moves 17.4 and 17.6; 512 heads, 64 moves
+// 22.5 and 22.9, 128 moves 33.7 and 31.5.)
 constexpr int64_t kMovedBySelect = 16384;
 
 template <int KPT>
@@ -271,7 +275,8 @@ void launch_select(const EvictArgs &a, unsigned rows, int width, int elem, const
     else if (width == 1) hipLaunchKernelGGL((paged_select_kernel<KPT, 1>), grid, block, 0, s, a, elem, per_row);
     else hipLaunchKernelGGL((paged_select_kernel<KPT, 0>), grid, block, 0, s, a, elem, per_row);
 }
-// Rounds in steps of 2^k + 1: budgets are powers of two as a rule, and a cache that is kept at one has a block or two more.
+// Rounds in steps of 2^k + 1: budgets are powers of two as a rule, and a cache that is kept at one has a block or two more.  A
+// round too many costs 0.2 to 0.6 us (one token over 8192: 11.9 us in 9 rounds, 15.1 in 16, 24 where nothing is held).
 void launch_select(const EvictArgs &a, unsigned rows, int width, int elem, const FastDiv &per_row, hipStream_t s)
 {
     if (a.capacity <= 2 * kSelectThreads) launch_select<2>(a, rows, width, elem, per_row, s);
