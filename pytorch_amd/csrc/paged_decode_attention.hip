@@ -24,6 +24,11 @@
 // of more units than the card's fair share is cut into equal pieces of at most that.  A workgroup takes a piece at a time; a
 // pair of one piece is finished there, else the workgroup leaves (sums, m, l) in the workspace, and the last one to arrive adds
 // them in their order.
+//
+// Bound by memory, at 5.5 to 5.9 TB/s where the work is long (32 sequences of 8192, 1.07 GB, in 188 us), behind about 12 us that
+// do not depend on it: the launch, two trips to memory for lengths and blocks, the first rows, and at the end the four
+// wavefronts' sums, their trip through the workspace and the addition.  With 32 query heads on 8 heads of 128: 32 sequences of up to 4095 tokens
+// (280 MB) 62 us, one of 131071 (537 MB) 104 us, int8, 64 of up to 8192 (563 MB) 120 us, one of 37 6.5 us.
 #include "paged_cache.h"
 #include "weight_quant_common.h"
 
@@ -218,9 +223,13 @@ __device__ __forceinline__ float over_groups(float v, Op op)
 //   kRows   lane by lane: any block size, stride, width and alignment
 //   kBlock  the half lies in one block: a scalar descriptor that ends with the half's last row, constant lane offsets; rows in
 //           16-byte pieces.  Rows behind the end read as zero without traffic, so the loop needs no edge code.
-//   kBlockAlike  as kBlock; keys and values lie alike, so that one offset serves both - the loop has half the scalar
-//           instructions -, and so do the scales (int8), those of four tokens of a head in 16 aligned bytes
+//   kBlockAlike  int8, as kBlock; keys and values lie alike, so that one offset serves both, and so do the scales, those of four
+//           tokens of a head in 16 aligned bytes (64 sequences of up to 8192, 8 heads of 128: 123.4 us, 124.5 as kBlock; 32 of up
+//           to 4095, 8 heads of 64: 24.8 and 25.4.  16-bit caches have no scales and gain nothing)
 //   kBlockMask  as kBlock, with a mask, whose bytes are read four at a time
+// 32 sequences of up to 4095, 8 heads of 128, blocks of 16: 62.9 us as kBlock, 74.4 as kRows; 16 masked ones, 32 heads of 80,
+// blocks of 24: 28.6 as kBlockMask, 36.4 as kRows; int8, 64 of up to 8192: 219.9 as kRows.  A short half wastes its operand's
+// rows, so kBlock loses with small blocks: 66.2 and 74.8 us for blocks of 8, 79.8 and 75 for 5, 84.9 and 75.4 for 4.
 enum Addressing { kRows, kBlock, kBlockAlike, kBlockMask };
 
 // DP: head_dim rounded up to 64, 128 or 256.  QT: type of q and out (0 bf16, 1 fp16).
@@ -366,7 +375,7 @@ struct Decode {
             if constexpr (AD != kRows) {
                 if constexpr (AD == kBlockAlike) {
                     start[s] = start_of(a->cache.key, p, s), reach[s] = reach_of(a->cache.key, p, s, D * ES);
-                    if constexpr (QUANT) scale_start[s] = start_of(a->cache.key_scale, p, s);
+                    scale_start[s] = start_of(a->cache.key_scale, p, s);
                 }
                 const __amdgpu_buffer_rsrc_t r = AD == kBlockAlike ? rows_at(kbase, start[s], reach[s]) : rows_of(kbase, a->cache.key, p, s, D * ES);
 #pragma unroll
@@ -496,7 +505,7 @@ struct Decode {
     // keeps a uniform branch a branch: the edge cases would cost selects in every tile
     __device__ static __forceinline__ void no_select() { asm volatile(""); }
     // every position of the tile is seen, known without a look at the lanes
-    __device__ __forceinline__ bool full(const Place &p) const { return (AD == kBlock || AD == kBlockAlike) && p.n[0] + p.n[1] == 2 * kHalf; }
+    __device__ __forceinline__ bool full(const Place &p) const { return AD != kRows && AD != kBlockMask && p.n[0] + p.n[1] == 2 * kHalf; }
     __device__ __forceinline__ void store_scores(const Place &p, const f32x4 (&z)[2], int head0, int rows) const
     {
         if (col >= rows) return;
@@ -866,8 +875,9 @@ __global__ __launch_bounds__(256, resident(DP, QUANT)) void paged_decode_kernel(
         const Args a = args_now();
         const int64_t out_row = (int64_t)b * a->heads + head0;
         Global<uint32_t> *arrived = at(a->arrived);
-        // Of a pair that is cut, the last of its workgroups to arrive adds everybody's sums.  Where those are more than some
-        // hundred kilobytes, groups of about the root of their number are added first, so that no workgroup has many to read.  The
+        // Of a pair that is cut, the last of its workgroups to arrive adds everybody's sums.  Where those are more than 64 KiB, groups
+        // of about the root of their number are added first, so that no workgroup has many to read (one sequence of 8000, 16
+        // query heads each: 19.5 us, 25.7 without groups; with 4 heads each and 4000 tokens 11.9 us at once, 13.8 in groups).  The
         // counter of a group is its first piece's, that of the groups lies behind all of these.
         int size = n;
         if (n >= kJoin || n * rows * (DP / 4) > 512 * kFlight) {
@@ -1022,9 +1032,9 @@ void launch_attention(const AttnArgs &a, Addressing ad, unsigned workgroups, hip
 {
     const dim3 grid(workgroups), block(256);
     if (ad == kRows) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kRows>), grid, block, 0, s, a);
-    else if (ad == kBlockAlike) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlockAlike>), grid, block, 0, s, a);
     else if (ad == kBlockMask) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlockMask>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlock>), grid, block, 0, s, a);
+    else if (ad == kBlock) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlock>), grid, block, 0, s, a);
+    else if constexpr (QUANT) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlockAlike>), grid, block, 0, s, a);
 }
 
 template <int DP>
@@ -1119,7 +1129,7 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
         if (i >= 2) scales = scales && x.token == 4 && aligned(x.base, 16) && x.block % 16 == 0 && x.head % 16 == 0;
     }
     const auto alike = [](const PagedArray &x, const PagedArray &y) { return x.block == y.block && x.token == y.token && x.head == y.head; };
-    const bool same = alike(a.cache.key, a.cache.value) && (!quant || (scales && alike(a.cache.key_scale, a.cache.value_scale)));
+    const bool same = quant && scales && alike(a.cache.key, a.cache.value) && alike(a.cache.key_scale, a.cache.value_scale);
     const Addressing ad = !blocks ? kRows : mask ? kBlockMask : same ? kBlockAlike : kBlock;
     // Rows of several heads in a cache line, with other heads' rows of the same token: work on them at the same time and on one XCD,
     // so that the line comes once (16 sequences of up to 1001 tokens, 32 heads of 80: 32.4 -> 28.6 us; int8, 32 sequences of up to
