@@ -959,24 +959,36 @@ __global__ __launch_bounds__(256, resident(DP, QUANT)) void paged_decode_kernel(
 }
 
 // attn_sums[b, kv head, j] += sum over the kv head's query heads of 2^(z_j - lse2), in the heads' order.  Four positions per
-// thread; what was hidden has z = -infinity.
+// thread, four heads requested at once; what was hidden has z = -infinity.  Bound by latency: 16 sequences of 4097, 32 heads on
+// 8, 12.6 MB in 5.2 us (5.8 with one head at a time).
 __global__ __launch_bounds__(256) void paged_sums_kernel(AttnArgs a)
 {
     const int b = blockIdx.z, kvh = blockIdx.y;
     const int len = min(max(a.lens[b], 0), a.capacity);
+    const int64_t first = (int64_t)b * a.heads + kvh * a.group;
     for (int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; j < len; j += (int64_t)gridDim.x * 1024) {
-        f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int h = 0; h < a.group; h++) {
-            const int64_t at = (int64_t)b * a.heads + kvh * a.group + h;
-            const float lse2 = a.lse2[at];
-            const f32x4 z = *reinterpret_cast<const f32x4 *>(a.scores + at * a.score_pitch + j);
-#pragma unroll
-            for (int i = 0; i < 4; i++) sum[i] += z[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(z[i] - lse2);
-        }
         float *to = a.sums + b * a.sums_batch + kvh * a.sums_head + j;
+        float old[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) old[i] = to[min((int64_t)i, len - 1 - j)];
+        f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int h0 = 0; h0 < a.group; h0 += 4) {
+            f32x4 z[4];
+            float lse2[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int64_t at = first + min(h0 + k, a.group - 1);
+                lse2[k] = a.lse2[at];
+                z[k] = *reinterpret_cast<const f32x4 *>(a.scores + at * a.score_pitch + j);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum[i] += h0 + k >= a.group || z[k][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(z[k][i] - lse2[k]);
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (j + i < len) to[i] += sum[i];
+            if (j + i < len) to[i] = old[i] + sum[i];
     }
 }
 
