@@ -397,7 +397,7 @@ struct Decode {
                     for (int r = 0; r < 4; r++) ks[s][r] = __shfl(mine, g * 4 + r, 64);
                 }
             }
-            if constexpr (AD == kBlockMask) {                    // (the host: blocks of a multiple of 4 tokens)
+            if constexpr (AD == kBlockMask) {                    // from any byte (the host: blocks of a multiple of 4 tokens)
                 const uint64_t first = (uint64_t)a->mask + (uint64_t)(b * a->mask_stride) + (uint32_t)p.key[s];
                 const __amdgpu_buffer_rsrc_t r = make_rsrc((const void *)uniform((int64_t)first), (uint32_t)(p.n[s] + 3) & ~3u);
                 hidden[s] = __builtin_amdgcn_raw_buffer_load_b32(r, g * 4, 0, 0);

@@ -67,10 +67,10 @@ void check_slots(const char *op, const Tensor &slots)
                 " ", slots.sizes());
 }
 
-// the table and the lengths as the kernels take them: int32
+// the table and the lengths as the kernels take them: int32, what does not fit still beyond every block and length
 Tensor as_int(const Tensor &t)
 {
-    Tensor i = t.scalar_type() == at::kInt ? t : t.to(at::kInt);
+    Tensor i = t.scalar_type() == at::kInt ? t : t.clamp(-1, 0x7fffffff).to(at::kInt);
     return i.dim() == 1 ? packed(i) : inner_contiguous(i) ? i : i.contiguous();
 }
 

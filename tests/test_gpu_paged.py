@@ -325,6 +325,37 @@ def test_attention_on_another_stream_and_in_a_graph(pa):
     assert not torch.equal(one, out)
 
 
+@pytest.mark.parametrize("offset,pitch", [(0, 0), (1, 3), (2, 8), (4, 2)])
+def test_attention_mask_that_is_a_view(pa, offset, pitch):
+    """Rows of the mask at any address and distance."""
+    g = torch.Generator().manual_seed(offset + pitch)
+    B, H, hkv, d, page = 4, 4, 2, 64, 16
+    kc, vc, _, _ = make_cache(g, 24, page, hkv, d, torch.bfloat16)
+    table, lens = tables(g, B, 6, 24, page), torch.tensor([96, 5, 50, 81], dtype=torch.int32)
+    whole = torch.rand(B, offset + 96 + pitch, generator=g) < 0.4
+    mask = whole[:, offset:offset + 96]
+    q = torch.randn(B, H, d, generator=g).to(torch.bfloat16)
+    got = run_attention(pa, q, kc, vc, table, lens, atten_mask=whole.cuda()[:, offset:offset + 96])
+    check_attention(got, attend_ref(q, kc, vc, table, lens, mask=mask), torch.bfloat16, False)
+
+
+def test_attention_and_eviction_take_64_bit_tables_and_lengths(pa):
+    """What does not fit into 32 bits names no block, and is longer or shorter than anything."""
+    g = torch.Generator().manual_seed(8)
+    B, H, hkv, d, page = 4, 4, 2, 64, 16
+    kc, vc, _, _ = make_cache(g, 24, page, hkv, d, torch.bfloat16)
+    table, lens = tables(g, B, 6, 24, page).long(), torch.tensor([96, 2 ** 32 + 5, -2 ** 33 + 7, 40])
+    table[0, 2] = 2 ** 32 + 3
+    table[3, 0] = -2 ** 32 + 1
+    table[1, 1] = 2 ** 40
+    q = torch.randn(B, H, d, generator=g).to(torch.bfloat16)
+    assert attend_ref(q, kc, vc, table, lens)[1][2].eq(-math.inf).all()
+    check_attention(run_attention(pa, q, kc, vc, table, lens), attend_ref(q, kc, vc, table, lens), torch.bfloat16, False)
+    sums, positions = torch.rand(B, hkv, 96, generator=g).cuda(), torch.arange(96, dtype=torch.int32).expand(B, hkv, 96).contiguous().cuda()
+    kept, _, _ = pa.npu_paged_cache_evict(gpu(kc), gpu(vc), table.cuda(), lens.cuda(), sums, positions, 30, 4)
+    assert kept.tolist() == [30, 30, 0, 30]
+
+
 @pytest.mark.parametrize("kind", [torch.bfloat16, "int8"])
 @pytest.mark.parametrize("page,d", [(16, 128), (24, 64), (64, 256)])
 def test_attention_keys_and_values_laid_out_differently(pa, kind, page, d):
