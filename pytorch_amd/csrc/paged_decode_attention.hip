@@ -658,7 +658,6 @@ __device__ __forceinline__ void store_lse(Args a, int64_t row, float m, float l,
 // what comes of adding those.
 template <int DP>
 struct Sums {
-    static constexpr int QPR = DP / 4;                           // quads of consecutive d in a row
     static constexpr int RP = (DP > 128 ? DP : 128) + 4;         // row pitch, 4 words past a bank cycle
     float (*row)[RP];
     float (*ml)[2];                                              // maximum, sum of probabilities
