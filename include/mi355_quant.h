@@ -467,6 +467,8 @@ int mi355_paged_cache_read(const mi355_paged_cache *cache, void *key, const int6
  *   attn_sums     NULL, or float32 [batch, kv_heads, max_blocks * block_size], positions contiguous, updated where seen
  *   workspace     mi355_paged_decode_attention_workspace() bytes, 16-byte aligned, its first MI355_WORKSPACE_ZERO_BYTES zero
  *                 and left zero, as for mi355_quant_matmul
+ * Calls that share a workspace, this one's or the eviction's, must not be made by several host threads at once, on one stream
+ * either: with attn_sums, and where an eviction has many rows to move, a second launch reads what the first left there.
  */
 size_t mi355_paged_decode_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_blocks,
                                               int64_t block_size, int with_sums);

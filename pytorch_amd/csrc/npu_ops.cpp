@@ -174,7 +174,10 @@ std::tuple<Tensor, Tensor, Tensor> dynamic_quant_asym_hip(const Tensor &input, c
 // The matmul kernels exchange split-K partial sums through a workspace whose leading zero area (arrival counters and
 // the exchange zone, MI355_WORKSPACE_ZERO_BYTES) must be zero before a launch; the kernels leave it zero.  One
 // zero-initialised buffer per (device, stream) is kept and reused; launches on one stream are ordered, so they never
-// overlap.  Lifetime rules, because a captured HIP graph keeps the pointer it was recorded with:
+// overlap.  An operator of several launches hands data from one to the next in it (a transposed weight, lists of moves,
+// scores), so whoever takes a stream's workspace holds it until its last launch is enqueued: another host thread's
+// launches on that stream come before all of them or behind all of them.
+// Lifetime rules, because a captured HIP graph keeps the pointer it was recorded with:
 //   * eager calls: a buffer that is superseded by a larger one is never released (it stays alive, zeroed, until the
 //     process ends), so a graph recorded earlier replays on valid, quiescent memory;
 //   * a call made while the stream is capturing uses the stream's eager buffer when there is one that is large enough
@@ -184,15 +187,16 @@ std::tuple<Tensor, Tensor, Tensor> dynamic_quant_asym_hip(const Tensor &input, c
 //     exactly as long as the graph.  Such a buffer is never handed to an eager call or to another capture; the cache
 //     drops its reference when it sees the next capture (or an eager call) on that stream, which returns the block
 //     to the pool of the graph that owns it.
+struct StreamWorkspaces {
+    std::mutex mu;                                                        // held by the call that uses one of these
+    Tensor eager;
+    unsigned long long capture_id = 0;
+    Tensor captured;
+    std::vector<Tensor> retired;                                          // never freed: an earlier graph may point into them
+};
 struct WorkspaceCache {
-    struct Captured {
-        unsigned long long id = 0;
-        Tensor ws;
-    };
-    std::mutex mu;
-    std::map<std::pair<int, void *>, Tensor> eager;
-    std::map<std::pair<int, void *>, Captured> captured;
-    std::vector<std::pair<std::pair<int, void *>, Tensor>> retired;       // never freed: an earlier graph may point into them
+    std::mutex mu;                                                        // of the map; never waited for with a stream's held
+    std::map<std::pair<int, void *>, StreamWorkspaces> streams;           // entries stay where they are
 };
 
 WorkspaceCache &workspace_cache()
@@ -225,42 +229,45 @@ Tensor new_workspace(const Tensor &like, int64_t bytes)
 // (16x9999x8192 59.6 -> 64.2 us, 1784x9313x8192 148.2 -> 153.3).
 constexpr size_t kKeptWorkspaceBytes = (size_t)MI355_WORKSPACE_ZERO_BYTES + ((size_t)64 << 20);
 
-Tensor zeroed_workspace(const Tensor &like, size_t bytes, bool large_for_call = false)
+Workspace zeroed_workspace(const Tensor &like, size_t bytes, bool large_for_call = false)
 {
     WorkspaceCache &wc = workspace_cache();
-    std::lock_guard<std::mutex> lock(wc.mu);
-    const auto key = std::make_pair((int)like.device().index(), stream_of(like));
+    void *const stream = stream_of(like);
+    StreamWorkspaces *of_stream;
+    {
+        std::lock_guard<std::mutex> lock(wc.mu);
+        of_stream = &wc.streams[std::make_pair((int)like.device().index(), stream)];
+    }
+    std::unique_lock<std::mutex> held(of_stream->mu);
     int64_t want = (int64_t)std::max<size_t>(bytes, (size_t)MI355_WORKSPACE_ZERO_BYTES + ((size_t)1 << 20));
     hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
     unsigned long long capture_id = 0;
-    TORCH_CHECK(hipStreamGetCaptureInfo(static_cast<hipStream_t>(key.second), &capturing, &capture_id) == hipSuccess,
+    TORCH_CHECK(hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &capturing, &capture_id) == hipSuccess,
                 "hipStreamGetCaptureInfo failed");
+    Tensor &ws = of_stream->eager, &captured = of_stream->captured;
     if (capturing != hipStreamCaptureStatusNone) {
-        const auto eager = wc.eager.find(key);
-        if (eager != wc.eager.end() && eager->second.defined() && (size_t)eager->second.numel() >= bytes) return eager->second;
-        WorkspaceCache::Captured &c = wc.captured[key];
-        if (!c.ws.defined() || c.id != capture_id || (size_t)c.ws.numel() < bytes) {
-            c.ws = new_workspace(like, want);                               // the fill is recorded into this capture
-            c.id = capture_id;
+        if (ws.defined() && (size_t)ws.numel() >= bytes) return {std::move(held), ws};
+        if (!captured.defined() || of_stream->capture_id != capture_id || (size_t)captured.numel() < bytes) {
+            captured = new_workspace(like, want);                           // the fill is recorded into this capture
+            of_stream->capture_id = capture_id;
         }
-        return c.ws;
+        return {std::move(held), captured};
     }
-    wc.captured.erase(key);
-    if (large_for_call && bytes > kKeptWorkspaceBytes) return new_workspace(like, want);
-    Tensor &ws = wc.eager[key];
+    captured.reset();
+    if (large_for_call && bytes > kKeptWorkspaceBytes) return {std::move(held), new_workspace(like, want)};
     if (!ws.defined() || (size_t)ws.numel() < bytes) {
         if (ws.defined()) {
             // geometric growth bounds the buffers a stream can retire (a handful between 17 MiB and the largest problem)
             want = std::max<int64_t>(want, 2 * ws.numel());
             Tensor old = ws;
-            wc.retired.emplace_back(key, old);
+            of_stream->retired.push_back(old);
             ws = at::zeros({want}, like.options().dtype(at::kChar));
-            check_workspace(old, key.second, "when its workspace was outgrown");
+            check_workspace(old, stream, "when its workspace was outgrown");
         } else {
             ws = at::zeros({want}, like.options().dtype(at::kChar));
         }
     }
-    return ws;
+    return {std::move(held), ws};
 }
 
 // ---------------------------------------------------------------- npu_trans_quant_param
@@ -480,15 +487,15 @@ Tensor quant_matmul_hip(const Tensor &x1, const Tensor &x2, const Tensor &scale,
         if (w.stride(0) == 1 && !rows_aligned(w, w.stride(1))) w = aligned_rows(w.t(), p.K).t();
         const int64_t m = a.size(0);
         const size_t ws_bytes = mi355_quant_matmul_workspace(m, p.N, p.K, w.stride(0), w.stride(1));
-        const Tensor ws = ws_bytes ? zeroed_workspace(xa, ws_bytes, (p.K & 15) != 0) : Tensor();   // such a K: padded copies of the operands
+        const Workspace ws = ws_bytes ? zeroed_workspace(xa, ws_bytes, (p.K & 15) != 0) : Workspace();   // such a K: padded copies of the operands
         void *o = static_cast<char *>(out.data_ptr()) + row0 * p.N * (int64_t)out.element_size();
         const int st = qp.defined()
             ? mi355_quant_matmul_qparam(static_cast<int8_t *>(a.data_ptr()), static_cast<int8_t *>(w.data_ptr()), static_cast<uint64_t *>(qp.data_ptr()),
                                         qp.numel(), ptr(b), bias_dtype, o, out_dtype, m, p.N, p.K, a.stride(0), w.stride(0), w.stride(1),
-                                        p.N, ptr(ws), ws_bytes, stream_of(x1))
+                                        p.N, ptr(ws.memory), ws_bytes, stream_of(x1))
             : mi355_quant_matmul(static_cast<int8_t *>(a.data_ptr()), static_cast<int8_t *>(w.data_ptr()), static_cast<float *>(ptr(ps)),
                                  static_cast<float *>(ptr(scale_f)), bf16 ? scale_f.numel() : 0, ptr(b), bias_dtype, o, out_dtype, m, p.N, p.K,
-                                 a.stride(0), w.stride(0), w.stride(1), p.N, ptr(ws), ws_bytes, stream_of(x1));
+                                 a.stride(0), w.stride(0), w.stride(1), p.N, ptr(ws.memory), ws_bytes, stream_of(x1));
         check_status(st, "npu_quant_matmul");
     };
     if (xa.dim() == 2 && xb.dim() == 2) {
@@ -639,16 +646,17 @@ Tensor weight_quant_hip(const Tensor &x, const Tensor &weight, const Tensor &ant
     Tensor bias_c;
     if (const Tensor *t = opt(bias)) bias_c = packed(*t);
     const size_t ws_bytes = mi355_weight_quant_matmul_workspace(p.M, p.N, p.K, p.bits, group_size);
-    Tensor ws;
-    if (ws_bytes) ws = zeroed_workspace(x, ws_bytes);
-    check_status(mi355_weight_quant_matmul(x2.data_ptr(), x.scalar_type() == at::kHalf ? MI355_DTYPE_FP16 : MI355_DTYPE_BF16,
-                                           w.data_ptr(), p.bits, s.data_ptr(), o.defined() ? o.data_ptr() : nullptr,
-                                           bias_c.defined() ? bias_c.data_ptr() : nullptr,
-                                           out.data_ptr(), p.M, p.N, p.K, group_size, ld_param_g, ld_param_n, x2.stride(0),
-                                           ldw_k, ldw_n, p.N,
-                                           ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0,
-                                           stream_of(x)),
-                 "npu_weight_quant_batchmatmul");
+    {
+        const Workspace ws = ws_bytes ? zeroed_workspace(x, ws_bytes) : Workspace();
+        check_status(mi355_weight_quant_matmul(x2.data_ptr(), x.scalar_type() == at::kHalf ? MI355_DTYPE_FP16 : MI355_DTYPE_BF16,
+                                               w.data_ptr(), p.bits, s.data_ptr(), o.defined() ? o.data_ptr() : nullptr,
+                                               bias_c.defined() ? bias_c.data_ptr() : nullptr,
+                                               out.data_ptr(), p.M, p.N, p.K, group_size, ld_param_g, ld_param_n, x2.stride(0),
+                                               ldw_k, ldw_n, p.N,
+                                               ws.memory.defined() ? ws.memory.data_ptr() : nullptr, ws.memory.defined() ? (size_t)ws.memory.numel() : 0,
+                                               stream_of(x)),
+                     "npu_weight_quant_batchmatmul");
+    }
     const Tensor *qs = opt(quant_scale);
     if (!qs) return out;
     // int8 output: y = clamp(rint(float(out) * quant_scale[n] + quant_offset[n]), -128, 127), the product rounded to the
@@ -941,7 +949,7 @@ Tensor quantize_hip(const Tensor &x, const Tensor &scales, const optional<Tensor
 
 } // namespace
 
-at::Tensor mi355_ops::workspace(const at::Tensor &like, size_t bytes, bool large_for_call) { return zeroed_workspace(like, bytes, large_for_call); }
+mi355_ops::Workspace mi355_ops::workspace(const at::Tensor &like, size_t bytes, bool large_for_call) { return zeroed_workspace(like, bytes, large_for_call); }
 
 TORCH_LIBRARY_FRAGMENT(npu, m)
 {
@@ -995,17 +1003,21 @@ TORCH_LIBRARY_IMPL(npu, Meta, m)
 extern "C" int mi355_npu_check_workspaces(void)
 {
     WorkspaceCache &wc = workspace_cache();
-    std::vector<std::pair<std::pair<int, void *>, Tensor>> all;
+    std::vector<std::pair<void *, StreamWorkspaces *>> all;
     {
         std::lock_guard<std::mutex> lock(wc.mu);
-        for (auto &kv : wc.eager)
-            if (kv.second.defined()) all.emplace_back(kv.first, kv.second);
-        for (auto &kv : wc.retired) all.push_back(kv);
+        for (auto &kv : wc.streams) all.emplace_back(kv.first.second, &kv.second);
     }
     int failures = 0;
-    for (auto &kv : all) {
-        c10::hip::HIPGuardMasqueradingAsCUDA guard(kv.second.device());
-        if (mi355_workspace_status(kv.second.data_ptr(), (size_t)kv.second.numel(), 1, kv.first.second) != MI355_OK) failures++;
+    for (auto &[stream, of_stream] : all) {
+        std::lock_guard<std::mutex> held(of_stream->mu);
+        const auto check = [&failures, stream = stream](const Tensor &ws) {
+            if (!ws.defined()) return;
+            c10::hip::HIPGuardMasqueradingAsCUDA guard(ws.device());
+            if (mi355_workspace_status(ws.data_ptr(), (size_t)ws.numel(), 1, stream) != MI355_OK) failures++;
+        };
+        check(of_stream->eager);
+        for (const Tensor &ws : of_stream->retired) check(ws);
     }
     return failures;
 }

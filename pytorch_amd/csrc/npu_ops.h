@@ -6,17 +6,25 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <mutex>
+
 #include "mi355_quant.h"
 
 namespace mi355_ops {
-// the stream's workspace, its zero area (MI355_WORKSPACE_ZERO_BYTES) zero (npu_ops.cpp)
-at::Tensor workspace(const at::Tensor &like, size_t bytes, bool large_for_call = false);
+// A stream's workspace, its zero area (MI355_WORKSPACE_ZERO_BYTES) zero (npu_ops.cpp).  It is this call's as long as the object
+// lives: keep it until the last launch that uses it is enqueued, and take no second one meanwhile.
+struct Workspace {
+    std::unique_lock<std::mutex> held;
+    at::Tensor memory;
+};
+Workspace workspace(const at::Tensor &like, size_t bytes, bool large_for_call = false);
 } // namespace mi355_ops
 
 namespace {
 
 using at::Tensor;
 using c10::optional;
+using mi355_ops::Workspace;
 
 void check_status(int status, const char *op)
 {

@@ -214,14 +214,14 @@ std::tuple<Tensor, Tensor> attention_hip(const Tensor &query, const Tensor &key_
     const Tensor hidden = !mask || inner_contiguous(*mask) ? (mask ? *mask : Tensor()) : mask->contiguous();
     const mi355_paged_cache c = describe(key_cache, value_cache, ks, vs);
     const size_t bytes = mi355_paged_decode_attention_workspace(batch, heads, kv_heads, q.size(2), table.size(1), key_cache.size(1), sums != nullptr);
-    const Tensor ws = mi355_ops::workspace(q, bytes, sums != nullptr);
+    const Workspace ws = mi355_ops::workspace(q, bytes, sums != nullptr);
     const double scale = scale_value.has_value() ? *scale_value : 1.0 / std::sqrt((double)q.size(2));
     check_status(mi355_paged_decode_attention(&c, q.data_ptr(), act_code(q.scalar_type()), q.stride(0), q.stride(1), out.data_ptr(),
                                               softmax_lse ? lse.data_ptr<float>() : nullptr, batch, heads, table.data_ptr<int32_t>(), table.stride(0),
                                               table.size(1), lens.data_ptr<int32_t>(), (float)scale,
                                               mask ? reinterpret_cast<const uint8_t *>(hidden.data_ptr()) : nullptr, mask ? hidden.stride(0) : 0,
                                               sums ? sums->data_ptr<float>() : nullptr, sums ? sums->stride(0) : 0, sums ? sums->stride(1) : 0,
-                                              ws.data_ptr(), bytes, stream_of(query)),
+                                              ws.memory.data_ptr(), bytes, stream_of(query)),
                  op);
     return {out, lse};
 }
@@ -267,11 +267,11 @@ std::tuple<Tensor, Tensor, Tensor> evict_hip(const Tensor &key_cache, const Tens
     const mi355_paged_cache c = describe(key_cache, value_cache, ks, vs);
     const size_t bytes = mi355_paged_cache_evict_workspace(batch, key_cache.size(2), table.size(1), key_cache.size(1), keep);
     // behind the zero area of the stream's workspace: 0.35 us less on the host than memory of its own
-    const Tensor ws = mi355_ops::workspace(key_cache, MI355_WORKSPACE_ZERO_BYTES + bytes, true);
+    const Workspace ws = mi355_ops::workspace(key_cache, MI355_WORKSPACE_ZERO_BYTES + bytes, true);
     check_status(mi355_paged_cache_evict(&c, table.data_ptr<int32_t>(), table.stride(0), table.size(1), lens.data_ptr<int32_t>(), batch,
                                          sums.data_ptr<float>(), sums.stride(0), sums.stride(1), pos.data_ptr<int32_t>(), pos.stride(0), pos.stride(1),
                                          keep, recent, new_lens.data_ptr<int32_t>(), new_sums.data_ptr<float>(), new_positions.data_ptr<int32_t>(),
-                                         static_cast<char *>(ws.data_ptr()) + MI355_WORKSPACE_ZERO_BYTES, bytes, stream_of(key_cache)),
+                                         static_cast<char *>(ws.memory.data_ptr()) + MI355_WORKSPACE_ZERO_BYTES, bytes, stream_of(key_cache)),
                  op);
     return {new_lens, new_sums, new_positions};
 }
