@@ -85,8 +85,9 @@ class PagedKVCache:
         self._write(key, value, self.block_table, self.context_lens)
         if self.budget is not None:
             at = self.context_lens.clamp(max=self.capacity - 1).long()[:, None, None].expand(-1, self.positions.shape[1], 1)
-            self.positions.scatter_(2, at, self.next_position[:, None, None].expand_as(at))
-            self.next_position += 1
+            fits = self.context_lens < self.capacity              # else the last place keeps its position
+            self.positions.scatter_(2, at, torch.where(fits[:, None], self.next_position[:, None], self.positions[:, :, -1])[..., None])
+            self.next_position += fits
         self.context_lens.add_(1).clamp_(max=self.capacity)
 
     def prefill(self, sequence: int, key: torch.Tensor, value: torch.Tensor) -> None:
@@ -95,12 +96,14 @@ class PagedKVCache:
         self._room([sequence], tokens)
         place = self.context_lens[sequence] + torch.arange(tokens, dtype=torch.int32, device=self.context_lens.device)
         self._write(key, value, self.block_table[sequence].expand(tokens, -1), place)
+        held = (self.context_lens[sequence] + tokens).clamp(max=self.capacity)
         if self.budget is not None:
-            at = place.clamp(max=self.capacity - 1).long().expand(self.positions.shape[1], -1)
+            at = place.clamp(max=self.capacity).long().expand(self.positions.shape[1], -1)
             position = self.next_position[sequence] + torch.arange(tokens, dtype=torch.int32, device=at.device)
-            self.positions[sequence].scatter_(1, at, position.expand_as(at))
-            self.next_position[sequence] += tokens
-        self.context_lens[sequence] = (self.context_lens[sequence] + tokens).clamp(max=self.capacity)
+            row = torch.nn.functional.pad(self.positions[sequence], (0, 1))       # (what does not fit goes to the place behind)
+            self.positions[sequence] = row.scatter_(1, at, position.expand_as(at))[:, :-1]
+            self.next_position[sequence] += held - self.context_lens[sequence]
+        self.context_lens[sequence] = held
 
     def attend(self, query: torch.Tensor, *, scale_value: float | None = None, atten_mask: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of one token per sequence over what the sequence holds; with a budget the weights are summed."""
