@@ -69,6 +69,8 @@ class PagedKVCache:
         full = [b for b in sequences if self._held[b] + tokens > self.capacity]
         if full:
             raise RuntimeError(f"sequence {full[0]} holds up to {self._held[full[0]]} tokens, {tokens} more do not fit into {self.capacity}")
+
+    def _count(self, sequences, tokens: int) -> None:
         for b in sequences:
             self._held[b] += tokens
 
@@ -81,8 +83,10 @@ class PagedKVCache:
 
     def append(self, key: torch.Tensor, value: torch.Tensor) -> None:
         """One new token for every sequence."""
-        self._room(range(len(self._held)), 1)
+        everyone = range(len(self._held))
+        self._room(everyone, 1)
         self._write(key, value, self.block_table, self.context_lens)
+        self._count(everyone, 1)                                  # (the operator has taken them)
         if self.budget is not None:
             at = self.context_lens.clamp(max=self.capacity - 1).long()[:, None, None].expand(-1, self.positions.shape[1], 1)
             fits = self.context_lens < self.capacity              # else the last place keeps its position
@@ -96,6 +100,7 @@ class PagedKVCache:
         self._room([sequence], tokens)
         place = self.context_lens[sequence] + torch.arange(tokens, dtype=torch.int32, device=self.context_lens.device)
         self._write(key, value, self.block_table[sequence].expand(tokens, -1), place)
+        self._count([sequence], tokens)
         held = (self.context_lens[sequence] + tokens).clamp(max=self.capacity)
         if self.budget is not None:
             at = place.clamp(max=self.capacity).long().expand(self.positions.shape[1], -1)

@@ -64,3 +64,20 @@ def test_replays_that_overfill_prefill_what_fits(operator):
     assert operator.slots[1:] == [[14, 15, -1, -1, -1], [-1] * 5]
     assert c.context_lens.tolist() == [0, 8] and c.next_position.tolist() == [0, 8]
     assert c.positions[1].tolist() == [list(range(8))] * HEADS
+
+
+def test_refused_calls_do_not_count(operator):
+    """What the operator does not take leaves the host's count, and everything else, as it was."""
+    c = Bookkeeping()
+    c.prefill(0, *rows(5))
+    wrong = torch.zeros(3, HEADS, DIM, dtype=torch.float16)
+    for call in (lambda: c.prefill(0, wrong, wrong), lambda: c.append(wrong, wrong), lambda: c.append(*rows(BATCH + 1))):
+        for _ in range(3):
+            with pytest.raises(RuntimeError, match="key must have shape"):
+                call()
+    with pytest.raises(RuntimeError, match="sequence 0 holds up to 5 tokens, 4 more do not fit into 8"):
+        c.prefill(0, *rows(4))
+    c.prefill(0, *rows(3))
+    assert c.context_lens.tolist() == [8, 0]
+    with pytest.raises(RuntimeError, match="do not fit"):
+        c.append(*rows(BATCH))
