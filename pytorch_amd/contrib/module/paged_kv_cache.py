@@ -74,10 +74,14 @@ class PagedKVCache:
         for b in sequences:
             self._held[b] += tokens
 
+    def _slots(self, table, place):
+        """Slots, in 64 bits, of `place` (int64 [tokens]) of the sequences in the rows of `table`."""
+        block = (place // self.block_size).clamp(max=self.block_table.shape[1] - 1)
+        return torch.add(place % self.block_size, table.gather(1, block[:, None])[:, 0], alpha=self.block_size)
+
     def _write(self, key, value, table, place) -> None:
         """key, value of the tokens that go to `place` (int32 [tokens]) of the sequence in their row of `table`."""
-        block = (place // self.block_size).clamp(max=self.block_table.shape[1] - 1)
-        slots = table.gather(1, block[:, None].long())[:, 0] * self.block_size + place % self.block_size
+        slots = self._slots(table, place.long())
         slots = torch.where(place < self.capacity, slots, -1)     # (a replayed step does not pass through _room)
         torch.ops.npu.npu_paged_cache_write(key, value, self.key_cache, self.value_cache, slots, key_scale=self.key_scale, value_scale=self.value_scale)
 
@@ -133,8 +137,8 @@ class PagedKVCache:
         """Keys and values in places [start, stop) of one sequence, as ``dtype``: what a later chunk of a prompt attends to."""
         if not 0 <= start <= stop <= self.capacity:
             raise IndexError(f"places [{start}, {stop}) of {self.capacity}")
-        place = torch.arange(start, stop, dtype=torch.int32, device=self.block_table.device)
-        slots = self.block_table[sequence][(place // self.block_size).long()] * self.block_size + place % self.block_size
+        place = torch.arange(start, stop, device=self.block_table.device)
+        slots = self._slots(self.block_table[sequence].expand(stop - start, -1), place)
         return torch.ops.npu.npu_paged_cache_read(self.key_cache, self.value_cache, slots, key_scale=self.key_scale, value_scale=self.value_scale,
                                                   dtype=self.dtype)
 

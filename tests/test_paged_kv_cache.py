@@ -81,3 +81,22 @@ def test_refused_calls_do_not_count(operator):
     assert c.context_lens.tolist() == [8, 0]
     with pytest.raises(RuntimeError, match="do not fit"):
         c.append(*rows(BATCH))
+
+
+def test_blocks_that_the_table_does_not_name_take_nothing(operator):
+    """Whatever stands in the table: no slot of the cache comes of a number that names no block."""
+    c = Bookkeeping()
+    for entry in (-1, -2 ** 31, 2 ** 31 - 1, 2 ** 30, 2 ** 30 + 1, BATCH * 2):
+        c.block_table[0, 0] = entry
+        c.append(*rows(BATCH))
+        c.context_lens.zero_()
+        c._held = [0] * BATCH
+        assert not 0 <= operator.slots[-1][0] < BATCH * 8 and operator.slots[-1][1] == 8
+
+
+def test_read_of_blocks_that_the_table_does_not_name(operator, monkeypatch):
+    c = Bookkeeping()
+    c.block_table[1] = torch.tensor([2 ** 30, 3])
+    monkeypatch.setattr(torch.ops.npu, "npu_paged_cache_read", lambda key_cache, value_cache, slots, **more: slots.tolist())
+    assert c.read(1, 2, 7) == [2 ** 32 + 2, 2 ** 32 + 3, 12, 13, 14]
+    assert c.read(0, 3, 3) == []
