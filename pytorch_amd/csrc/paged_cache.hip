@@ -245,33 +245,8 @@ void launch_rows(RowArgs &a, bool quant, bool fp16, hipStream_t s)
 }
 
 template <bool WRITE>
-int move_rows(const mi355_paged_cache *cache, int dtype, void *key, const int64_t *key_stride, void *value, const int64_t *value_stride,
-              const void *slots, int slots_dtype, int64_t tokens, void *stream)
+void launch_tokens(RowArgs &a, bool vec, bool quant, bool fp16, hipStream_t s)
 {
-    RowArgs a;
-    if (const int st = open_cache(cache, &a.cache); st != MI355_OK) return st;
-    const bool quant = cache->dtype == MI355_DTYPE_INT8;
-    if (tokens < 0 || (dtype != MI355_DTYPE_BF16 && dtype != MI355_DTYPE_FP16) || (!quant && cache->dtype != dtype)) return MI355_ERR_BAD_ARGUMENT;
-    if (slots_dtype != MI355_DTYPE_INT32 && slots_dtype != MI355_DTYPE_INT64) return MI355_ERR_BAD_ARGUMENT;
-    if (tokens == 0) return MI355_OK;
-    if (!key || !value || !slots || !key_stride || !value_stride) return MI355_ERR_BAD_ARGUMENT;
-    if (tokens > 0x7fffff00 / cache->kv_heads - 16) return MI355_ERR_UNSUPPORTED;
-    if (!aligned(key, 2) || !aligned(value, 2) || !aligned(slots, slots_dtype == MI355_DTYPE_INT64 ? 8 : 4)) return MI355_ERR_ALIGNMENT;
-    a.plane[0] = static_cast<uint16_t *>(key);
-    a.plane[1] = static_cast<uint16_t *>(value);
-    bool vec = a.cache.dim % 8 == 0 && a.cache.dim <= 256;
-    const int64_t *strides[2] = {key_stride, value_stride};
-    for (int i = 0; i < 2; i++) {
-        a.tok[i] = strides[i][0];
-        a.head[i] = strides[i][1];
-        vec = vec && aligned(a.plane[i], 16) && a.tok[i] % 8 == 0 && a.head[i] % 8 == 0 && rows_aligned(i ? a.cache.value : a.cache.key, quant ? 8 : 16);
-    }
-    a.slot_ids = slots;
-    a.slots64 = slots_dtype == MI355_DTYPE_INT64;
-    a.run = a.cache.key.token < a.cache.key.head ? 4 : 0;
-    a.tokens = (uint32_t)tokens;
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    const bool fp16 = dtype == MI355_DTYPE_FP16;
     if (!vec) {
         number_groups(a, 1);
         const dim3 grid((a.groups + 3) / 4, 2);
@@ -288,6 +263,43 @@ int move_rows(const mi355_paged_cache *cache, int dtype, void *key, const int64_
         launch_rows<WRITE, 16>(a, quant, fp16, s);
     } else {
         launch_rows<WRITE, 32>(a, quant, fp16, s);
+    }
+}
+
+// Rows of one launch at most: the threads of a grid, up to 64 for a row, are numbered in 32 bits (beyond, the grid wraps without
+// an error), and a token has up to 65535 rows.
+constexpr int64_t kRowsPerLaunch = (int64_t)1 << 25;
+
+template <bool WRITE>
+int move_rows(const mi355_paged_cache *cache, int dtype, void *key, const int64_t *key_stride, void *value, const int64_t *value_stride,
+              const void *slots, int slots_dtype, int64_t tokens, void *stream)
+{
+    RowArgs a;
+    if (const int st = open_cache(cache, &a.cache); st != MI355_OK) return st;
+    const bool quant = cache->dtype == MI355_DTYPE_INT8;
+    if (tokens < 0 || (dtype != MI355_DTYPE_BF16 && dtype != MI355_DTYPE_FP16) || (!quant && cache->dtype != dtype)) return MI355_ERR_BAD_ARGUMENT;
+    if (slots_dtype != MI355_DTYPE_INT32 && slots_dtype != MI355_DTYPE_INT64) return MI355_ERR_BAD_ARGUMENT;
+    if (tokens == 0) return MI355_OK;
+    if (!key || !value || !slots || !key_stride || !value_stride) return MI355_ERR_BAD_ARGUMENT;
+    if (tokens > 0x7fffff00 / cache->kv_heads - 16) return MI355_ERR_UNSUPPORTED;
+    const int id_bytes = slots_dtype == MI355_DTYPE_INT64 ? 8 : 4;
+    if (!aligned(key, 2) || !aligned(value, 2) || !aligned(slots, id_bytes)) return MI355_ERR_ALIGNMENT;
+    uint16_t *const plane[2] = {static_cast<uint16_t *>(key), static_cast<uint16_t *>(value)};
+    bool vec = a.cache.dim % 8 == 0 && a.cache.dim <= 256;
+    const int64_t *strides[2] = {key_stride, value_stride};
+    for (int i = 0; i < 2; i++) {
+        a.tok[i] = strides[i][0];
+        a.head[i] = strides[i][1];
+        vec = vec && aligned(plane[i], 16) && a.tok[i] % 8 == 0 && a.head[i] % 8 == 0 && rows_aligned(i ? a.cache.value : a.cache.key, quant ? 8 : 16);
+    }
+    a.slots64 = slots_dtype == MI355_DTYPE_INT64;
+    a.run = a.cache.key.token < a.cache.key.head ? 4 : 0;
+    const int64_t most = kRowsPerLaunch / cache->kv_heads;
+    for (int64_t t0 = 0; t0 < tokens; t0 += most) {
+        for (int i = 0; i < 2; i++) a.plane[i] = plane[i] + t0 * a.tok[i];
+        a.slot_ids = static_cast<const char *>(slots) + t0 * id_bytes;
+        a.tokens = (uint32_t)(tokens - t0 < most ? tokens - t0 : most);
+        launch_tokens<WRITE>(a, vec, quant, dtype == MI355_DTYPE_FP16, static_cast<hipStream_t>(stream));
     }
     return check_launch();
 }
