@@ -344,19 +344,28 @@ extern "C" int mi355_paged_cache_evict(const mi355_paged_cache *cache, const int
     const bool wide = bytes % 16 == 0 && rows_aligned(a.cache.key, 16) && rows_aligned(a.cache.value, 16);
     const FastDiv per_row = fast_div((uint32_t)(bytes / (wide ? 16 : elem)) * 2);
     const bool here = a.most * bytes <= kMovedBySelect;
-    launch_select(a, (unsigned)rows, here ? (wide ? 16 : elem) : 0, elem, per_row, s);
-    if (!here) {
-        const int64_t chunks = (a.most * per_row.d + 255) / 256, n = 65535 / cache->kv_heads * cache->kv_heads;
-        for (int64_t r0 = 0; r0 < rows; r0 += n) {               // a grid's second dimension has 16 bits
-            EvictArgs c = a;
-            c.count += r0;
-            c.moves += r0 * 2 * a.most;
-            c.table += r0 / cache->kv_heads * table_stride;
-            const dim3 grid((unsigned)(chunks < 64 ? chunks : 64), (unsigned)(rows - r0 < n ? rows - r0 : n));
-            if (wide) hipLaunchKernelGGL(paged_move_kernel<16>, grid, dim3(256), 0, s, c, elem, per_row);
-            else if (elem == 2) hipLaunchKernelGGL(paged_move_kernel<2>, grid, dim3(256), 0, s, c, elem, per_row);
-            else hipLaunchKernelGGL(paged_move_kernel<1>, grid, dim3(256), 0, s, c, elem, per_row);
-        }
+    // Rows are a grid's second dimension (16 bits) for the moves, and 1024 threads each (32 bits in all; beyond, a grid wraps
+    // without an error) for the choice: more of them go sequence by sequence into several launches.
+    const int64_t sequences = (here ? (int64_t)1 << 21 : 65535) / cache->kv_heads;
+    for (int64_t b0 = 0; b0 < batch; b0 += sequences) {
+        const int64_t n = (batch - b0 < sequences ? batch - b0 : sequences) * cache->kv_heads, r0 = b0 * cache->kv_heads;
+        EvictArgs c = a;
+        c.table += b0 * table_stride;
+        c.lens += b0;
+        c.sums += b0 * sums_stride_batch;
+        c.positions += b0 * positions_stride_batch;
+        c.new_lens += b0;
+        c.new_sums += r0 * capacity;
+        c.new_positions += r0 * capacity;
+        c.count += r0;
+        c.moves += r0 * 2 * a.most;
+        launch_select(c, (unsigned)n, here ? (wide ? 16 : elem) : 0, elem, per_row, s);
+        if (here) continue;
+        const int64_t chunks = (a.most * per_row.d + 255) / 256;
+        const dim3 grid((unsigned)(chunks < 64 ? chunks : 64), (unsigned)n);
+        if (wide) hipLaunchKernelGGL(paged_move_kernel<16>, grid, dim3(256), 0, s, c, elem, per_row);
+        else if (elem == 2) hipLaunchKernelGGL(paged_move_kernel<2>, grid, dim3(256), 0, s, c, elem, per_row);
+        else hipLaunchKernelGGL(paged_move_kernel<1>, grid, dim3(256), 0, s, c, elem, per_row);
     }
     return check_launch();
 }
