@@ -75,39 +75,39 @@ class PagedKVCache:
             self._held[b] += tokens
 
     def _slots(self, table, place):
-        """Slots, in 64 bits, of `place` (int64 [tokens]) of the sequences in the rows of `table`."""
-        block = (place // self.block_size).clamp(max=self.block_table.shape[1] - 1)
-        return torch.add(place % self.block_size, table.gather(1, block[:, None])[:, 0], alpha=self.block_size)
+        """Slots, in 64 bits, of `place` (int64 [tokens], below the capacity) of the sequences in the rows of `table`."""
+        return torch.add(place % self.block_size, table.gather(1, (place // self.block_size)[:, None])[:, 0], alpha=self.block_size)
 
-    def _write(self, key, value, table, place) -> None:
-        """key, value of the tokens that go to `place` (int32 [tokens]) of the sequence in their row of `table`."""
-        slots = self._slots(table, place.long())
-        slots = torch.where(place < self.capacity, slots, -1)     # (a replayed step does not pass through _room)
+    def _write(self, key, value, table, place, fits) -> None:
+        """key, value of the tokens that go to `place` of the sequence in their row of `table`, if they fit."""
+        slots = torch.where(fits, self._slots(table, place), -1)  # (a replayed step does not pass through _room)
         torch.ops.npu.npu_paged_cache_write(key, value, self.key_cache, self.value_cache, slots, key_scale=self.key_scale, value_scale=self.value_scale)
 
     def append(self, key: torch.Tensor, value: torch.Tensor) -> None:
         """One new token for every sequence."""
         everyone = range(len(self._held))
         self._room(everyone, 1)
-        self._write(key, value, self.block_table, self.context_lens)
+        fits = self.context_lens < self.capacity
+        place = self.context_lens.clamp(max=self.capacity - 1).long()
+        self._write(key, value, self.block_table, place, fits)
         self._count(everyone, 1)                                  # (the operator has taken them)
         if self.budget is not None:
-            at = self.context_lens.clamp(max=self.capacity - 1).long()[:, None, None].expand(-1, self.positions.shape[1], 1)
-            fits = self.context_lens < self.capacity              # else the last place keeps its position
+            at = place[:, None, None].expand(-1, self.positions.shape[1], 1)
+            # (of a token that does not fit: the last place keeps its position)
             self.positions.scatter_(2, at, torch.where(fits[:, None], self.next_position[:, None], self.positions[:, :, -1])[..., None])
             self.next_position += fits
-        self.context_lens.add_(1).clamp_(max=self.capacity)
+        self.context_lens += fits
 
     def prefill(self, sequence: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Tokens of one sequence behind those that it has."""
         tokens = key.shape[0]
         self._room([sequence], tokens)
-        place = self.context_lens[sequence] + torch.arange(tokens, dtype=torch.int32, device=self.context_lens.device)
-        self._write(key, value, self.block_table[sequence].expand(tokens, -1), place)
+        place = self.context_lens[sequence] + torch.arange(tokens, device=self.context_lens.device)
+        self._write(key, value, self.block_table[sequence].expand(tokens, -1), place.clamp(max=self.capacity - 1), place < self.capacity)
         self._count([sequence], tokens)
         held = (self.context_lens[sequence] + tokens).clamp(max=self.capacity)
         if self.budget is not None:
-            at = place.clamp(max=self.capacity).long().expand(self.positions.shape[1], -1)
+            at = place.clamp(max=self.capacity).expand(self.positions.shape[1], -1)
             position = self.next_position[sequence] + torch.arange(tokens, dtype=torch.int32, device=at.device)
             row = torch.nn.functional.pad(self.positions[sequence], (0, 1))       # (what does not fit goes to the place behind)
             self.positions[sequence] = row.scatter_(1, at, position.expand_as(at))[:, :-1]
