@@ -20,7 +20,9 @@ __all__ = ["PagedKVCache"]
 class PagedKVCache:
     """``max_tokens``: what a sequence can hold at once.  ``quantized``: int8 codes with a float32 scale per token and head in
     place of ``dtype``.  ``budget``: the tokens that ``evict`` leaves, each key/value head choosing its own by the attention
-    they got; the newest ``recent`` (default: a quarter) always stay.  The cache needs room for at least one token beyond it.
+    they got from ``attend``; the newest ``recent`` (default: a quarter) always stay.  The cache needs room for at least one token
+    beyond it.  Tokens of a prompt have got none before the first ``attend``: an ``evict`` before it keeps the recent tokens and
+    the first ones.
 
     Tensors on ``device``: ``key_cache``, ``value_cache`` [blocks, block_size, kv_heads, head_dim] (``key_scale``, ``value_scale`` without the
     last dimension), stored so that the tokens of one head of a block follow each other; ``block_table`` [batch, blocks per
@@ -28,7 +30,8 @@ class PagedKVCache:
     ``positions`` [batch, kv_heads, capacity] and ``next_position`` [batch].
 
     A call that would overfill a sequence raises, as far as the host knows the lengths: replays of a captured step pass it by.
-    What does not fit then is not written, and a length stays at the capacity.
+    What does not fit then is not written and gets no position, and a length stays at the capacity.  ``append`` takes a token for
+    every sequence; one that has ended is cleared, so that it does not fill up.
     """
 
     def __init__(self, batch: int, max_tokens: int, kv_heads: int, head_dim: int, *, block_size: int = 64, budget: int | None = None,

@@ -7,10 +7,12 @@
 // `keep` then fill the holes before it, both in ascending order: the fewest rows move, sources and destinations are disjoint,
 // so all of them move at once, in place.
 //
-// One workgroup of 1024 threads chooses for one (sequence, head).  Thread t holds the places t, t + 1024, ..., whose keys stay
-// in registers over the three digits (rows of more than 33 rounds are read again for each); ranks in the order of the places
+// One workgroup of 1024 threads chooses for one (sequence, head).  Thread t holds the places t, t + 1024, ...: their sums,
+// positions and keys stay in its registers over the three digits, up to 17 rounds; at 33 rounds (99 words) 86 registers spill to
+// scratch, still faster than reading again; rows of more rounds are read again for each digit.  Ranks in the order of the places
 // come from ballots, counted per wavefront and 1024 places, and one scan over those counts.  Bound by latency: a dozen
-// barriers, three trips to memory, and 0.6 us per 1024 places.  One token over a budget of 4096, 128 rows of 128 elements:
+// barriers, three trips to memory, and 0.6 us per 1024 places.  All of that also runs for a row with one token too many, where
+// the least worth alone would do.  One token over a budget of 4096, 128 rows of 128 elements:
 // 7.7 us in one launch, of 16384 17.7.  64 rows of 8192 places halved: 12 us, and 15.7 for the moves of 62 MB, 4.0 TB/s.
 #include "paged_cache.h"
 
@@ -93,7 +95,7 @@ __device__ __forceinline__ void move_pieces(const EvictArgs &a, int row, uint32_
 }
 
 // KPT: rounds of 1024 places whose keys are held, KPT * 1024 >= capacity; 0: any number, read again for every digit (64 rows of
-// 16000 places halved: 52 us held, 82 read again; of 32000 114 and 157).
+// 16000 places halved: 52 us held, 82 read again; of 32000, held in part in scratch, 114 and 157).
 // W: bytes per access of the moves that this kernel makes itself; 0: it leaves them to paged_move_kernel.
 template <int KPT, int W>
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a, int elem, FastDiv per_row)

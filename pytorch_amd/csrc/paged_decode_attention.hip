@@ -3,7 +3,8 @@
 // Per sequence b and query head h (key/value head h / group), over the positions j that are seen:
 //   z_j = scale * log2(e) * sum_d q_d k_jd      m = max z_j      l = sum_j 2^(z_j - m)
 //   out_d = sum_j 2^(z_j - m) v_jd / l          lse = (m + log2 l) / log2(e)
-// Every cached byte is read once and used for `group` heads, so the bound is the cache's bytes over the memory's rate.
+// Every cached byte is read once for up to 16 query heads of its key/value head (a larger group reads it once for each 16), so
+// the bound is the cache's bytes over the memory's rate.
 //
 // One wavefront takes 32 positions at a time and keeps running (m, l, out) for up to 16 heads:
 //   scores   C[position][head] = K[position][d] Q[d][head]: MFMA 16x16x32, keys as the first operand straight from memory
@@ -18,6 +19,12 @@
 //
 // int8 caches: codes become 16-bit numbers exactly; the scale of a position's keys multiplies its score, the scale of its
 // values multiplies its probability, in float32.
+//
+// Scores, maxima, l and out are float32.  The second product takes 16-bit operands, so probabilities are rounded once, to the
+// values' own type: 2^-8 of each in bf16, 2^-11 in fp16, which is what the values themselves carry, and l sums them unrounded.
+// Against probabilities kept in float32 the outputs' error grows from 0.0017 to 0.0018 of their norm for 37 bf16 positions, and by
+// less over more of them; the rounding of out to its own type makes the rest.  Products with value scales, on int8 caches, whose
+// values are exact, keep two bf16 terms, 2^-16.
 //
 // Work is dealt out on the device, because the lengths are known only there: the positions of every (sequence, head) pair
 // are cut into halves of a tile, 16 positions of one block (fewer at a block's end), eight halves make a unit, and a pair
@@ -42,11 +49,12 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417
 constexpr uint32_t kDealt = 64;              // pieces that are dealt to the XCDs at once
 constexpr int kSC1 = 16;                     // cache-policy bit: agent scope, past the caches of one XCD
 
-// Workgroups that a compute unit holds, as their registers allow: one wavefront's keys, values and sums are 2 rows of 16 tokens
-// and 16 rows of outputs.  Rows of 512 bytes take more than 256 registers (16-bit heads of 256, one sequence of 65000, 532 MB:
-// 99 us with one workgroup and no spills, 190 with two that spill).  The work is cut for as many workgroups as the card holds:
-// a piece more or fewer for each leaves compute units waiting for the last (heads of 128, 32 sequences of up to 4095, 280 MB:
-// 62 us for 768 pieces, 66 for 512, 64 for 1024, 68 for 1536).
+// Workgroups of a compute unit that the work is cut for, no more than their registers allow: one wavefront's keys, values and
+// sums are 2 rows of 16 tokens and 16 rows of outputs, 139 to 168 registers for heads of 65 to 128, where three fit.  Rows of 512
+// bytes take more than 256 (16-bit heads of 256, one sequence of 65000, 532 MB: 99 us with one workgroup and no spills, 190 with
+// two that spill).  A piece more or fewer for each leaves compute units waiting for the last (heads of 128, 32 sequences of up to
+// 4095, 280 MB: 62 us for 768 pieces, 66 for 512, 64 for 1024, 68 for 1536).  Heads of up to 64 take 103 to 124 registers, of
+// which four would fit; they are cut for three like the others.
 constexpr int resident(int dp, bool quant) { return dp < 256 ? 3 : quant ? 2 : 1; }
 
 struct AttnArgs {
@@ -546,7 +554,8 @@ struct Decode {
             l += p[i];
         }
         if constexpr (QUANT) {
-            // probabilities times value scales in two bf16 terms: 16 significant bits of any magnitude
+            // probabilities times value scales in two bf16 terms: 16 significant bits of any magnitude (one term would be 2^-8 of
+            // each, where the codes are exact)
 #pragma unroll
             for (int i = 0; i < 8; i++) p[i] = p[i] * vs[i / 4][i % 4];
             if (!full(place)) {                                  // (a scale that is not seen may be anything)
@@ -560,6 +569,7 @@ struct Decode {
                 pl[i] = pack_bf16x2(p[2 * i] - bf16_lo(ph[i]), p[2 * i + 1] - bf16_hi(ph[i]));
             }
         } else {
+            // one term, as precise as the values
 #pragma unroll
             for (int i = 0; i < 4; i++) ph[i] = pack_act2<PT>(p[2 * i], p[2 * i + 1]);
         }
