@@ -417,6 +417,46 @@ int mi355_probe_clock(unsigned long long *out, int workgroups, int iters, void *
 /* Measurement aid: a kernel that does nothing, `workgroups` x 256 threads (the per-launch floor inside a captured graph). */
 int mi355_probe_empty_launch(int workgroups, void *stream);
 
+/* ---- between the projections of a decoder layer ---- */
+
+/*
+ * The residual's addition and the root-mean-square norm behind it.  Not in the reference's tree.  Per row of x1, x2
+ * [rows, cols] (dtype bf16 or fp16, *_stride elements between rows; x2 NULL: x1 alone), in float32, every operation rounded by itself:
+ *   s = x1 + x2     rstd = 1 / sqrt(sum s^2 / cols + epsilon)     y = (s * rstd) * gamma     x = s
+ *   gamma  [cols] of dtype or float32 (gamma_dtype)      y  [rows, cols] of dtype, contiguous
+ *   rstd   float32 [rows] or NULL                        x  [rows, cols] of dtype, contiguous; with x2, else NULL
+ */
+int mi355_add_rms_norm(const void *x1, const void *x2, int dtype, const void *gamma, int gamma_dtype, void *y, float *rstd, void *x,
+                       int64_t rows, int64_t cols, int64_t x1_stride, int64_t x2_stride, float epsilon, void *stream);
+
+/*
+ * The same into int8 codes with one scale per row, as mi355_quant_matmul takes them.  rstd, a factor of the whole row, cancels in
+ * the codes:
+ *   u = s * gamma     step = max |u| / 127     y = rint_half_even(u / step)     scale = step * rstd
+ * A row whose u are all 0, or that holds a NaN or an infinity, has codes of 0 where they are not finite; its scale is 0 or NaN.
+ */
+int mi355_add_rms_norm_dynamic_quant(const void *x1, const void *x2, int dtype, const void *gamma, int gamma_dtype, int8_t *y, float *scale,
+                                     void *x, int64_t rows, int64_t cols, int64_t x1_stride, int64_t x2_stride, float epsilon, void *stream);
+
+/*
+ * Rotary positions on 1 to 4 axes for the queries and keys of the same tokens.  Not in the reference's tree.  The first rotary_dim
+ * elements of a head are pairs, (i, i + rotary_dim / 2) or, interleaved, (2 i, 2 i + 1), one for each frequency f; with p the
+ * token's position on the axis whose section holds f, in float32:
+ *   a' = a * cos[p][f] - b * sin[p][f]     b' = b * cos[p][f] + a * sin[p][f]
+ * and one rounding.  The other elements are copied.
+ *   positions   int32 or int64 (positions_dtype), [axes, tokens] with any strides
+ *   sections    [axes] on the HOST: frequencies of the axes in turn, rotary_dim / 2 in all; NULL with one axis
+ *   query, key  [tokens, heads / kv_heads, head_dim] of dtype (bf16 or fp16), the last dimension contiguous; *_stride[0], *_stride[1]:
+ *               elements between tokens and between heads; *_out the same, contiguous.  Either may have no heads
+ *   cos_sin     [max_positions, rotary_dim] of dtype or float32 (cos_sin_dtype), rows cos_sin_stride elements apart: cosines of the
+ *               frequencies, then their sines.  A position outside it counts as cos = sin = 0
+ */
+int mi355_mrope(const void *positions, int positions_dtype, int64_t positions_stride_axis, int64_t positions_stride_token, int64_t axes,
+                const int64_t *sections, const void *query, const int64_t *query_stride, int64_t heads, const void *key,
+                const int64_t *key_stride, int64_t kv_heads, int dtype, const void *cos_sin, int cos_sin_dtype, int64_t cos_sin_stride,
+                int64_t max_positions, int64_t tokens, int64_t head_dim, int64_t rotary_dim, int interleaved, void *query_out,
+                void *key_out, void *stream);
+
 /* ---- paged key-value cache ----
  *
  * Not in the reference's tree; named and laid out like the operators above.  A cache holds the keys and values of one

@@ -22,7 +22,8 @@ EXPORTS = ("mi355_status_string", "mi355_quant_abi_version", "mi355_dynamic_quan
            "mi355_quant_matmul_noalloc", "mi355_stream_capture_id", "mi355_probe_clock", "mi355_device_info", "mi355_transpose_int8", "mi355_probe_empty_launch",
            "mi355_workspace_status", "mi355_workspace_zero_bytes",
            "mi355_paged_cache_write", "mi355_paged_cache_read", "mi355_paged_decode_attention_workspace", "mi355_paged_decode_attention",
-           "mi355_paged_cache_evict_workspace", "mi355_paged_cache_evict")
+           "mi355_paged_cache_evict_workspace", "mi355_paged_cache_evict",
+           "mi355_add_rms_norm", "mi355_add_rms_norm_dynamic_quant", "mi355_mrope")
 
 _lib = None
 

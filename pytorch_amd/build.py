@@ -19,7 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 KERNEL_LIB = os.path.join(CSRC, "libmi355_quant.so")
 OPS_LIB = os.path.join(CSRC, "libmi355_npu_ops.so")
 CALL_LIB = os.path.join(HERE, "_op_call.so")
-KERNEL_SOURCES = ["dynamic_quant.hip", "dynamic_quant_asym.hip", "quant_matmul.hip", "quant_matmul_decode.hip", "weight_quant_matmul.hip", "weight_quant_gemm.hip", "weight_quant_kmajor_gemm.hip", "weight_quant_kpacked.hip", "weight_quant_kpacked_decode.hip", "weight_quant_kmajor_decode.hip", "weight_quant_decode.hip", "weight_quant_gemm4.hip", "weight_quant_repack.hip", "swiglu.hip", "anti_quant.hip", "unpack_int4.hip", "quantize.hip", "paged_cache.hip", "paged_decode_attention.hip", "paged_cache_evict.hip", "tuning.hip", "device_probe.hip"]
+KERNEL_SOURCES = ["dynamic_quant.hip", "dynamic_quant_asym.hip", "quant_matmul.hip", "quant_matmul_decode.hip", "weight_quant_matmul.hip", "weight_quant_gemm.hip", "weight_quant_kmajor_gemm.hip", "weight_quant_kpacked.hip", "weight_quant_kpacked_decode.hip", "weight_quant_kmajor_decode.hip", "weight_quant_decode.hip", "weight_quant_gemm4.hip", "weight_quant_repack.hip", "swiglu.hip", "anti_quant.hip", "unpack_int4.hip", "quantize.hip", "paged_cache.hip", "paged_decode_attention.hip", "paged_cache_evict.hip", "add_rms_norm.hip", "mrope.hip", "tuning.hip", "device_probe.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -ffp-contract=off: the dequantising epilogues must round every operation separately.
@@ -85,7 +85,7 @@ def build_ops(verbose: bool = False) -> str:
     """torch operator library: host-only C++ against libtorch + the C ABI; and the operators' direct call path."""
     import sysconfig
 
-    for cmd in (_torch_command(["npu_ops.cpp", "paged_ops.cpp"], OPS_LIB, "-L", CSRC, "-lc10_hip", "-ltorch_hip", "-lmi355_quant"),
+    for cmd in (_torch_command(["npu_ops.cpp", "paged_ops.cpp", "layer_ops.cpp"], OPS_LIB, "-L", CSRC, "-lc10_hip", "-ltorch_hip", "-lmi355_quant"),
                 _torch_command(["op_call.cpp"], CALL_LIB, "-I", sysconfig.get_paths()["include"], "-ltorch_python")):
         out = _run(cmd)
         if verbose and out.strip():

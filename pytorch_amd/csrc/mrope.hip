@@ -1,0 +1,294 @@
+// npu_mrope for gfx950: rotary positions on one or several axes, for the queries and keys of a fused projection in one launch.
+//
+// The first R of a head's D elements are R / 2 pairs - (i, i + R / 2), or (2 i, 2 i + 1) interleaved -, one for each frequency
+// f; with the position p of the token on the axis that f belongs to, in float32, every operation rounded by itself:
+//   a' = a * cos[p][f] - b * sin[p][f]     b' = b * cos[p][f] + a * sin[p][f]
+// and one rounding to 16 bits.  The other D - R elements are copied.  Cosines and sines come from a table [positions][R], the
+// cosines first.  A position outside the table counts as cos = sin = 0.
+//
+// Bound by memory: every element is read and written once.  A thread takes eight frequencies (two pieces of 16 bytes) of several
+// heads of a token, which share its cosines and sines; neighbouring threads take neighbouring pieces, then neighbouring heads.
+#include "paged_cache.h"
+#include "weight_quant_common.h"
+
+namespace mi355 {
+namespace {
+
+constexpr int kAxes = 4;
+
+struct RopeArgs {
+    const uint16_t *in[2];             // query, key: [tokens, heads, dim]
+    uint16_t *out[2];                  // the same, contiguous
+    int64_t tok[2], head[2];           // elements between tokens and heads of the inputs
+    int heads[2];
+    const void *table;
+    int64_t table_stride, positions;   // elements between rows; rows
+    const void *pos;
+    int64_t pos_axis, pos_tok;
+    int pos64, axes, end[kAxes];       // frequencies of the axes up to and with this one
+    int dim, half;                     // half = R / 2
+    int interleaved;
+    uint32_t tokens, units;            // units = tokens * groups * pieces
+    FastDiv pieces, groups;            // pieces of a head; threads that share the heads of a token
+};
+
+__device__ __forceinline__ int64_t position(const RopeArgs &a, uint32_t token, int axis)
+{
+    const int64_t at = axis * a.pos_axis + token * a.pos_tok;
+    return a.pos64 ? static_cast<const int64_t *>(a.pos)[at] : (int64_t) static_cast<const int32_t *>(a.pos)[at];
+}
+__device__ __forceinline__ int axis_of(const RopeArgs &a, int f)
+{
+    int axis = 0;
+#pragma unroll
+    for (int i = 0; i < kAxes - 1; i++) axis += i + 1 < a.axes && f >= a.end[i];
+    return axis;
+}
+
+// TABLE: type of the cosines and sines: 0 bf16, 1 fp16, 2 float32
+template <int TABLE>
+__device__ __forceinline__ float table_1(const RopeArgs &a, int64_t at)
+{
+    if constexpr (TABLE == 2) return static_cast<const float *>(a.table)[at];
+    else return act_1<TABLE>(static_cast<const uint16_t *>(a.table)[at]);
+}
+template <int TABLE>
+__device__ __forceinline__ void table_8(const RopeArgs &a, int64_t at, float (&to)[8])
+{
+    if constexpr (TABLE == 2) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.table) + at);
+        const f32x4 lo = p[0], hi = p[1];
+#pragma unroll
+        for (int i = 0; i < 4; i++) to[i] = lo[i], to[4 + i] = hi[i];
+    } else {
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.table) + at);
+#pragma unroll
+        for (int i = 0; i < 4; i++) to[2 * i] = act_lo<TABLE>(v[i]), to[2 * i + 1] = act_hi<TABLE>(v[i]);
+    }
+}
+// one value of cosine and sine
+template <int TABLE>
+__device__ __forceinline__ void turn_of(const RopeArgs &a, uint32_t token, int f, float &c, float &s)
+{
+    const int64_t p = position(a, token, axis_of(a, f));
+    const bool there = p >= 0 && p < a.positions;
+    c = there ? table_1<TABLE>(a, p * a.table_stride + f) : 0.0f;
+    s = there ? table_1<TABLE>(a, p * a.table_stride + a.half + f) : 0.0f;
+}
+
+// Pairs (x[i], y[i]) of eight frequencies, packed in two pieces of 16 bytes
+template <bool FP16, bool INTERLEAVED>
+__device__ __forceinline__ void turn8(u32x4 &x, u32x4 &y, const float (&c)[8], const float (&s)[8])
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (INTERLEAVED) {
+            const auto turn = [&](uint32_t w, float c, float s) {
+                const float p = act_lo<FP16>(w), q = act_hi<FP16>(w);
+                return pack_act2<FP16>(p * c - q * s, q * c + p * s);
+            };
+            x[i] = turn(x[i], c[i], s[i]);
+            y[i] = turn(y[i], c[4 + i], s[4 + i]);
+        } else {
+            const float p0 = act_lo<FP16>(x[i]), p1 = act_hi<FP16>(x[i]), q0 = act_lo<FP16>(y[i]), q1 = act_hi<FP16>(y[i]);
+            const float c0 = c[2 * i], c1 = c[2 * i + 1], s0 = s[2 * i], s1 = s[2 * i + 1];
+            x[i] = pack_act2<FP16>(p0 * c0 - q0 * s0, p1 * c1 - q1 * s1);
+            y[i] = pack_act2<FP16>(q0 * c0 + p0 * s0, q1 * c1 + p1 * s1);
+        }
+    }
+}
+
+// N heads at most per thread, `groups` threads side by side for those of a token.  SPLIT: an axis may end inside eight
+// frequencies.  Rows on 16-byte boundaries, half a multiple of 8 and dim of 16.
+template <int N, bool FP16, int TABLE, bool INTERLEAVED, bool SPLIT>
+__global__ __launch_bounds__(256) void rope_kernel(RopeArgs a)
+{
+    const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
+    if (unit >= a.units) return;
+    const uint32_t rest = div_by(unit, a.pieces), piece = unit - rest * a.pieces.d;
+    const uint32_t token = div_by(rest, a.groups), first = rest - token * a.groups.d;
+    const int turned = a.half / 8, f = (int)piece * 8, heads = a.heads[0] + a.heads[1];
+    const bool copied = (int)piece >= turned;
+    // first elements of the two pieces of 8
+    const int e0 = copied || INTERLEAVED ? (int)piece * 16 : f, e1 = copied || INTERLEAVED ? e0 + 8 : a.half + f;
+
+    u32x4 x[N], y[N];
+    const auto row_in = [&](int head) {
+        const int which = head >= a.heads[0];
+        return a.in[which] + token * a.tok[which] + (head - (which ? a.heads[0] : 0)) * a.head[which];
+    };
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int head = (int)(first + i * a.groups.d);
+        if (head >= heads) continue;
+        const uint16_t *row = row_in(head);
+        x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + e0));
+        y[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + e1));
+    }
+    float c[8], s[8];
+    if (!copied) {
+        if constexpr (SPLIT) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) turn_of<TABLE>(a, token, f + i, c[i], s[i]);
+        } else {
+            const int64_t p = position(a, token, axis_of(a, f));
+            if (p >= 0 && p < a.positions) {
+                table_8<TABLE>(a, p * a.table_stride + f, c);
+                table_8<TABLE>(a, p * a.table_stride + a.half + f, s);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) c[i] = s[i] = 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int head = (int)(first + i * a.groups.d);
+        if (head >= heads) continue;
+        if (!copied) turn8<FP16, INTERLEAVED>(x[i], y[i], c, s);
+        const int which = head >= a.heads[0];
+        uint16_t *row = a.out[which] + ((int64_t)token * a.heads[which] + (head - (which ? a.heads[0] : 0))) * a.dim;
+        __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4 *>(row + e0));
+        __builtin_nontemporal_store(y[i], reinterpret_cast<u32x4 *>(row + e1));
+    }
+}
+
+// Any width, alignment and strides: a thread per pair or copied element.  pieces = half + (dim - R), groups = heads.
+template <int TABLE>
+__global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int fp16)
+{
+    const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
+    if (unit >= a.units) return;
+    const uint32_t rest = div_by(unit, a.pieces);
+    const int piece = (int)(unit - rest * a.pieces.d);
+    const uint32_t token = div_by(rest, a.groups);
+    int head = (int)(rest - token * a.groups.d);
+    const int which = head >= a.heads[0];
+    head -= which ? a.heads[0] : 0;
+    const uint16_t *row = a.in[which] + token * a.tok[which] + head * a.head[which];
+    uint16_t *out = a.out[which] + ((int64_t)token * a.heads[which] + head) * a.dim;
+    if (piece >= a.half) {
+        out[a.half + piece] = row[a.half + piece];
+        return;
+    }
+    const int e0 = a.interleaved ? 2 * piece : piece, e1 = a.interleaved ? e0 + 1 : a.half + piece;
+    float c, s;
+    turn_of<TABLE>(a, token, piece, c, s);
+    const float p = fp16 ? act_1<1>(row[e0]) : act_1<0>(row[e0]), q = fp16 ? act_1<1>(row[e1]) : act_1<0>(row[e1]);
+    const float x = p * c - q * s, y = q * c + p * s;
+    const uint32_t w = fp16 ? pack_act2<1>(x, y) : pack_act2<0>(x, y);
+    out[e0] = (uint16_t)w;
+    out[e1] = (uint16_t)(w >> 16);
+}
+
+template <int N, bool FP16, int TABLE>
+void launch_rope(const RopeArgs &a, bool split, unsigned blocks, hipStream_t s)
+{
+    const dim3 grid(blocks), block(256);
+    if (a.interleaved) {
+        if (split) hipLaunchKernelGGL((rope_kernel<N, FP16, TABLE, true, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((rope_kernel<N, FP16, TABLE, true, false>), grid, block, 0, s, a);
+    } else {
+        if (split) hipLaunchKernelGGL((rope_kernel<N, FP16, TABLE, false, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((rope_kernel<N, FP16, TABLE, false, false>), grid, block, 0, s, a);
+    }
+}
+template <int N>
+void launch_rope(const RopeArgs &a, bool fp16, int table, bool split, unsigned blocks, hipStream_t s)
+{
+    if (table == MI355_DTYPE_FP32) {
+        if (fp16) launch_rope<N, true, 2>(a, split, blocks, s);
+        else launch_rope<N, false, 2>(a, split, blocks, s);
+    } else if (fp16) {
+        launch_rope<N, true, 1>(a, split, blocks, s);
+    } else {
+        launch_rope<N, false, 0>(a, split, blocks, s);
+    }
+}
+
+// Threads of one launch at most: they are numbered in 31 bits.
+constexpr int64_t kUnitsPerLaunch = (int64_t)1 << 30;
+
+} // namespace
+} // namespace mi355
+
+extern "C" int mi355_mrope(const void *positions, int positions_dtype, int64_t positions_stride_axis, int64_t positions_stride_token, int64_t axes,
+                           const int64_t *sections, const void *query, const int64_t *query_stride, int64_t heads, const void *key,
+                           const int64_t *key_stride, int64_t kv_heads, int dtype, const void *cos_sin, int cos_sin_dtype, int64_t cos_sin_stride,
+                           int64_t max_positions, int64_t tokens, int64_t head_dim, int64_t rotary_dim, int interleaved, void *query_out,
+                           void *key_out, void *stream)
+{
+    using namespace mi355;
+    const bool fp16 = dtype == MI355_DTYPE_FP16;
+    if (tokens < 0 || heads < 0 || kv_heads < 0 || max_positions < 0 || axes < 1 || (axes > 1 && !sections)) return MI355_ERR_BAD_ARGUMENT;
+    if (rotary_dim < 2 || rotary_dim % 2 || head_dim < rotary_dim || (dtype != MI355_DTYPE_BF16 && !fp16)) return MI355_ERR_BAD_ARGUMENT;
+    if (cos_sin_dtype != dtype && cos_sin_dtype != MI355_DTYPE_FP32) return MI355_ERR_BAD_ARGUMENT;
+    if (positions_dtype != MI355_DTYPE_INT32 && positions_dtype != MI355_DTYPE_INT64) return MI355_ERR_BAD_ARGUMENT;
+    if (axes > kAxes || heads > 65535 || kv_heads > 65535 || head_dim > 65536) return MI355_ERR_UNSUPPORTED;
+    RopeArgs a;
+    a.half = (int)(rotary_dim / 2);
+    bool split = false;
+    int64_t end = 0;
+    for (int i = 0; i < kAxes; i++) {
+        if (axes > 1 && i < axes) {
+            if (sections[i] < 0 || sections[i] > a.half) return MI355_ERR_BAD_ARGUMENT;
+            end += sections[i];
+            split = split || end % 8;
+        } else if (axes == 1) {
+            end = a.half;
+        }
+        a.end[i] = (int)end;
+    }
+    if (end != a.half) return MI355_ERR_BAD_ARGUMENT;
+    if (tokens == 0 || heads + kv_heads == 0) return MI355_OK;
+    if (!positions || (max_positions > 0 && !cos_sin) || (heads > 0 && (!query || !query_stride || !query_out)) ||
+        (kv_heads > 0 && (!key || !key_stride || !key_out)))
+        return MI355_ERR_BAD_ARGUMENT;
+    const int table_bytes = cos_sin_dtype == MI355_DTYPE_FP32 ? 4 : 2, pos_bytes = positions_dtype == MI355_DTYPE_INT64 ? 8 : 4;
+    if (!aligned(query, 2) || !aligned(key, 2) || !aligned(query_out, 2) || !aligned(key_out, 2) || !aligned(cos_sin, (size_t)table_bytes) ||
+        !aligned(positions, (size_t)pos_bytes))
+        return MI355_ERR_ALIGNMENT;
+    a.heads[0] = (int)heads, a.heads[1] = (int)kv_heads;
+    bool vec = rotary_dim % 16 == 0 && head_dim % 16 == 0 && aligned(cos_sin, 16) && cos_sin_stride * table_bytes % 16 == 0;
+    const void *const in[2] = {query, key};
+    void *const out[2] = {query_out, key_out};
+    const int64_t *const stride[2] = {query_stride, key_stride};
+    for (int i = 0; i < 2; i++) {
+        const bool any = a.heads[i] > 0;
+        a.tok[i] = any ? stride[i][0] : 0, a.head[i] = any ? stride[i][1] : 0;
+        vec = vec && (!any || (aligned(in[i], 16) && aligned(out[i], 16) && a.tok[i] % 8 == 0 && a.head[i] % 8 == 0));
+    }
+    a.table = cos_sin;
+    a.table_stride = cos_sin_stride;
+    a.positions = max_positions;
+    a.pos64 = positions_dtype == MI355_DTYPE_INT64;
+    a.pos_axis = positions_stride_axis;
+    a.pos_tok = positions_stride_token;
+    a.axes = (int)axes;
+    a.dim = (int)head_dim;
+    a.interleaved = interleaved != 0;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t all = heads + kv_heads, pieces = vec ? head_dim / 16 : a.half + (head_dim - rotary_dim);
+    const bool many = all * pieces * tokens >= (int64_t)kNumCU * 8 * 256;
+    const int64_t per_thread = !vec ? 1 : many ? 4 : 1, groups = (all + per_thread - 1) / per_thread;
+    a.pieces = fast_div((uint32_t)pieces);
+    a.groups = fast_div((uint32_t)groups);
+    const int64_t most = kUnitsPerLaunch / (groups * pieces) > 0 ? kUnitsPerLaunch / (groups * pieces) : 1;
+    if (groups * pieces > 0x7fffff00) return MI355_ERR_UNSUPPORTED;
+    for (int64_t t0 = 0; t0 < tokens; t0 += most) {
+        a.tokens = (uint32_t)(tokens - t0 < most ? tokens - t0 : most);
+        a.units = (uint32_t)(a.tokens * groups * pieces);
+        a.pos = static_cast<const char *>(positions) + t0 * positions_stride_token * pos_bytes;
+        for (int i = 0; i < 2; i++) {
+            a.in[i] = static_cast<const uint16_t *>(in[i]) + t0 * a.tok[i];
+            a.out[i] = static_cast<uint16_t *>(out[i]) + t0 * a.heads[i] * head_dim;
+        }
+        const unsigned blocks = (a.units + 255) / 256;
+        if (vec && many) launch_rope<4>(a, fp16, cos_sin_dtype, split, blocks, s);
+        else if (vec) launch_rope<1>(a, fp16, cos_sin_dtype, split, blocks, s);
+        else if (cos_sin_dtype == MI355_DTYPE_FP32) hipLaunchKernelGGL(rope_any_kernel<2>, dim3(blocks), dim3(256), 0, s, a, fp16);
+        else if (fp16) hipLaunchKernelGGL(rope_any_kernel<1>, dim3(blocks), dim3(256), 0, s, a, 1);
+        else hipLaunchKernelGGL(rope_any_kernel<0>, dim3(blocks), dim3(256), 0, s, a, 0);
+    }
+    return check_launch();
+}

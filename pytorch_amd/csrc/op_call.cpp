@@ -88,6 +88,55 @@ struct Arg<std::optional<double>> {
     std::optional<double> get() const { return v; }
 };
 template <>
+struct Arg<double> {
+    double v = 0.0;
+    bool load(PyObject *o)
+    {
+        if (!PyFloat_CheckExact(o)) return false;
+        v = PyFloat_AS_DOUBLE(o);
+        return true;
+    }
+    bool load_default(const c10::IValue &d) { return d.isDouble() ? (v = d.toDouble(), true) : false; }
+    double get() const { return v; }
+};
+template <>
+struct Arg<at::OptionalIntArrayRef> {
+    std::optional<c10::SmallVector<int64_t, 4>> v;
+    bool load(PyObject *o)
+    {
+        if (o == Py_None) return true;
+        if (!PyList_CheckExact(o) && !PyTuple_CheckExact(o)) return false;
+        v.emplace();
+        for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(o); i++) {
+            PyObject *e = PySequence_Fast_GET_ITEM(o, i);
+            int overflow = 0;
+            if (!PyLong_CheckExact(e)) return false;
+            v->push_back(PyLong_AsLongLongAndOverflow(e, &overflow));
+            if (overflow) return false;
+        }
+        return true;
+    }
+    bool load_default(const c10::IValue &d) { return d.isNone(); }
+    at::OptionalIntArrayRef get() const { return v ? at::OptionalIntArrayRef(at::IntArrayRef(*v)) : at::OptionalIntArrayRef(); }
+};
+template <>
+struct Arg<c10::string_view> {
+    c10::string_view v;                                    // the Python object, or the schema's default, outlives the call
+    bool load(PyObject *o)
+    {
+        Py_ssize_t size = 0;
+        const char *text = PyUnicode_CheckExact(o) ? PyUnicode_AsUTF8AndSize(o, &size) : nullptr;
+        if (!text) {
+            PyErr_Clear();
+            return false;
+        }
+        v = c10::string_view(text, (size_t)size);
+        return true;
+    }
+    bool load_default(const c10::IValue &d) { return d.isString() ? (v = d.toStringView(), true) : false; }
+    c10::string_view get() const { return v; }
+};
+template <>
 struct Arg<bool> {
     bool v = false;
     bool load(PyObject *o)
@@ -296,6 +345,9 @@ using PagedAttention = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &
                                                   const OptTensor &, std::optional<double>, const OptTensor &, const OptTensor &, bool);
 using PagedEvict = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
                                                       int64_t, int64_t, const OptTensor &, const OptTensor &);
+using AddRmsNorm = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const OptTensor &, const Tensor &, double);
+using Mrope = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, int64_t, at::OptionalIntArrayRef,
+                                         c10::string_view);
 using Quantize = Tensor(const Tensor &, const Tensor &, const OptTensor &, at::ScalarType, int64_t, bool);
 
 // ---- forward passes of the contrib modules.  A module stores [out_features, in_features] weights and [N, G] parameters and the
@@ -383,7 +435,10 @@ PyObject *install(PyObject *, PyObject *args)
                     install_one<struct T9, PagedWrite>(namespace_, "npu_paged_cache_write") &&
                     install_one<struct T10, PagedRead>(namespace_, "npu_paged_cache_read") &&
                     install_one<struct T11, PagedAttention>(namespace_, "npu_paged_decode_attention") &&
-                    install_one<struct T12, PagedEvict>(namespace_, "npu_paged_cache_evict");
+                    install_one<struct T12, PagedEvict>(namespace_, "npu_paged_cache_evict") &&
+                    install_one<struct T13, AddRmsNorm>(namespace_, "npu_add_rms_norm") &&
+                    install_one<struct T14, AddRmsNorm>(namespace_, "npu_add_rms_norm_dynamic_quant") &&
+                    install_one<struct T15, Mrope>(namespace_, "npu_mrope");
     if (!ok) return nullptr;
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
