@@ -45,6 +45,7 @@ typedef enum mi355_status {
 #define MI355_DTYPE_INT32 3  /* likewise */
 #define MI355_DTYPE_INT8 4   /* likewise */
 #define MI355_DTYPE_INT64 5  /* likewise */
+#define MI355_DTYPE_INT4 6   /* int32 words of eight codes in two's complement, the first in the lowest bits; likewise */
 
 /* Output formats of mi355_quant_matmul. */
 #define MI355_OUT_BF16 0
@@ -465,27 +466,35 @@ int mi355_mrope(const void *positions, int positions_dtype, int64_t positions_st
  */
 typedef struct mi355_paged_cache {
     void *key, *value;                    /* [num_blocks, block_size, kv_heads, head_dim] of dtype, the last dimension contiguous */
-    float *key_scale, *value_scale;       /* [num_blocks, block_size, kv_heads] for int8 (element = code * scale), else NULL */
-    int dtype;                            /* MI355_DTYPE_BF16, MI355_DTYPE_FP16 or MI355_DTYPE_INT8 */
-    int64_t num_blocks, block_size, kv_heads, head_dim;   /* num_blocks * block_size < 2^31 */
-    int64_t key_stride[3], value_stride[3];               /* elements between blocks, tokens and heads */
+    float *key_scale, *value_scale;       /* [num_blocks, block_size, kv_heads] for int8 (element = code * scale) and int4, else NULL */
+    int dtype;                            /* MI355_DTYPE_BF16, MI355_DTYPE_FP16, MI355_DTYPE_INT8 or MI355_DTYPE_INT4 */
+    int64_t num_blocks, block_size, kv_heads, head_dim;   /* num_blocks * block_size < 2^31; int4: head_dim a multiple of 8 */
+    int64_t key_stride[3], value_stride[3];               /* elements (int4: words) between blocks, tokens and heads */
     int64_t key_scale_stride[3], value_scale_stride[3];
+    /* Looked at for int4 alone, so a caller's structure may end above for the other types. */
+    float *key_offset, *value_offset;     /* [num_blocks, block_size, kv_heads]: element = (code + offset) * scale */
+    int64_t key_offset_stride[3], value_offset_stride[3];
 } mi355_paged_cache;
 
 /*
  * Writes the keys and values of new tokens into their slots.
- *   key, value  [tokens, kv_heads, head_dim] of dtype (bf16 / fp16; the cache's own type unless that is int8), the last
+ *   key, value  [tokens, kv_heads, head_dim] of dtype (bf16 / fp16; the cache's own type unless that holds codes), the last
  *               dimension contiguous; *_stride[0], *_stride[1]: elements between tokens and between heads
  *   slots       [tokens] int32 or int64 (slots_dtype), distinct; a token whose slot lies outside the cache is skipped
  * An int8 cache gets, per token and head, scale = max_d |x_d| / 127 and code_d = rint_half_even(x_d / scale), the rule of
- * mi355_dynamic_quant, and the scale.
+ * mi355_dynamic_quant, and the scale.  An int4 cache gets, with lo and hi the least and the largest x_d, in float32, every operation
+ * rounded by itself:
+ *   scale = (hi - lo) / 15     offset = lo / scale + 8     code_d = rint_half_even((x_d - lo) * 15 / (hi - lo)) - 8
+ * where hi - lo is at most 2^-120 scale 1, offset lo and codes of 0.  A row with a NaN or an infinity, or whose hi - lo is more
+ * than 2^124, comes back as NaN.
  */
 int mi355_paged_cache_write(const mi355_paged_cache *cache, const void *key, const int64_t *key_stride, const void *value,
                             const int64_t *value_stride, int dtype, const void *slots, int slots_dtype, int64_t tokens, void *stream);
 
 /*
  * Copies the tokens of `slots` out of the cache, in their order: key, value [tokens, kv_heads, head_dim] of dtype (the
- * cache's own type; from int8 bf16 or fp16, round(code * scale)).  A slot outside the cache gives zeros.
+ * cache's own type; from codes bf16 or fp16, round(code * scale) or round((code + offset) * scale)).  A slot outside the cache
+ * gives zeros.
  */
 int mi355_paged_cache_read(const mi355_paged_cache *cache, void *key, const int64_t *key_stride, void *value,
                            const int64_t *value_stride, int dtype, const void *slots, int slots_dtype, int64_t tokens, void *stream);
@@ -499,7 +508,7 @@ int mi355_paged_cache_read(const mi355_paged_cache *cache, void *key, const int6
  *   attn_sums[b, kv head, j] += sum over the kv head's query heads of exp(s_j - lse)
  * Scores, sums and outputs are accumulated in float32.  Where nothing is seen out is 0 and lse -infinity.  Values and keys
  * that are not seen have no influence, NaN included.
- *   q             [batch, heads, head_dim] of q_dtype (the cache's own type; bf16 or fp16 with int8), strides in elements
+ *   q             [batch, heads, head_dim] of q_dtype (the cache's own type; bf16 or fp16 with int8 and int4), strides in elements
  *   out           [batch, heads, head_dim] of q_dtype, contiguous; lse float32 [batch, heads] or NULL
  *   block_table   int32 [batch, max_blocks], rows table_stride elements apart; entries outside [0, num_blocks) name no block
  *   context_lens  int32 [batch], clamped to [0, max_blocks * block_size]
@@ -528,7 +537,7 @@ int mi355_paged_decode_attention(const mi355_paged_cache *cache, const void *q, 
  *                            weight and the token's position in its sequence; strides in elements, places contiguous
  *   new_lens                 int32 [batch]: min(n, keep)
  *   new_sums, new_positions  contiguous, the same shape: moved like the tokens; 0 and -1 from place new_lens on
- * Cache rows (and int8 scales) are moved in place.  A row whose old or new block the table does not name is not moved.
+ * Cache rows (and their scales and offsets) are moved in place.  A row whose old or new block the table does not name is not moved.
  * Sequences must not share blocks.  workspace: mi355_paged_cache_evict_workspace() bytes, 16-byte aligned.
  */
 size_t mi355_paged_cache_evict_workspace(int64_t batch, int64_t kv_heads, int64_t max_blocks, int64_t block_size, int64_t keep);

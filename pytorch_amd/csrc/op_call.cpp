@@ -339,12 +339,15 @@ using SwigluQuant = std::tuple<Tensor, Tensor>(const Tensor &, const OptTensor &
                                                OptType);
 using AntiQuant = Tensor(const Tensor &, const Tensor &, const OptTensor &, OptType, OptType);
 using TransParam = Tensor(const Tensor &, const OptTensor &);
-using PagedWrite = void(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const OptTensor &, const OptTensor &);
-using PagedRead = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const OptTensor &, const OptTensor &, OptType);
+using PagedWrite = void(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const OptTensor &, const OptTensor &,
+                        const OptTensor &, const OptTensor &);
+using PagedRead = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const OptTensor &, const OptTensor &, OptType,
+                                             const OptTensor &, const OptTensor &);
 using PagedAttention = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const OptTensor &,
-                                                  const OptTensor &, std::optional<double>, const OptTensor &, const OptTensor &, bool);
+                                                  const OptTensor &, std::optional<double>, const OptTensor &, const OptTensor &, bool, const OptTensor &,
+                                                  const OptTensor &);
 using PagedEvict = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
-                                                      int64_t, int64_t, const OptTensor &, const OptTensor &);
+                                                      int64_t, int64_t, const OptTensor &, const OptTensor &, const OptTensor &, const OptTensor &);
 using AddRmsNorm = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const OptTensor &, const Tensor &, double);
 using Mrope = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, int64_t, at::OptionalIntArrayRef,
                                          c10::string_view);

@@ -22,13 +22,13 @@ inline FastDiv fast_div(uint32_t d)
 }
 __host__ __device__ inline uint32_t div_by(uint32_t n, const FastDiv &f) { return (uint32_t)(((uint64_t)n * f.mul) >> f.shift); }
 
-// One of the four arrays of a cache; strides in bytes.
+// One of the arrays of a cache; strides in bytes.
 struct PagedArray {
     char *base;
     int64_t block, token, head;
 };
 struct PagedCache {
-    PagedArray key, value, key_scale, value_scale;
+    PagedArray key, value, key_scale, value_scale, key_offset, value_offset;     // the last four: null where there are none
     FastDiv page;
     int num_blocks, heads, dim;
     int slots;                      // num_blocks * block_size
@@ -40,19 +40,23 @@ struct PagedCache {
     }
 };
 
-inline int cache_elem_bytes(int dtype) { return dtype == MI355_DTYPE_INT8 ? 1 : 2; }
+inline int cache_bits(int dtype) { return dtype == MI355_DTYPE_INT4 ? 4 : dtype == MI355_DTYPE_INT8 ? 8 : 16; }
+// what a row is addressed in: elements, or words of eight codes
+inline int cache_elem_bytes(int dtype) { return dtype == MI355_DTYPE_INT4 ? 4 : dtype == MI355_DTYPE_INT8 ? 1 : 2; }
 
 // Checks a descriptor and translates it; MI355_OK or the status to return.
 inline int open_cache(const mi355_paged_cache *c, PagedCache *out)
 {
     if (!c || !c->key || !c->value || c->num_blocks < 1 || c->block_size < 1 || c->kv_heads < 1 || c->head_dim < 1) return MI355_ERR_BAD_ARGUMENT;
-    const bool quantised = c->dtype == MI355_DTYPE_INT8;
+    const bool int4 = c->dtype == MI355_DTYPE_INT4, quantised = int4 || c->dtype == MI355_DTYPE_INT8;
     if (!quantised && c->dtype != MI355_DTYPE_BF16 && c->dtype != MI355_DTYPE_FP16) return MI355_ERR_BAD_ARGUMENT;
     if (quantised != (c->key_scale != nullptr) || quantised != (c->value_scale != nullptr)) return MI355_ERR_BAD_ARGUMENT;
+    if (int4 && (!c->key_offset || !c->value_offset || c->head_dim % 8)) return MI355_ERR_BAD_ARGUMENT;
     constexpr int64_t kMost = 0x7fffffff;                  // slots are numbered in 31 bits; byte offsets have 64
     if (c->block_size > kMost || c->num_blocks > kMost / c->block_size || c->kv_heads > 65535 || c->head_dim > 65536) return MI355_ERR_UNSUPPORTED;
     const int size = cache_elem_bytes(c->dtype);
-    if (!aligned(c->key, size) || !aligned(c->value, size) || (quantised && (!aligned(c->key_scale, 4) || !aligned(c->value_scale, 4))))
+    if (!aligned(c->key, size) || !aligned(c->value, size) || (quantised && (!aligned(c->key_scale, 4) || !aligned(c->value_scale, 4))) ||
+        (int4 && (!aligned(c->key_offset, 4) || !aligned(c->value_offset, 4))))
         return MI355_ERR_ALIGNMENT;
     const auto array = [](void *p, const int64_t *stride, int64_t bytes) {
         return PagedArray{static_cast<char *>(p), p ? stride[0] * bytes : 0, p ? stride[1] * bytes : 0, p ? stride[2] * bytes : 0};
@@ -61,6 +65,11 @@ inline int open_cache(const mi355_paged_cache *c, PagedCache *out)
     out->value = array(c->value, c->value_stride, size);
     out->key_scale = array(c->key_scale, c->key_scale_stride, 4);
     out->value_scale = array(c->value_scale, c->value_scale_stride, 4);
+    out->key_offset = out->value_offset = PagedArray{nullptr, 0, 0, 0};
+    if (int4) {
+        out->key_offset = array(c->key_offset, c->key_offset_stride, 4);
+        out->value_offset = array(c->value_offset, c->value_offset_stride, 4);
+    }
     out->page = fast_div((uint32_t)c->block_size);
     out->num_blocks = (int)c->num_blocks;
     out->heads = (int)c->kv_heads;

@@ -1,9 +1,14 @@
 // npu_paged_cache_write and npu_paged_cache_read for gfx950: rows of head_dim elements between [tokens, heads, dim] tensors
-// and the slots of a paged cache, as they are or as int8 codes with one float32 scale per row.
+// and the slots of a paged cache, as they are, as int8 codes with one float32 scale per row, or as int4 codes, eight to a word,
+// with one scale and one offset.
 //
 // Per row and plane (keys, values), with float32 arithmetic rounded operation by operation:
 //   write int8   scale = max_d |x_d| / 127,  code_d = rint_half_even(x_d / scale)      (npu_dynamic_quant's rule)
 //   read  int8   x_d = round(code_d * scale)
+//   write int4   lo, hi = min_d, max_d x_d; scale = (hi - lo) / 15; offset = lo / scale + 8
+//                code_d = rint_half_even((x_d - lo) * 15 / (hi - lo)) - 8: a value between two codes is told exactly as long as x_d - lo
+//                has 20 bits;  hi - lo <= 2^-120: scale 1, offset lo, codes 0
+//   read  int4   x_d = round((code_d + offset) * scale)
 // Both only move bytes.  A row is handled by a group of 8, 16 or 32 lanes with 8 elements each, so the maximum of a row takes
 // three to five lane exchanges and no barrier, and a wavefront's loads cover whole rows.
 //
@@ -73,10 +78,76 @@ struct RowQuant {
     }
 };
 
+// (x - lo) * 15 / (hi - lo), rounded to the nearest integer, of a row between lo and hi.  With r = 1 / (hi - lo) correctly rounded,
+// one correction of t * r by its residual gives one of the two floats next to the quotient, and by Markstein's theorem a second
+// one the correctly rounded quotient, where nothing leaves the normal range: for hi - lo in [2^-60, 2^60] only quotients below 2^-40
+// do, which round to 0 either way.  The sum with 1.5 * 2^23 rounds, ties to even; its low bits are the number, 0 to 15.
+struct RowQuant4 {
+    float lo, span, scale, offset, r;
+    bool flat, fast, finite;
+    __device__ RowQuant4(float lo_, float hi) : lo(lo_), span(hi - lo_)
+    {
+        flat = span <= 0x1p-120f;
+        finite = span <= 0x1p124f;                           // 15 times it is a number (false for NaN)
+        scale = flat ? 1.0f : finite ? span / 15.0f : NAN;
+        offset = flat ? lo : lo / scale + 8.0f;
+        r = 1.0f / span;
+        fast = span >= 0x1p-60f && span <= 0x1p60f;
+    }
+    // the code plus 8
+    __device__ __forceinline__ uint32_t operator()(float x) const
+    {
+        const float t = (x - lo) * 15.0f;
+        if (fast) {
+            float q = t * r;
+            q = __builtin_fmaf(__builtin_fmaf(-span, q, t), r, q);
+            q = __builtin_fmaf(__builtin_fmaf(-span, q, t), r, q);
+            return __float_as_uint(q + 12582912.0f) & 15u;
+        }
+        if (flat) return 8;
+        return finite ? (uint32_t)(int)__builtin_rintf(t / span) & 15u : 0;
+    }
+};
+// codes of eight elements in a word
+template <bool FP16>
+__device__ __forceinline__ uint32_t quant_word(const RowQuant4 &q, u32x4 v)
+{
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w |= q(act_lo<FP16>(v[i])) << (8 * i) | q(act_hi<FP16>(v[i])) << (8 * i + 4);
+    return w ^ 0x88888888u;                                  // u - 8 in two's complement
+}
+// 16-bit values as integers in their order (and back: its own inverse); NaN lies beyond the infinities
+__device__ __forceinline__ uint32_t order16(uint32_t two)
+{
+    typedef int16_t ss2 __attribute__((ext_vector_type(2)));
+    const ss2 x = __builtin_bit_cast(ss2, two);
+    return two ^ (__builtin_bit_cast(uint32_t, x >> (int16_t)15) & 0x7fff7fffu);
+}
+__device__ __forceinline__ uint32_t max16(uint32_t x, uint32_t y)
+{
+    typedef int16_t ss2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ss2, x), __builtin_bit_cast(ss2, y)));
+}
+// [largest, largest of the complements] of eight values, in the low and the high half
+__device__ __forceinline__ uint32_t range8(u32x4 v)
+{
+    const uint32_t a = order16(v.x), b = order16(v.y), c = order16(v.z), d = order16(v.w);
+    const uint32_t top = max16(max16(a, b), max16(c, d)), low = max16(max16(~a, ~b), max16(~c, ~d));
+    return max16(__builtin_amdgcn_perm(low, top, 0x05040100u), __builtin_amdgcn_perm(low, top, 0x07060302u));
+}
+constexpr uint32_t kNoRange = 0x80008000u;                   // of no values: below everything
+template <bool FP16>
+__device__ __forceinline__ RowQuant4 quant_of(uint32_t range)
+{
+    return RowQuant4(act_1<FP16>((uint16_t)order16(~range >> 16)), act_1<FP16>((uint16_t)order16(range & 0xffffu)));
+}
+__device__ __forceinline__ float nibble_f32(uint32_t w, int i) { return (float)((int32_t)(w << (28 - 4 * i)) >> 28); }
+
 // GL lanes per row, eight elements per lane: rows that start on 16-byte boundaries, dim % 8 == 0 and <= 8 GL.  N heads of a
 // token per group of lanes: slot and addresses are worked out once (they were half of the instructions, and the int8 writer
-// is bound by those), the rows requested together.  QUANT: int8 cache; FP16: the 16-bit type (for the conversions alone).
-template <int GL, int N, bool QUANT, bool FP16>
+// is bound by those), the rows requested together.  BITS: of the cache's elements; FP16: the 16-bit type (for the conversions alone).
+template <int GL, int N, int BITS, bool FP16>
 __global__ __launch_bounds__(256) void paged_write_kernel(RowArgs a)
 {
     const int plane = blockIdx.y, lane = threadIdx.x % GL;
@@ -92,12 +163,25 @@ __global__ __launch_bounds__(256) void paged_write_kernel(RowArgs a)
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = mine ? *reinterpret_cast<const u32x4 *>(src + i * a.head[plane]) : u32x4{0, 0, 0, 0};
     if (slot < 0 || slot >= a.cache.slots) return;
-    char *dst = to.base + a.cache.offset(to, (uint32_t)slot, (int)(part * N)) + lane * (QUANT ? 8 : 16);
-    char *scale = QUANT ? sc.base + a.cache.offset(sc, (uint32_t)slot, (int)(part * N)) : nullptr;
+    char *dst = to.base + a.cache.offset(to, (uint32_t)slot, (int)(part * N)) + lane * BITS;
+    char *scale = BITS < 16 ? sc.base + a.cache.offset(sc, (uint32_t)slot, (int)(part * N)) : nullptr;
+    const PagedArray &of = plane ? a.cache.value_offset : a.cache.key_offset;
+    char *offset = BITS == 4 ? of.base + a.cache.offset(of, (uint32_t)slot, (int)(part * N)) : nullptr;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        if constexpr (!QUANT) {
+        if constexpr (BITS == 16) {
             if (mine) *reinterpret_cast<u32x4 *>(dst + i * to.head) = v[i];
+        } else if constexpr (BITS == 4) {
+            uint32_t range = mine ? range8(v[i]) : kNoRange;
+#pragma unroll
+            for (int off = GL / 2; off >= 1; off >>= 1) range = max16(range, (uint32_t)__shfl_xor((int)range, off, GL));
+            const RowQuant4 q = quant_of<FP16>(range);
+            const uint32_t word = quant_word<FP16>(q, v[i]);
+            if (mine) *reinterpret_cast<uint32_t *>(dst + i * to.head) = word;
+            if (lane == 0) {
+                *reinterpret_cast<float *>(scale + i * sc.head) = q.scale;
+                *reinterpret_cast<float *>(offset + i * of.head) = q.offset;
+            }
         } else {
             uint32_t m = absmax8(v[i]);
 #pragma unroll
@@ -113,7 +197,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(RowArgs a)
 }
 
 // Any width, alignment and strides: one wavefront per row, element by element, each a trip of its own.
-template <bool QUANT>
+template <int BITS>
 __global__ __launch_bounds__(256) void paged_write_any_kernel(RowArgs a, int fp16)
 {
     const int plane = blockIdx.y, lane = threadIdx.x % 64;
@@ -126,8 +210,28 @@ __global__ __launch_bounds__(256) void paged_write_any_kernel(RowArgs a, int fp1
     const uint16_t *x = a.plane[plane] + t * a.tok[plane] + h * a.head[plane];
     const PagedArray &to = plane ? a.cache.value : a.cache.key;
     char *dst = to.base + a.cache.offset(to, (uint32_t)slot, (int)h);
-    if constexpr (!QUANT) {
+    if constexpr (BITS == 16) {
         for (int d = lane; d < a.cache.dim; d += 64) reinterpret_cast<uint16_t *>(dst)[d] = x[d];
+    } else if constexpr (BITS == 4) {
+        uint32_t range = kNoRange;
+        for (int d = lane; d < a.cache.dim; d += 64) {
+            const uint32_t o = order16(x[d]) & 0xffffu;
+            range = max16(range, o | ~o << 16);
+        }
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) range = max16(range, (uint32_t)__shfl_xor((int)range, off, 64));
+        const RowQuant4 q = fp16 ? quant_of<true>(range) : quant_of<false>(range);
+        for (int w = lane; w < a.cache.dim / 8; w += 64) {
+            u32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = x[8 * w + 2 * i] | (uint32_t)x[8 * w + 2 * i + 1] << 16;
+            reinterpret_cast<uint32_t *>(dst)[w] = fp16 ? quant_word<true>(q, v) : quant_word<false>(q, v);
+        }
+        if (lane == 0) {
+            const PagedArray &s = plane ? a.cache.value_scale : a.cache.key_scale, &o = plane ? a.cache.value_offset : a.cache.key_offset;
+            *reinterpret_cast<float *>(s.base + a.cache.offset(s, (uint32_t)slot, (int)h)) = q.scale;
+            *reinterpret_cast<float *>(o.base + a.cache.offset(o, (uint32_t)slot, (int)h)) = q.offset;
+        }
     } else {
         uint32_t m = 0;
         for (int d = lane; d < a.cache.dim; d += 64) m = max(m, (uint32_t)(x[d] & 0x7fffu));
@@ -142,7 +246,7 @@ __global__ __launch_bounds__(256) void paged_write_any_kernel(RowArgs a, int fp1
     }
 }
 
-template <int GL, int N, bool QUANT, bool FP16>
+template <int GL, int N, int BITS, bool FP16>
 __global__ __launch_bounds__(256) void paged_read_kernel(RowArgs a)
 {
     const int plane = blockIdx.y, lane = threadIdx.x % GL;
@@ -154,8 +258,24 @@ __global__ __launch_bounds__(256) void paged_read_kernel(RowArgs a)
     const int64_t slot = load_slot(a, t);
     u32x4 v[N] = {};
     if (slot >= 0 && slot < a.cache.slots) {
-        const char *src = from.base + a.cache.offset(from, (uint32_t)slot, (int)(part * N)) + lane * (QUANT ? 8 : 16);
-        if constexpr (QUANT) {
+        const char *src = from.base + a.cache.offset(from, (uint32_t)slot, (int)(part * N)) + lane * BITS;
+        if constexpr (BITS == 4) {
+            const PagedArray &of = plane ? a.cache.value_offset : a.cache.key_offset;
+            const char *at = sc.base + a.cache.offset(sc, (uint32_t)slot, (int)(part * N)), *at_of = of.base + a.cache.offset(of, (uint32_t)slot, (int)(part * N));
+            uint32_t w[N];
+            float scale[N], offset[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                w[i] = *reinterpret_cast<const uint32_t *>(src + i * from.head);
+                scale[i] = *reinterpret_cast<const float *>(at + i * sc.head);
+                offset[i] = *reinterpret_cast<const float *>(at_of + i * of.head);
+            }
+#pragma unroll
+            for (int i = 0; i < N; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    v[i][k] = pack_act2<FP16>((nibble_f32(w[i], 2 * k) + offset[i]) * scale[i], (nibble_f32(w[i], 2 * k + 1) + offset[i]) * scale[i]);
+        } else if constexpr (BITS == 8) {
             const char *at = sc.base + a.cache.offset(sc, (uint32_t)slot, (int)(part * N));
             u32x2 c[N];
             float scale[N];
@@ -181,7 +301,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(RowArgs a)
     for (int i = 0; i < N; i++) __builtin_nontemporal_store(v[i], reinterpret_cast<u32x4 *>(dst + i * a.head[plane]));
 }
 
-template <bool QUANT>
+template <int BITS>
 __global__ __launch_bounds__(256) void paged_read_any_kernel(RowArgs a, int fp16)
 {
     const int plane = blockIdx.y, lane = threadIdx.x % 64;
@@ -195,12 +315,14 @@ __global__ __launch_bounds__(256) void paged_read_any_kernel(RowArgs a, int fp16
     const PagedArray &from = plane ? a.cache.value : a.cache.key;
     const PagedArray &s = plane ? a.cache.value_scale : a.cache.key_scale;
     const char *src = there ? from.base + a.cache.offset(from, (uint32_t)slot, (int)h) : nullptr;
-    const float scale = QUANT && there ? *reinterpret_cast<const float *>(s.base + a.cache.offset(s, (uint32_t)slot, (int)h)) : 0.0f;
+    const float scale = BITS < 16 && there ? *reinterpret_cast<const float *>(s.base + a.cache.offset(s, (uint32_t)slot, (int)h)) : 0.0f;
+    const PagedArray &of = plane ? a.cache.value_offset : a.cache.key_offset;
+    const float offset = BITS == 4 && there ? *reinterpret_cast<const float *>(of.base + a.cache.offset(of, (uint32_t)slot, (int)h)) : 0.0f;
     for (int d = lane; d < a.cache.dim; d += 64) {
         uint16_t o = 0;
         if (there) {
-            if constexpr (QUANT) {
-                const float f = (float)(int8_t)src[d] * scale;
+            if constexpr (BITS < 16) {
+                const float f = BITS == 4 ? (nibble_f32(reinterpret_cast<const uint32_t *>(src)[d / 8], d % 8) + offset) * scale : (float)(int8_t)src[d] * scale;
                 o = fp16 ? (uint16_t)pack_act2<1>(f, 0.0f) : (uint16_t)pack_act2<0>(f, 0.0f);
             } else {
                 o = reinterpret_cast<const uint16_t *>(src)[d];
@@ -219,50 +341,47 @@ void number_groups(RowArgs &a, int n)
 }
 
 template <bool WRITE, int GL, int N>
-void launch_rows(RowArgs &a, bool quant, bool fp16, hipStream_t s)
+void launch_rows(RowArgs &a, int bits, bool fp16, hipStream_t s)
 {
     number_groups(a, N);
     const dim3 grid((a.groups + 256 / GL - 1) / (256 / GL), 2);
+    const auto with = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
     if constexpr (WRITE) {
-        if (!quant) hipLaunchKernelGGL((paged_write_kernel<GL, N, false, false>), grid, dim3(256), 0, s, a);
-        else if (fp16) hipLaunchKernelGGL((paged_write_kernel<GL, N, true, true>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((paged_write_kernel<GL, N, true, false>), grid, dim3(256), 0, s, a);
+        if (bits == 16) with(paged_write_kernel<GL, N, 16, false>);
+        else if (bits == 8) fp16 ? with(paged_write_kernel<GL, N, 8, true>) : with(paged_write_kernel<GL, N, 8, false>);
+        else fp16 ? with(paged_write_kernel<GL, N, 4, true>) : with(paged_write_kernel<GL, N, 4, false>);
     } else {
-        if (!quant) hipLaunchKernelGGL((paged_read_kernel<GL, N, false, false>), grid, dim3(256), 0, s, a);
-        else if (fp16) hipLaunchKernelGGL((paged_read_kernel<GL, N, true, true>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((paged_read_kernel<GL, N, true, false>), grid, dim3(256), 0, s, a);
+        if (bits == 16) with(paged_read_kernel<GL, N, 16, false>);
+        else if (bits == 8) fp16 ? with(paged_read_kernel<GL, N, 8, true>) : with(paged_read_kernel<GL, N, 8, false>);
+        else fp16 ? with(paged_read_kernel<GL, N, 4, true>) : with(paged_read_kernel<GL, N, 4, false>);
     }
 }
 template <bool WRITE, int GL>
-void launch_rows(RowArgs &a, bool quant, bool fp16, hipStream_t s)
+void launch_rows(RowArgs &a, int bits, bool fp16, hipStream_t s)
 {
     // One row per group of lanes while that leaves the card short of workgroups.  Beyond: 8192 tokens to int8, 8 heads of 128,
     // 14.3 us with one row per group, 13.2 with two, 13.9 with four; 32768 tokens from int8 33.6, 31.3 and 31.2.
     const bool many = (int64_t)a.tokens * a.cache.heads * 2 / (256 / GL) >= kNumCU * 16;
-    if (many && !WRITE && a.cache.heads % 4 == 0) launch_rows<WRITE, GL, 4>(a, quant, fp16, s);
-    else if (many && a.cache.heads % 2 == 0) launch_rows<WRITE, GL, 2>(a, quant, fp16, s);
-    else launch_rows<WRITE, GL, 1>(a, quant, fp16, s);
+    if (many && !WRITE && a.cache.heads % 4 == 0) launch_rows<WRITE, GL, 4>(a, bits, fp16, s);
+    else if (many && a.cache.heads % 2 == 0) launch_rows<WRITE, GL, 2>(a, bits, fp16, s);
+    else launch_rows<WRITE, GL, 1>(a, bits, fp16, s);
 }
 
 template <bool WRITE>
-void launch_tokens(RowArgs &a, bool vec, bool quant, bool fp16, hipStream_t s)
+void launch_tokens(RowArgs &a, bool vec, int bits, bool fp16, hipStream_t s)
 {
     if (!vec) {
         number_groups(a, 1);
         const dim3 grid((a.groups + 3) / 4, 2);
-        if constexpr (WRITE) {
-            if (quant) hipLaunchKernelGGL(paged_write_any_kernel<true>, grid, dim3(256), 0, s, a, fp16);
-            else hipLaunchKernelGGL(paged_write_any_kernel<false>, grid, dim3(256), 0, s, a, fp16);
-        } else {
-            if (quant) hipLaunchKernelGGL(paged_read_any_kernel<true>, grid, dim3(256), 0, s, a, fp16);
-            else hipLaunchKernelGGL(paged_read_any_kernel<false>, grid, dim3(256), 0, s, a, fp16);
-        }
+        const auto with = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, fp16); };
+        if constexpr (WRITE) bits == 16 ? with(paged_write_any_kernel<16>) : bits == 8 ? with(paged_write_any_kernel<8>) : with(paged_write_any_kernel<4>);
+        else bits == 16 ? with(paged_read_any_kernel<16>) : bits == 8 ? with(paged_read_any_kernel<8>) : with(paged_read_any_kernel<4>);
     } else if (a.cache.dim <= 64) {
-        launch_rows<WRITE, 8>(a, quant, fp16, s);
+        launch_rows<WRITE, 8>(a, bits, fp16, s);
     } else if (a.cache.dim <= 128) {
-        launch_rows<WRITE, 16>(a, quant, fp16, s);
+        launch_rows<WRITE, 16>(a, bits, fp16, s);
     } else {
-        launch_rows<WRITE, 32>(a, quant, fp16, s);
+        launch_rows<WRITE, 32>(a, bits, fp16, s);
     }
 }
 
@@ -276,8 +395,8 @@ int move_rows(const mi355_paged_cache *cache, int dtype, void *key, const int64_
 {
     RowArgs a;
     if (const int st = open_cache(cache, &a.cache); st != MI355_OK) return st;
-    const bool quant = cache->dtype == MI355_DTYPE_INT8;
-    if (tokens < 0 || (dtype != MI355_DTYPE_BF16 && dtype != MI355_DTYPE_FP16) || (!quant && cache->dtype != dtype)) return MI355_ERR_BAD_ARGUMENT;
+    const int bits = cache_bits(cache->dtype);
+    if (tokens < 0 || (dtype != MI355_DTYPE_BF16 && dtype != MI355_DTYPE_FP16) || (bits == 16 && cache->dtype != dtype)) return MI355_ERR_BAD_ARGUMENT;
     if (slots_dtype != MI355_DTYPE_INT32 && slots_dtype != MI355_DTYPE_INT64) return MI355_ERR_BAD_ARGUMENT;
     if (tokens == 0) return MI355_OK;
     if (!key || !value || !slots || !key_stride || !value_stride) return MI355_ERR_BAD_ARGUMENT;
@@ -290,7 +409,7 @@ int move_rows(const mi355_paged_cache *cache, int dtype, void *key, const int64_
     for (int i = 0; i < 2; i++) {
         a.tok[i] = strides[i][0];
         a.head[i] = strides[i][1];
-        vec = vec && aligned(plane[i], 16) && a.tok[i] % 8 == 0 && a.head[i] % 8 == 0 && rows_aligned(i ? a.cache.value : a.cache.key, quant ? 8 : 16);
+        vec = vec && aligned(plane[i], 16) && a.tok[i] % 8 == 0 && a.head[i] % 8 == 0 && rows_aligned(i ? a.cache.value : a.cache.key, bits);
     }
     a.slots64 = slots_dtype == MI355_DTYPE_INT64;
     a.run = a.cache.key.token < a.cache.key.head ? 4 : 0;
@@ -299,7 +418,7 @@ int move_rows(const mi355_paged_cache *cache, int dtype, void *key, const int64_
         for (int i = 0; i < 2; i++) a.plane[i] = plane[i] + t0 * a.tok[i];
         a.slot_ids = static_cast<const char *>(slots) + t0 * id_bytes;
         a.tokens = (uint32_t)(tokens - t0 < most ? tokens - t0 : most);
-        launch_tokens<WRITE>(a, vec, quant, dtype == MI355_DTYPE_FP16, static_cast<hipStream_t>(stream));
+        launch_tokens<WRITE>(a, vec, bits, dtype == MI355_DTYPE_FP16, static_cast<hipStream_t>(stream));
     }
     return check_launch();
 }

@@ -60,10 +60,10 @@ __device__ __forceinline__ uint32_t scan_threads(uint32_t v, uint32_t *lds, uint
     return op(others, left_lane);
 }
 
-// Moves rows of keys and values (and their scales) within one (sequence, head), W bytes per access: pieces first,
+// Moves rows of keys and values (and their scales and offsets) within one (sequence, head), W bytes per access: pieces first,
 // first + step, ... of all of them.  per_row = pieces of a row of keys, then of the row of values.
 template <int W>
-__device__ __forceinline__ void move_pieces(const EvictArgs &a, int row, uint32_t count, uint32_t first, uint32_t step, int elem, const FastDiv &per_row)
+__device__ __forceinline__ void move_pieces(const EvictArgs &a, int row, uint32_t count, uint32_t first, uint32_t step, const FastDiv &per_row)
 {
     typedef uint32_t word __attribute__((ext_vector_type(W >= 4 ? W / 4 : 1)));
     const int b = row / a.cache.heads, head = row % a.cache.heads;
@@ -86,10 +86,13 @@ __device__ __forceinline__ void move_pieces(const EvictArgs &a, int row, uint32_
         if constexpr (W >= 4) *reinterpret_cast<word *>(d) = *reinterpret_cast<const word *>(s);
         else if constexpr (W == 2) *reinterpret_cast<uint16_t *>(d) = *reinterpret_cast<const uint16_t *>(s);
         else *d = *s;
-        if (elem == 1 && at == 0) {
-            const PagedArray &sc = value ? a.cache.value_scale : a.cache.key_scale;
-            *reinterpret_cast<float *>(sc.base + a.cache.offset(sc, dst_slot, head)) =
-                *reinterpret_cast<const float *>(sc.base + a.cache.offset(sc, src_slot, head));
+        if (at == 0 && a.cache.key_scale.base) {
+            const auto move = [&](const PagedArray &one) {
+                *reinterpret_cast<float *>(one.base + a.cache.offset(one, dst_slot, head)) =
+                    *reinterpret_cast<const float *>(one.base + a.cache.offset(one, src_slot, head));
+            };
+            move(value ? a.cache.value_scale : a.cache.key_scale);
+            if (a.cache.key_offset.base) move(value ? a.cache.value_offset : a.cache.key_offset);
         }
     }
 }
@@ -98,7 +101,7 @@ __device__ __forceinline__ void move_pieces(const EvictArgs &a, int row, uint32_
 // 16000 places halved: 52 us held, 82 read again; of 32000, held in part in scratch, 114 and 157).
 // W: bytes per access of the moves that this kernel makes itself; 0: it leaves them to paged_move_kernel.
 template <int KPT, int W>
-__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a, int elem, FastDiv per_row)
+__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a, FastDiv per_row)
 {
     // places per scan of the counts below: 64 rounds with one count per thread
     constexpr int kBatch = KPT ? KPT : 64;
@@ -253,14 +256,14 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
         new_sums[place] = sums[src];
         new_pos[place] = pos[src];
     }
-    if constexpr (W > 0) move_pieces<W>(a, row, holes, tid, kSelectThreads, elem, per_row);
+    if constexpr (W > 0) move_pieces<W>(a, row, holes, tid, kSelectThreads, per_row);
     else if (tid == 0) a.count[row] = (int32_t)holes;
 }
 
 template <int W>
-__global__ __launch_bounds__(256) void paged_move_kernel(EvictArgs a, int elem, FastDiv per_row)
+__global__ __launch_bounds__(256) void paged_move_kernel(EvictArgs a, FastDiv per_row)
 {
-    move_pieces<W>(a, blockIdx.y, (uint32_t)a.count[blockIdx.y], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, elem, per_row);
+    move_pieces<W>(a, blockIdx.y, (uint32_t)a.count[blockIdx.y], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, per_row);
 }
 
 // A workgroup that chooses moves its rows itself where there can be few: up to this many bytes of keys.  (128 heads, rows of 256
@@ -269,25 +272,26 @@ __global__ __launch_bounds__(256) void paged_move_kernel(EvictArgs a, int elem, 
 constexpr int64_t kMovedBySelect = 16384;
 
 template <int KPT>
-void launch_select(const EvictArgs &a, unsigned rows, int width, int elem, const FastDiv &per_row, hipStream_t s)
+void launch_select(const EvictArgs &a, unsigned rows, int width, const FastDiv &per_row, hipStream_t s)
 {
     const dim3 grid(rows), block(kSelectThreads);
-    if (width == 16) hipLaunchKernelGGL((paged_select_kernel<KPT, 16>), grid, block, 0, s, a, elem, per_row);
-    else if (width == 2) hipLaunchKernelGGL((paged_select_kernel<KPT, 2>), grid, block, 0, s, a, elem, per_row);
-    else if (width == 1) hipLaunchKernelGGL((paged_select_kernel<KPT, 1>), grid, block, 0, s, a, elem, per_row);
-    else hipLaunchKernelGGL((paged_select_kernel<KPT, 0>), grid, block, 0, s, a, elem, per_row);
+    if (width == 16) hipLaunchKernelGGL((paged_select_kernel<KPT, 16>), grid, block, 0, s, a, per_row);
+    else if (width == 4) hipLaunchKernelGGL((paged_select_kernel<KPT, 4>), grid, block, 0, s, a, per_row);
+    else if (width == 2) hipLaunchKernelGGL((paged_select_kernel<KPT, 2>), grid, block, 0, s, a, per_row);
+    else if (width == 1) hipLaunchKernelGGL((paged_select_kernel<KPT, 1>), grid, block, 0, s, a, per_row);
+    else hipLaunchKernelGGL((paged_select_kernel<KPT, 0>), grid, block, 0, s, a, per_row);
 }
 // Rounds in steps of 2^k + 1: budgets are powers of two as a rule, and a cache that is kept at one has a block or two more.  A
 // round too many costs 0.2 to 0.6 us (one token over 8192: 11.9 us in 9 rounds, 15.1 in 16, 24 where nothing is held).
-void launch_select(const EvictArgs &a, unsigned rows, int width, int elem, const FastDiv &per_row, hipStream_t s)
+void launch_select(const EvictArgs &a, unsigned rows, int width, const FastDiv &per_row, hipStream_t s)
 {
-    if (a.capacity <= 2 * kSelectThreads) launch_select<2>(a, rows, width, elem, per_row, s);
-    else if (a.capacity <= 3 * kSelectThreads) launch_select<3>(a, rows, width, elem, per_row, s);
-    else if (a.capacity <= 5 * kSelectThreads) launch_select<5>(a, rows, width, elem, per_row, s);
-    else if (a.capacity <= 9 * kSelectThreads) launch_select<9>(a, rows, width, elem, per_row, s);
-    else if (a.capacity <= 17 * kSelectThreads) launch_select<17>(a, rows, width, elem, per_row, s);
-    else if (a.capacity <= 33 * kSelectThreads) launch_select<33>(a, rows, width, elem, per_row, s);
-    else launch_select<0>(a, rows, width, elem, per_row, s);
+    if (a.capacity <= 2 * kSelectThreads) launch_select<2>(a, rows, width, per_row, s);
+    else if (a.capacity <= 3 * kSelectThreads) launch_select<3>(a, rows, width, per_row, s);
+    else if (a.capacity <= 5 * kSelectThreads) launch_select<5>(a, rows, width, per_row, s);
+    else if (a.capacity <= 9 * kSelectThreads) launch_select<9>(a, rows, width, per_row, s);
+    else if (a.capacity <= 17 * kSelectThreads) launch_select<17>(a, rows, width, per_row, s);
+    else if (a.capacity <= 33 * kSelectThreads) launch_select<33>(a, rows, width, per_row, s);
+    else launch_select<0>(a, rows, width, per_row, s);
 }
 
 // moves of one row at most
@@ -342,7 +346,7 @@ extern "C" int mi355_paged_cache_evict(const mi355_paged_cache *cache, const int
     a.count = static_cast<int32_t *>(workspace);
     a.moves = reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + (rows * 4 + 255) / 256 * 256);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int elem = cache_elem_bytes(cache->dtype), bytes = (int)cache->head_dim * elem;
+    const int elem = cache_elem_bytes(cache->dtype), bytes = (int)(cache->head_dim * cache_bits(cache->dtype) / 8);
     const bool wide = bytes % 16 == 0 && rows_aligned(a.cache.key, 16) && rows_aligned(a.cache.value, 16);
     const FastDiv per_row = fast_div((uint32_t)(bytes / (wide ? 16 : elem)) * 2);
     const bool here = a.most * bytes <= kMovedBySelect;
@@ -361,13 +365,14 @@ extern "C" int mi355_paged_cache_evict(const mi355_paged_cache *cache, const int
         c.new_positions += r0 * capacity;
         c.count += r0;
         c.moves += r0 * 2 * a.most;
-        launch_select(c, (unsigned)n, here ? (wide ? 16 : elem) : 0, elem, per_row, s);
+        launch_select(c, (unsigned)n, here ? (wide ? 16 : elem) : 0, per_row, s);
         if (here) continue;
         const int64_t chunks = (a.most * per_row.d + 255) / 256;
         const dim3 grid((unsigned)(chunks < 64 ? chunks : 64), (unsigned)n);
-        if (wide) hipLaunchKernelGGL(paged_move_kernel<16>, grid, dim3(256), 0, s, c, elem, per_row);
-        else if (elem == 2) hipLaunchKernelGGL(paged_move_kernel<2>, grid, dim3(256), 0, s, c, elem, per_row);
-        else hipLaunchKernelGGL(paged_move_kernel<1>, grid, dim3(256), 0, s, c, elem, per_row);
+        if (wide) hipLaunchKernelGGL(paged_move_kernel<16>, grid, dim3(256), 0, s, c, per_row);
+        else if (elem == 4) hipLaunchKernelGGL(paged_move_kernel<4>, grid, dim3(256), 0, s, c, per_row);
+        else if (elem == 2) hipLaunchKernelGGL(paged_move_kernel<2>, grid, dim3(256), 0, s, c, per_row);
+        else hipLaunchKernelGGL(paged_move_kernel<1>, grid, dim3(256), 0, s, c, per_row);
     }
     return check_launch();
 }

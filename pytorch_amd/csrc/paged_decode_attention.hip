@@ -20,6 +20,11 @@
 // int8 caches: codes become 16-bit numbers exactly; the scale of a position's keys multiplies its score, the scale of its
 // values multiplies its probability, in float32.
 //
+// int4 caches: the image of a code c is c + 24 = 16 + u, its four bits u = c + 8 placed as the top mantissa bits of 16.0: one
+// three-input instruction for two codes, where a conversion would take five.  A value is (c + offset) * scale = (image + offset - 24)
+// * scale, so the second addend, the same for a whole row, is left to float32:
+//   z_j += scale_j (offset_j - 24) sum_d q_d, the sum once per head       out_d += sum_j P_j (offset_j - 24), P_j = 2^(z_j - m) scale_j
+//
 // Scores, maxima, l and out are float32.  The second product takes 16-bit operands, so probabilities are rounded once, to the
 // values' own type: 2^-8 of each in bf16, 2^-11 in fp16, which is what the values themselves carry, and l sums them unrounded.
 // Against probabilities kept in float32 the outputs' error grows from 0.0017 to 0.0018 of their norm for 37 bf16 positions, and by
@@ -56,6 +61,8 @@ constexpr int kSC1 = 16;                     // cache-policy bit: agent scope, p
 // 4095, 280 MB: 62 us for 768 pieces, 66 for 512, 64 for 1024, 68 for 1536).  Heads of up to 64 take 103 to 124 registers, of
 // which four would fit; they are cut for three like the others.
 constexpr int resident(int dp, bool quant) { return dp < 256 ? 3 : quant ? 2 : 1; }
+// what removes the bias of int4 images, offset - 24, is computed with the offsets
+constexpr float kBias4 = 24.0f;
 
 struct AttnArgs {
     PagedCache cache;
@@ -240,15 +247,26 @@ __device__ __forceinline__ float over_groups(float v, Op op)
 // rows, so kBlock loses with small blocks: 66.2 and 74.8 us for blocks of 8, 79.8 and 75 for 5, 84.9 and 75.4 for 4.
 enum Addressing { kRows, kBlock, kBlockAlike, kBlockMask };
 
-// DP: head_dim rounded up to 64, 128 or 256.  QT: type of q and out (0 bf16, 1 fp16).
-template <int DP, bool QUANT, int QT, Addressing AD>
+// The images of an int4 word's codes i and i + 4: its bits 4 i and 16 + 4 i on, as the top mantissa bits of 16.0, the sign bit turned.
+template <int ACT>
+__device__ __forceinline__ uint32_t image4(uint32_t w, int i)
+{
+    constexpr int place = ACT == 0 ? 3 : 6;
+    constexpr uint32_t mask = ACT == 0 ? 0x00780078u : 0x03c003c0u, one = ACT == 0 ? 0x41804180u | 0x00400040u : 0x4c004c00u | 0x02000200u;
+    return bit_blend(4 * i > place ? w >> (4 * i - place) : w << (place - 4 * i), mask, one);
+}
+
+// DP: head_dim rounded up to 64, 128 or 256.  BITS: of the cache's elements.  QT: type of q and out (0 bf16, 1 fp16).
+template <int DP, int BITS, int QT, Addressing AD>
 struct Decode {
-    static constexpr int ES = QUANT ? 1 : 2;
+    static constexpr bool QUANT = BITS < 16;
     static constexpr int NCH = DP / 32;                          // chunks of 32 d, one MFMA each
-    static constexpr int KL = QUANT ? NCH / 2 : NCH;             // 16-byte loads of a key row per lane
+    static constexpr int KL = QUANT ? NCH / 2 : NCH;             // loads of a key row per lane
+    static constexpr int KW = BITS == 4 ? 2 : 4;                 // and their registers
     static constexpr int PE = DP >= 128 ? 8 : 4;                 // consecutive d of a value row per lane and piece
     static constexpr int NP = DP / (16 * PE);
-    static constexpr int VW = PE * ES / 4;                       // registers of a piece
+    static constexpr int VW = BITS == 4 ? 1 : PE * BITS / 32;    // registers of a piece (int4, PE 4: a word that two lanes share)
+    static constexpr int PARAMS = BITS == 4 ? 4 : 2;             // arrays of scales and offsets, as they lie in PagedCache
     static constexpr int PT = QUANT ? 0 : QT;                    // type of the probabilities and of the values' images
     // fp16 probabilities are 2^14 times as large, so that ones down to 2^-38 of the largest keep their place
     static constexpr float kShift = PT == 1 ? 14.0f : 0.0f;
@@ -261,18 +279,19 @@ struct Decode {
 
     const Args a;
     const int wave, col, g, D;
-    uint32_t koff[KL], voff[4][NP], soff[2][4];                  // lane offsets of key pieces, value pieces, scales
-    uint32_t k[2][KL][4], v[2][4][NP][VW], hidden[2];
-    float ks[2][4], vs[2][4];
+    uint32_t koff[KL], voff[4][NP], soff[PARAMS][4];             // lane offsets of key pieces, value pieces, scales, offsets
+    uint32_t k[2][KL][KW], v[2][4][NP][VW], hidden[2];
+    float ks[2][4], vs[2][4], ko[2][4], vo[2][4];
     uint32_t lane_slot[2], v_slot[2];                            // kRows: slot of position 16 s + col of the tile, or ~0
     u32x4 q[NCH];
     f32x4 acc[NP][PE];
     float m, l;
+    float qsum, osum;                                            // int4: sum of the head's query; the lane's sum of P_j (offset_j - 24)
 
     // of the pair that is being worked on
     int b, kvh, len, half_end;
     const int32_t *table;
-    const char *kbase, *vbase, *ksbase, *vsbase;
+    const char *kbase, *vbase, *ksbase, *vsbase, *kobase, *vobase;
     uint64_t start[2], scale_start[2];                           // kBlockAlike: of the tile whose keys were requested last
     uint32_t reach[2];
 
@@ -286,18 +305,22 @@ struct Decode {
 #pragma unroll
             for (int c = 0; c < KL; c++) {
                 const int d = first_d(c);
-                koff[c] = d < D ? (uint32_t)col * (uint32_t)a->cache.key.token + d * ES : kOutOfRange;
+                koff[c] = d < D ? (uint32_t)col * (uint32_t)a->cache.key.token + bytes(d) : kOutOfRange;
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
 #pragma unroll
                 for (int h = 0; h < NP; h++) {
-                    const int d = h * 128 + col * PE;
-                    voff[j][h] = d < D ? (uint32_t)(g * 4 + j) * (uint32_t)a->cache.value.token + d * ES : kOutOfRange;
+                    const int d = value_d(h);
+                    voff[j][h] = d < D ? (uint32_t)(g * 4 + j) * (uint32_t)a->cache.value.token + bytes(d) : kOutOfRange;
                 }
                 if constexpr (QUANT) {
                     soff[0][j] = (uint32_t)(g * 4 + j) * (uint32_t)a->cache.key_scale.token;
                     soff[1][j] = (uint32_t)(g * 4 + j) * (uint32_t)a->cache.value_scale.token;
+                }
+                if constexpr (BITS == 4) {
+                    soff[PARAMS - 2][j] = (uint32_t)(g * 4 + j) * (uint32_t)a->cache.key_offset.token;
+                    soff[PARAMS - 1][j] = (uint32_t)(g * 4 + j) * (uint32_t)a->cache.value_offset.token;
                 }
             }
         }
@@ -309,7 +332,10 @@ struct Decode {
         const uint32_t block = divide(slot, a->cache.page);
         return block * x.block + (int64_t)(slot - block * a->cache.page.d) * x.token + kvh * x.head;
     }
-    // first d of the lane's key piece c; an int8 piece serves the chunks 2c and 2c + 1
+    __device__ static __forceinline__ int bytes(int d) { return BITS == 4 ? d / 2 : d * (BITS / 8); }
+    // first d of the lane's value piece h (int4: of its word)
+    __device__ __forceinline__ int value_d(int h) const { return h * 128 + (BITS == 4 && PE == 4 ? col / 2 * 8 : col * PE); }
+    // first d of the lane's key piece c; a piece of codes serves the chunks 2c and 2c + 1
     __device__ __forceinline__ int first_d(int c) const { return QUANT ? c * 64 + g * 16 : c * 32 + g * 8; }
 
     __device__ __forceinline__ void begin(int b_, int kvh_, int head0, int rows, int len_, int half_end_)
@@ -319,6 +345,7 @@ struct Decode {
         kbase = a->cache.key.base + kvh * a->cache.key.head;
         vbase = a->cache.value.base + kvh * a->cache.value.head;
         if constexpr (QUANT) ksbase = a->cache.key_scale.base + kvh * a->cache.key_scale.head, vsbase = a->cache.value_scale.base + kvh * a->cache.value_scale.head;
+        if constexpr (BITS == 4) kobase = a->cache.key_offset.base + kvh * a->cache.key_offset.head, vobase = a->cache.value_offset.base + kvh * a->cache.value_offset.head;
         const uint16_t *row = a->q + b * a->q_batch + (head0 + min(col, rows - 1)) * a->q_head;
 #pragma unroll
         for (int c = 0; c < NCH; c++) {
@@ -326,6 +353,19 @@ struct Decode {
             uint32_t w[4];
             load_piece<16>(w, (const Global<char> *)(row + d), col < rows ? 2 * (D - d) : 0);
             q[c] = u32x4{w[0], w[1], w[2], w[3]};
+        }
+        if constexpr (BITS == 4) {
+            qsum = osum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NCH; c++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) qsum += act_lo<QT>(q[c][i]) + act_hi<QT>(q[c][i]);
+                // in the order of image4: (d, d + 4)
+                const u32x4 w = q[c];
+                q[c] = u32x4{__builtin_amdgcn_perm(w.z, w.x, 0x05040100u), __builtin_amdgcn_perm(w.z, w.x, 0x07060302u),
+                             __builtin_amdgcn_perm(w.w, w.y, 0x05040100u), __builtin_amdgcn_perm(w.w, w.y, 0x07060302u)};
+            }
+            qsum = over_groups(qsum, [](float x, float y) { return x + y; });
         }
         m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -382,13 +422,14 @@ struct Decode {
         for (int s = 0; s < 2; s++) {
             if constexpr (AD != kRows) {
                 if constexpr (AD == kBlockAlike) {
-                    start[s] = start_of(a->cache.key, p, s), reach[s] = reach_of(a->cache.key, p, s, D * ES);
+                    start[s] = start_of(a->cache.key, p, s), reach[s] = reach_of(a->cache.key, p, s, bytes(D));
                     scale_start[s] = start_of(a->cache.key_scale, p, s);
                 }
-                const __amdgpu_buffer_rsrc_t r = AD == kBlockAlike ? rows_at(kbase, start[s], reach[s]) : rows_of(kbase, a->cache.key, p, s, D * ES);
+                const __amdgpu_buffer_rsrc_t r = AD == kBlockAlike ? rows_at(kbase, start[s], reach[s]) : rows_of(kbase, a->cache.key, p, s, bytes(D));
 #pragma unroll
-                for (int c = 0; c < KL; c++) buffer_load<4>(k[s][c], r, koff[c]);
+                for (int c = 0; c < KL; c++) buffer_load<KW>(k[s][c], r, koff[c]);
                 if constexpr (QUANT) load_scales(ks[s], ksbase, a->cache.key_scale, p, s, soff[0]);
+                if constexpr (BITS == 4) load_scales(ko[s], kobase, a->cache.key_offset, p, s, soff[PARAMS - 2]);
             } else {
                 const int key = p.key[s] + col;
                 const uint32_t block = divide((uint32_t)key, a->cache.page);
@@ -398,12 +439,9 @@ struct Decode {
                 lane_slot[s] = there ? (uint32_t)id * a->cache.page.d + ((uint32_t)key - block * a->cache.page.d) : ~0u;
                 const Global<char> *row = at(a->cache.key.base) + (there ? offset(a->cache.key, lane_slot[s]) : 0);
 #pragma unroll
-                for (int c = 0; c < KL; c++) load_piece<16>(k[s][c], row + first_d(c) * ES, there ? (D - first_d(c)) * ES : 0);
-                if constexpr (QUANT) {
-                    const float mine = there ? *(const Global<float> *)(at(a->cache.key_scale.base) + offset(a->cache.key_scale, lane_slot[s])) : 0.0f;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) ks[s][r] = __shfl(mine, g * 4 + r, 64);
-                }
+                for (int c = 0; c < KL; c++) load_piece<KW * 4>(k[s][c], row + bytes(first_d(c)), there ? bytes(D - first_d(c)) : 0);
+                if constexpr (QUANT) spread(ks[s], a->cache.key_scale, there, lane_slot[s]);
+                if constexpr (BITS == 4) spread(ko[s], a->cache.key_offset, there, lane_slot[s]);
             }
             if constexpr (AD == kBlockMask) {                    // from any byte (the host: blocks of a multiple of 4 tokens)
                 const uint64_t first = (uint64_t)a->mask + (uint64_t)(b * a->mask_stride) + (uint32_t)p.key[s];
@@ -411,6 +449,13 @@ struct Decode {
                 hidden[s] = __builtin_amdgcn_raw_buffer_load_b32(r, g * 4, 0, 0);
             }
         }
+    }
+    // kRows: each lane of the 16 loads the parameter of its slot; a lane gets those of its group's four positions
+    __device__ __forceinline__ void spread(float (&to)[4], ArgArray &x, bool there, uint32_t slot) const
+    {
+        const float mine = there ? *(const Global<float> *)(at(x.base) + offset(x, slot)) : 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; r++) to[r] = __shfl(mine, g * 4 + r, 64);
     }
     __device__ __forceinline__ void load_scales(float (&to)[4], const char *base, ArgArray &x, const Place &p, int s, const uint32_t (&off)[4]) const
     {
@@ -430,27 +475,25 @@ struct Decode {
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             if constexpr (AD != kRows) {
-                const __amdgpu_buffer_rsrc_t r = AD == kBlockAlike ? rows_at(vbase, start[s], reach[s]) : rows_of(vbase, a->cache.value, p, s, D * ES);
+                const __amdgpu_buffer_rsrc_t r = AD == kBlockAlike ? rows_at(vbase, start[s], reach[s]) : rows_of(vbase, a->cache.value, p, s, bytes(D));
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
                     for (int h = 0; h < NP; h++) buffer_load<VW>(v[s][j][h], r, voff[j][h]);
                 if constexpr (QUANT) load_scales(vs[s], vsbase, a->cache.value_scale, p, s, soff[1]);
+                if constexpr (BITS == 4) load_scales(vo[s], vobase, a->cache.value_offset, p, s, soff[PARAMS - 1]);
             } else {
                 const int64_t mine = lane_slot[s] == ~0u ? -1 : offset(a->cache.value, lane_slot[s]);
-                if constexpr (QUANT) {
-                    const float scale = mine >= 0 ? *(const Global<float> *)(at(a->cache.value_scale.base) + offset(a->cache.value_scale, lane_slot[s])) : 0.0f;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) vs[s][r] = __shfl(scale, g * 4 + r, 64);
-                }
+                if constexpr (QUANT) spread(vs[s], a->cache.value_scale, mine >= 0, lane_slot[s]);
+                if constexpr (BITS == 4) spread(vo[s], a->cache.value_offset, mine >= 0, lane_slot[s]);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int64_t from = __shfl(mine, g * 4 + j, 64);
                     const Global<char> *row = at(a->cache.value.base) + (from < 0 ? 0 : from);
 #pragma unroll
                     for (int h = 0; h < NP; h++) {
-                        const int d = h * 128 + col * PE;
-                        load_piece<VW * 4>(v[s][j][h], row + d * ES, from < 0 ? 0 : (D - d) * ES);
+                        const int d = value_d(h);
+                        load_piece<VW * 4>(v[s][j][h], row + bytes(d), from < 0 ? 0 : bytes(D - d));
                     }
                 }
             }
@@ -489,7 +532,10 @@ struct Decode {
 #pragma unroll
             for (int c = 0; c < NCH; c++) {
                 u32x4 image;
-                if constexpr (QUANT) {
+                if constexpr (BITS == 4) {
+                    const uint32_t w = k[s][c / 2][c % 2];
+                    image = u32x4{image4<QT>(w, 0), image4<QT>(w, 1), image4<QT>(w, 2), image4<QT>(w, 3)};
+                } else if constexpr (QUANT) {
                     const u32x2 lo = sbytes_act4<QT>(k[s][c / 2][(c % 2) * 2]), hi = sbytes_act4<QT>(k[s][c / 2][(c % 2) * 2 + 1]);
                     image = u32x4{lo.x, lo.y, hi.x, hi.y};
                 } else {
@@ -502,6 +548,7 @@ struct Decode {
         for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
+                if constexpr (BITS == 4) z[s][r] = __builtin_fmaf(ko[s][r] - kBias4, qsum, z[s][r]);
                 z[s][r] = QUANT ? z[s][r] * (a->scale2 * ks[s][r]) : z[s][r] * a->scale2;
             }
         if (!full(p)) {
@@ -541,6 +588,7 @@ struct Decode {
             const float higher = fmaxf(m, top), f = weight_of(m, higher);
             m = higher;
             l *= f;
+            if constexpr (BITS == 4) osum *= f;
 #pragma unroll
             for (int h = 0; h < NP; h++)
 #pragma unroll
@@ -562,6 +610,14 @@ struct Decode {
                 no_select();
 #pragma unroll
                 for (int i = 0; i < 8; i++) p[i] = (valid >> i) & 1 ? p[i] : 0.0f;
+                if constexpr (BITS == 4) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) vo[i / 4][i % 4] = (valid >> i) & 1 ? vo[i / 4][i % 4] : 0.0f;
+                }
+            }
+            if constexpr (BITS == 4) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) osum = __builtin_fmaf(p[i], vo[i / 4][i % 4] - kBias4, osum);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -597,7 +653,11 @@ struct Decode {
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
                     const int s = w / 2, j = (w % 2) * 2;
-                    if constexpr (QUANT)
+                    if constexpr (BITS == 4) {
+                        // the low or the high half of the words of two positions; codes i % 4 of their halves
+                        const uint32_t half = PE == 4 ? (col & 1 ? 0x07060302u : 0x05040100u) : i < 4 ? 0x05040100u : 0x07060302u;
+                        image[w] = image4<PT>(__builtin_amdgcn_perm(v[s][j + 1][h][0], v[s][j][h][0], half), i % 4);
+                    } else if constexpr (QUANT)
                         image[w] = pack_bf16x2(sbyte_f32(v[s][j][h][i / 4], i % 4), sbyte_f32(v[s][j + 1][h][i / 4], i % 4));
                     else
                         image[w] = __builtin_amdgcn_perm(v[s][j + 1][h][i / 2], v[s][j][h][i / 2], i % 2 ? 0x07060302u : 0x05040100u);
@@ -638,6 +698,13 @@ struct Decode {
             __builtin_amdgcn_sched_barrier(0);
             cur = next;
             next = place(tile + 8);
+        }
+        if constexpr (BITS == 4) {
+            osum = over_groups(osum, [](float x, float y) { return x + y; });
+#pragma unroll
+            for (int h = 0; h < NP; h++)
+#pragma unroll
+                for (int i = 0; i < PE; i++) acc[h][i] += osum;
         }
     }
 };
@@ -818,10 +885,10 @@ __device__ __forceinline__ bool arrive(Global<uint32_t> *counter, int n, int *ld
     return uniform(*lds) != 0;
 }
 
-template <int DP, bool QUANT, int QT, Addressing AD>
-__global__ __launch_bounds__(256, resident(DP, QUANT)) void paged_decode_kernel(AttnArgs)
+template <int DP, int BITS, int QT, Addressing AD>
+__global__ __launch_bounds__(256, resident(DP, BITS < 16)) void paged_decode_kernel(AttnArgs)
 {
-    using W = Decode<DP, QUANT, QT, AD>;
+    using W = Decode<DP, BITS, QT, AD>;
     constexpr int RP = 128 + 4;                                  // row pitch of a wavefront's sums in LDS
     __shared__ float red[4][kHeads][RP];
     __shared__ float ml[4][kHeads][2];
@@ -1048,25 +1115,28 @@ static_assert(resident(256, false) <= resident(256, true), "the workspace's size
 static_assert(kNumCU * 3 * 4 * sizeof(uint32_t) <= kWorkspaceCounterBytes, "arrival counters");
 static_assert(kNumCU * 3 <= (kJoin / 2) * (kJoin / 2), "groups of pieces, and members of a group");
 
-template <int DP, bool QUANT, int QT>
+template <int DP, int BITS, int QT>
 void launch_attention(const AttnArgs &a, Addressing ad, unsigned workgroups, hipStream_t s)
 {
     const dim3 grid(workgroups), block(256);
-    if (ad == kRows) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kRows>), grid, block, 0, s, a);
-    else if (ad == kBlockMask) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlockMask>), grid, block, 0, s, a);
-    else if (ad == kBlock) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlock>), grid, block, 0, s, a);
-    else if constexpr (QUANT) hipLaunchKernelGGL((paged_decode_kernel<DP, QUANT, QT, kBlockAlike>), grid, block, 0, s, a);
+    if (ad == kRows) hipLaunchKernelGGL((paged_decode_kernel<DP, BITS, QT, kRows>), grid, block, 0, s, a);
+    else if (ad == kBlockMask) hipLaunchKernelGGL((paged_decode_kernel<DP, BITS, QT, kBlockMask>), grid, block, 0, s, a);
+    else if (ad == kBlock) hipLaunchKernelGGL((paged_decode_kernel<DP, BITS, QT, kBlock>), grid, block, 0, s, a);
+    else if constexpr (BITS < 16) hipLaunchKernelGGL((paged_decode_kernel<DP, BITS, QT, kBlockAlike>), grid, block, 0, s, a);
 }
 
 template <int DP>
-void launch_attention(const AttnArgs &a, bool quant, bool fp16, Addressing ad, unsigned workgroups, hipStream_t s)
+void launch_attention(const AttnArgs &a, int bits, bool fp16, Addressing ad, unsigned workgroups, hipStream_t s)
 {
-    if (quant) {
-        if (fp16) launch_attention<DP, true, 1>(a, ad, workgroups, s);
-        else launch_attention<DP, true, 0>(a, ad, workgroups, s);
+    if (bits == 4) {
+        if (fp16) launch_attention<DP, 4, 1>(a, ad, workgroups, s);
+        else launch_attention<DP, 4, 0>(a, ad, workgroups, s);
+    } else if (bits == 8) {
+        if (fp16) launch_attention<DP, 8, 1>(a, ad, workgroups, s);
+        else launch_attention<DP, 8, 0>(a, ad, workgroups, s);
     } else {
-        if (fp16) launch_attention<DP, false, 1>(a, ad, workgroups, s);
-        else launch_attention<DP, false, 0>(a, ad, workgroups, s);
+        if (fp16) launch_attention<DP, 16, 1>(a, ad, workgroups, s);
+        else launch_attention<DP, 16, 0>(a, ad, workgroups, s);
     }
 }
 
@@ -1090,7 +1160,8 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     using namespace mi355;
     AttnArgs a;
     if (const int st = open_cache(cache, &a.cache); st != MI355_OK) return st;
-    const bool quant = cache->dtype == MI355_DTYPE_INT8, fp16 = q_dtype == MI355_DTYPE_FP16;
+    const int bits = cache_bits(cache->dtype);
+    const bool quant = bits < 16, fp16 = q_dtype == MI355_DTYPE_FP16;
     if (batch < 0 || heads < 1 || heads % cache->kv_heads || max_blocks < 0 || (q_dtype != MI355_DTYPE_BF16 && !fp16) ||
         (!quant && cache->dtype != q_dtype))
         return MI355_ERR_BAD_ARGUMENT;
@@ -1137,20 +1208,21 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     a.part_bytes = p.part_bytes;
     a.part_ml_bytes = p.part_ml_bytes;
     a.scale2 = scale * kLog2e;
-    const int es = quant ? 1 : 2;
-    // pieces of 16 bytes: rows on 16-byte boundaries, and no piece reaching past a row's end
-    const bool pieces = cache->head_dim * es % 16 == 0 && rows_aligned(a.cache.key, 16) && rows_aligned(a.cache.value, 16);
+    // pieces of 16 bytes (int4: 8, in words): rows on 16-byte boundaries, and no piece reaching past a row's end
+    const int piece = bits == 4 ? 8 : 16, line = bits == 4 ? 4 : 16;
+    const bool pieces = cache->head_dim * bits / 8 % piece == 0 && rows_aligned(a.cache.key, line) && rows_aligned(a.cache.value, line);
     // Halves that lie in one block: block by block, the last half of a block may be short, so blocks of fewer than 8 tokens
     // would leave most of a tile empty.  Offsets within a block have 31 bits, a block's own offset is a 32 x 32-bit product.
-    const PagedArray *const arrays[] = {&a.cache.key, &a.cache.value, &a.cache.key_scale, &a.cache.value_scale};
+    const PagedArray *const arrays[] = {&a.cache.key, &a.cache.value, &a.cache.key_scale, &a.cache.value_scale, &a.cache.key_offset, &a.cache.value_offset};
     bool blocks = pieces && cache->block_size >= 8 && (!mask || cache->block_size % 4 == 0), scales = cache->block_size % 4 == 0;
-    for (int i = 0; i < (quant ? 4 : 2); i++) {
+    for (int i = 0; i < (bits == 4 ? 6 : quant ? 4 : 2); i++) {
         const PagedArray &x = *arrays[i];
         blocks = blocks && x.block >= 0 && x.block <= 0xffffffffll && x.token >= 0 && x.token <= 0x7fffffff / (cache->block_size + 16);
         if (i >= 2) scales = scales && x.token == 4 && aligned(x.base, 16) && x.block % 16 == 0 && x.head % 16 == 0;
     }
     const auto alike = [](const PagedArray &x, const PagedArray &y) { return x.block == y.block && x.token == y.token && x.head == y.head; };
-    const bool same = quant && scales && alike(a.cache.key, a.cache.value) && alike(a.cache.key_scale, a.cache.value_scale);
+    const bool same = quant && scales && alike(a.cache.key, a.cache.value) && alike(a.cache.key_scale, a.cache.value_scale) &&
+                      (bits == 8 || (alike(a.cache.key_scale, a.cache.key_offset) && alike(a.cache.key_scale, a.cache.value_offset)));
     const Addressing ad = !blocks ? kRows : mask ? kBlockMask : same ? kBlockAlike : kBlock;
     // Rows of several heads in a cache line, with other heads' rows of the same token: work on them at the same time and on one XCD,
     // so that the line comes once (16 sequences of up to 1001 tokens, 32 heads of 80: 32.4 -> 28.6 us; int8, 32 sequences of up to
@@ -1161,9 +1233,9 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     a.span = ad != kRows ? a.cache.page : fast_div(kHalf);
     a.halves = fast_div((a.span.d + kHalf - 1) / kHalf);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (p.dp == 64) launch_attention<64>(a, quant, fp16, ad, (unsigned)p.workgroups, s);
-    else if (p.dp == 128) launch_attention<128>(a, quant, fp16, ad, (unsigned)p.workgroups, s);
-    else launch_attention<256>(a, quant, fp16, ad, (unsigned)p.workgroups, s);
+    if (p.dp == 64) launch_attention<64>(a, bits, fp16, ad, (unsigned)p.workgroups, s);
+    else if (p.dp == 128) launch_attention<128>(a, bits, fp16, ad, (unsigned)p.workgroups, s);
+    else launch_attention<256>(a, bits, fp16, ad, (unsigned)p.workgroups, s);
     if (attn_sums && a.capacity > 0) {
         const int64_t chunks = (a.capacity + 1023) / 1024;
         for (int64_t b0 = 0; b0 < batch; b0 += 65535) {           // a grid's third dimension has 16 bits

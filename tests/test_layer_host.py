@@ -139,3 +139,87 @@ def test_c_entries_refuse_before_they_launch():
         assert rope(**change) == unsupported, change
     for change in (dict(pos=68), dict(q=65), dict(k=65), dict(table=66), dict(qo=65), dict(ko=65)):
         assert rope(**change) == alignment, change
+
+
+# ------------------------------------------------------------------------------------------------ the 4-bit paged cache
+
+def cache4(blocks=10, page=16, heads=2, dim=64):
+    c = {name: m(blocks, page, heads, dim // 8, dtype=I32) for name in ("key_cache", "value_cache")}
+    return c | {name: m(blocks, page, heads, dtype=F) for name in ("key_scale", "value_scale", "key_offset", "value_offset")}
+
+
+SLOTS = m(5, dtype=I64)
+TABLE = dict(block_table=m(3, 4, dtype=I32), context_lens=m(3, dtype=I32))
+
+
+def test_cache4_shapes(pa):
+    pa.npu_paged_cache_write(m(5, 2, 64), m(5, 2, 64), slots=SLOTS, **cache4())
+    k, v = pa.npu_paged_cache_read(slots=SLOTS, **cache4())
+    assert k.shape == v.shape == (5, 2, 64) and k.dtype == v.dtype == BF
+    assert pa.npu_paged_cache_read(slots=SLOTS, dtype=HF, **cache4())[0].dtype == HF
+    out, lse = pa.npu_paged_decode_attention(m(3, 8, 64, dtype=HF), **cache4(), **TABLE, softmax_lse=True)
+    assert out.shape == (3, 8, 64) and out.dtype == HF and lse.shape == (3, 8)
+    lens, sums, pos = pa.npu_paged_cache_evict(**cache4(), **TABLE, attn_sums=m(3, 2, 64, dtype=F), positions=m(3, 2, 64, dtype=I32), keep=40, recent=8)
+    assert lens.shape == (3,) and sums.shape == pos.shape == (3, 2, 64)
+
+
+@pytest.mark.parametrize("op", ["write", "read", "attend", "evict"])
+@pytest.mark.parametrize("change,text", [
+    (dict(key_offset=None), "needs key_scale, value_scale, key_offset and value_offset"),
+    (dict(value_scale=None), "needs key_scale, value_scale, key_offset and value_offset"),
+    (dict(key_offset=m(10, 16, 2, dtype=BF)), "key_offset and value_offset must be float32"),
+    (dict(value_offset=m(10, 16, 2, 1, dtype=F)), "key_offset and value_offset must be float32"),
+    (dict(value_scale=m(10, 16, 3, dtype=F)), "key_scale and value_scale must be float32"),
+    (dict(value_cache=m(10, 16, 2, 8, dtype=I8)), "the same dtype"),
+    (dict(key_cache=m(10, 16, 2, 64), value_cache=m(10, 16, 2, 64)), "belong to an int8 cache or a 4-bit one"),
+    (dict(key_cache=m(10, 16, 2, 64), value_cache=m(10, 16, 2, 64), key_scale=None, value_scale=None), "belong to a 4-bit cache"),
+    (dict(key_cache=m(10, 16, 2, 64, dtype=I8), value_cache=m(10, 16, 2, 64, dtype=I8)), "belong to a 4-bit cache"),
+    (dict(key_cache=m(10, 16, 2, 8, dtype=I64), value_cache=m(10, 16, 2, 8, dtype=I64)), "4-bit codes"),
+])
+def test_cache4_refusals(pa, op, change, text):
+    fn, more = {"write": (pa.npu_paged_cache_write, dict(key=m(5, 2, 64), value=m(5, 2, 64), slots=SLOTS)), "read": (pa.npu_paged_cache_read, dict(slots=SLOTS)),
+                "attend": (pa.npu_paged_decode_attention, dict(query=m(3, 8, 64), **TABLE)),
+                "evict": (pa.npu_paged_cache_evict, dict(attn_sums=m(3, 2, 64, dtype=F), positions=m(3, 2, 64, dtype=I32), keep=40, recent=8, **TABLE))}[op]
+    with pytest.raises(RuntimeError, match=text):
+        fn(**{**cache4(), **more, **change})
+
+
+def test_cache4_widths_and_memory(pa):
+    with pytest.raises(RuntimeError, match="key must have shape"):
+        pa.npu_paged_cache_write(m(5, 2, 8), m(5, 2, 8), slots=SLOTS, **cache4())
+    with pytest.raises(RuntimeError, match="query must have shape"):
+        pa.npu_paged_decode_attention(m(3, 8, 8), **cache4(), **TABLE)
+    with pytest.raises(RuntimeError, match="at most 256"):
+        pa.npu_paged_decode_attention(m(3, 8, 264), **cache4(dim=264), **TABLE)
+    with pytest.raises(RuntimeError, match="share memory"):
+        pa.npu_paged_cache_write(m(5, 2, 64), m(5, 2, 64), slots=SLOTS, **{**cache4(), "value_offset": m(1, 16, 2, dtype=F).expand(10, 16, 2)})
+
+
+class Descriptor4(ctypes.Structure):
+    _fields_ = [("key", ctypes.c_void_p), ("value", ctypes.c_void_p), ("key_scale", ctypes.c_void_p), ("value_scale", ctypes.c_void_p),
+                ("dtype", ctypes.c_int), ("num_blocks", ctypes.c_int64), ("block_size", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64), ("key_stride", ctypes.c_int64 * 3), ("value_stride", ctypes.c_int64 * 3),
+                ("key_scale_stride", ctypes.c_int64 * 3), ("value_scale_stride", ctypes.c_int64 * 3), ("key_offset", ctypes.c_void_p),
+                ("value_offset", ctypes.c_void_p), ("key_offset_stride", ctypes.c_int64 * 3), ("value_offset_stride", ctypes.c_int64 * 3)]
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(), 0), (dict(key_offset=None), -1), (dict(value_offset=None), -1), (dict(key_scale=None), -1), (dict(head_dim=60), -1), (dict(dtype=5), -1),
+    (dict(key=66), -3), (dict(value_offset=66), -3), (dict(key_scale=65), -3), (dict(num_blocks=1 << 30), -2)])
+def test_cache4_descriptor(change, status):
+    """Without tokens nothing is launched, so that the descriptor's own checks answer."""
+    lib = ctypes.CDLL(os.path.join(ROOT, "pytorch_amd", "csrc", "libmi355_quant.so"))
+    three = (ctypes.c_int64 * 3)(16 * 2 * 8, 2 * 8, 8)
+    one = (ctypes.c_int64 * 3)(32, 1, 16)
+    d = Descriptor4(**{**dict(key=64, value=64, key_scale=64, value_scale=64, dtype=6, num_blocks=10, block_size=16, kv_heads=2, head_dim=64, key_stride=three,
+                              value_stride=three, key_scale_stride=one, value_scale_stride=one, key_offset=64, value_offset=64, key_offset_stride=one,
+                              value_offset_stride=one), **change})
+    got = lib.mi355_paged_cache_write(ctypes.byref(d), None, None, None, None, 0, None, 5, ctypes.c_int64(0), None)
+    assert got == status
+
+
+def test_module_refusals():
+    from pytorch_amd.contrib.module import PagedKVCache
+    for more, text in ((dict(bits=4), "quantized=True"), (dict(bits=3, quantized=True), "bits should be"), (dict(bits=4, quantized=True, head_dim=60), "multiple of 8")):
+        with pytest.raises(ValueError, match=text):
+            PagedKVCache(**{**dict(batch=1, max_tokens=8, kv_heads=1, head_dim=64), **more})
