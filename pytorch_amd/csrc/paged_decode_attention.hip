@@ -29,7 +29,7 @@
 // values' own type: 2^-8 of each in bf16, 2^-11 in fp16, which is what the values themselves carry, and l sums them unrounded.
 // Against probabilities kept in float32 the outputs' error grows from 0.0017 to 0.0018 of their norm for 37 bf16 positions, and by
 // less over more of them; the rounding of out to its own type makes the rest.  Products with value scales, on int8 caches, whose
-// values are exact, keep two bf16 terms, 2^-16.
+// values are exact, keep two bf16 terms, 2^-16; int4 caches as int8 ones, or as Decode4 says.
 //
 // Work is dealt out on the device, because the lengths are known only there: the positions of every (sequence, head) pair
 // are cut into halves of a tile, 16 positions of one block (fewer at a block's end), eight halves make a unit, and a pair
@@ -40,7 +40,8 @@
 // Bound by memory, at 5.5 to 5.9 TB/s where the work is long (32 sequences of 8192, 1.07 GB, in 188 us), behind about 12 us that
 // do not depend on it: the launch, two trips to memory for lengths and blocks, the first rows, and at the end the four
 // wavefronts' sums, their trip through the workspace and the addition.  With 32 query heads on 8 heads of 128: 32 sequences of up to 4095 tokens
-// (280 MB) 62 us, one of 131071 (537 MB) 104 us, int8, 64 of up to 8192 (563 MB) 120 us, one of 37 6.5 us.
+// (280 MB) 62 us, one of 131071 (537 MB) 104 us, int8, 64 of up to 8192 (563 MB) 120 us, one of 37 6.5 us.  int4: 32 of up to 4095 (78 MB)
+// 25.7 us, 64 of up to 8192 (308 MB) 61.2 us, one of 131071 (151 MB) 39.8 us, one of 37 6.7 us.
 #include "paged_cache.h"
 #include "weight_quant_common.h"
 
@@ -61,6 +62,12 @@ constexpr int kSC1 = 16;                     // cache-policy bit: agent scope, p
 // 4095, 280 MB: 62 us for 768 pieces, 66 for 512, 64 for 1024, 68 for 1536).  Heads of up to 64 take 103 to 124 registers, of
 // which four would fit; they are cut for three like the others.
 constexpr int resident(int dp, bool quant) { return dp < 256 ? 3 : quant ? 2 : 1; }
+// int4, Decode4: halves of a step of a workgroup; its workgroups of a compute unit (135 to 138 registers for heads of 65 to 128, 207 and 211 for
+// wider ones); and what the start and the end of a sequence cost, in halves (32 sequences of up to 4095, 78 MB: 25.7 us with 24, 26.2 with 16 or
+// 30, 27.8 with 8, 26.7 with 40, 30.0 with 64; 64 of up to 8192, 308 MB: 60.4 to 61.3, with 8 and 64 63)
+constexpr int kStep = 8;
+constexpr int resident4(int dp) { return dp < 256 ? 3 : 2; }
+constexpr uint32_t kStart = 24;
 // what removes the bias of int4 images, offset - 24, is computed with the offsets
 constexpr float kBias4 = 24.0f;
 
@@ -81,7 +88,8 @@ struct AttnArgs {
     float *lse2;                             // [batch * heads] m + log2 l, with scores
     float *sums;
     int64_t score_pitch, sums_batch, sums_head;
-    FastDiv by_pairs, by_shares;
+    FastDiv by_pairs, by_shares, by_ranges;
+    uint32_t ranges;                         // int4: ranges of a pair at most
     FastDiv span, halves;                    // positions that are cut into halves together (a block, or 16), and their halves
     int batch, heads, group, rows, tiles, pairs, shares;        // pairs = key/value heads * tiles, of one sequence
     int capacity, max_blocks;                // capacity = max_blocks * block_size
@@ -245,7 +253,8 @@ __device__ __forceinline__ float over_groups(float v, Op op)
 // 32 sequences of up to 4095, 8 heads of 128, blocks of 16: 62.9 us as kBlock, 74.4 as kRows; 16 masked ones, 32 heads of 80,
 // blocks of 24: 28.6 as kBlockMask, 36.4 as kRows; int8, 64 of up to 8192: 219.9 as kRows.  A short half wastes its operand's
 // rows, so kBlock loses with small blocks: 66.2 and 74.8 us for blocks of 8, 79.8 and 75 for 5, 84.9 and 75.4 for 4.
-enum Addressing { kRows, kBlock, kBlockAlike, kBlockMask };
+//   kPlain  int4: as Decode4 wants it
+enum Addressing { kRows, kBlock, kBlockAlike, kBlockMask, kPlain };
 
 // The images of an int4 word's codes i and i + 4: its bits 4 i and 16 + 4 i on, as the top mantissa bits of 16.0, the sign bit turned.
 template <int ACT>
@@ -709,6 +718,428 @@ struct Decode {
     }
 };
 
+// int4, the layout that a cache has as a rule: blocks of a multiple of 16 tokens, keys and values alike, scales and offsets alike
+// with those of four tokens of a head in 16 aligned bytes, no mask.  Every half of a tile then lies in one block and starts at 16
+// times its number.  A row is 72 bytes of memory for as much arithmetic as one of 256 in 16 bits, so it is instructions that Decode runs short
+// of, not memory or matrix cycles, and this is about their number:
+//   the bias of the key images is what the first MFMA's sum starts from; that of the value images is taken off at the end, with the
+//   sum of the rounded products P_j scale_j that one more MFMA keeps, so it cancels exactly and one bf16 term is enough: 2^-8 of the
+//   codes' part of a value, which is what 16-bit outputs carry (float16 keeps two terms)
+//   exponents are taken from a number m that is raised only where a score is more than kSlack above it, so the look at all lanes
+//   of a head is left out as a rule; sums stay below 2^kSlack of what they would be, far from the end of float32
+//   scales and offsets come one position to a lane and are handed round through LDS: one load where Decode has four
+// Against Decode as kBlock, 8 heads of 128: 32 sequences of up to 4095 25.7 and 33.9 us, 64 of up to 8192 61.2 and 91.9, one of 131071
+// 39.8 and 45.8, one of 37 6.7 and 6.7; 64 of up to 8192, heads of 64 49 and 64, of 80 61 and 94; 32 of them, of 256 64 and 92.
+// TOGETHER: a token's heads share cache lines, and other workgroups want what this one leaves.  Where heads have lines of their own, nobody
+// does, and requests are marked so (64 of up to 8192: 61.2 us, 66.5 unmarked; heads of 64 48.6 and 49.6, of 80 62 and 65; one of 131071 39.8
+// and 42) - but rows of 65 bytes and more come in two requests for the same line, which the mark makes two trips (heads of 256: 68 us and
+// 66; 32 of up to 4095, token by token, 50 and 44).
+template <int DP, int QT, bool TOGETHER>
+struct Decode4 {
+    static constexpr int NCH = DP / 32, KL = NCH / 2, PE = DP >= 128 ? 8 : 4, NP = DP / (16 * PE);
+    static constexpr int TERMS = QT == 1 ? 2 : 1;
+    static constexpr float kShift = 0.0f, kSlack = 8.0f, kNone = -3.402823466e38f;
+    static constexpr int HS = kStep / 4;                         // halves of a step of a wavefront: a tile
+    static constexpr int kOnce = TOGETHER || DP == 256 ? 0 : 2;              // cache-policy bit: not temporal
+
+    struct Place {                                               // of a step's halves
+        int n[HS], off[HS], id[HS];                              // positions seen, the first one's token within its block, its block
+    };
+
+    const Args a;
+    const int wave, col, g, D;
+    const bool wide;
+    uint32_t koff[KL], voff[4][NP];
+    uint32_t k[HS][KL][2], v[HS][4][NP];
+    float param[4];                                              // of position `lane` of the step: key scale, offset, value scale, offset
+    float *const lds;                                            // [4][64], of the whole step: key scale times scale2, key offset, value scale, value
+                                                                 // offset times value scale
+    u32x4 q[NCH];
+    f32x4 acc[NP][PE], bias;
+    float m, l, qsum, osum;
+
+    int len, half_end;
+    const int32_t *table;
+    const char *kbase, *vbase;
+    const char *ksbase, *kobase, *vsbase, *vobase;
+
+    __device__ Decode4(Args args, float *own) : Decode4(args, thread_now(), own) {}
+    __device__ __forceinline__ Decode4(Args args, int thread, float *own)
+        : a(args), wave(uniform(thread >> 6)), col(thread & 15), g((thread & 63) >> 4), D(args->cache.dim), wide(args->cache.dim % 32 == 0), lds(own)
+    {
+#pragma unroll
+        for (int c = 0; c < KL; c++) {
+            const int d = first_d(c);
+            koff[c] = d < D ? (uint32_t)col * (uint32_t)a->cache.key.token + d / 2 : kOutOfRange;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int h = 0; h < NP; h++) {
+                const int d = h * 128 + (PE == 4 ? col / 2 * 8 : col * PE);
+                voff[j][h] = d < D ? (uint32_t)(g * 4 + j) * (uint32_t)a->cache.key.token + d / 2 : kOutOfRange;
+            }
+    }
+
+    // first d of the lane's key piece c, 16 codes: from DP 128 on pieces 2 i and 2 i + 1 lie side by side
+    __device__ __forceinline__ int first_d(int c) const { return KL >= 2 ? c / 2 * 128 + g * 32 + c % 2 * 16 : g * 16; }
+
+    __device__ __forceinline__ void begin(int b, int kvh, int head0, int rows, int len_, int half_end_)
+    {
+        len = len_, half_end = half_end_;
+        table = a->table + b * a->table_stride;
+        kbase = a->cache.key.base + kvh * a->cache.key.head;
+        vbase = a->cache.value.base + kvh * a->cache.value.head;
+        ksbase = a->cache.key_scale.base + kvh * a->cache.key_scale.head;
+        kobase = a->cache.key_offset.base + kvh * a->cache.key_offset.head;
+        vsbase = a->cache.value_scale.base + kvh * a->cache.value_scale.head;
+        vobase = a->cache.value_offset.base + kvh * a->cache.value_offset.head;
+        const uint16_t *row = a->q + b * a->q_batch + (head0 + min(col, rows - 1)) * a->q_head;
+#pragma unroll
+        for (int c = 0; c < NCH; c++) {
+            const int d = first_d(c / 2) + c % 2 * 8;            // (D is a multiple of 16: a piece exists as a whole or not at all)
+            typedef u32x4 anywhere __attribute__((aligned(2)));
+            q[c] = u32x4{0, 0, 0, 0};
+            if (col < rows && d < D) q[c] = *(const Global<anywhere> *)(row + d);
+        }
+        osum = 0.0f;
+        m = kNone, l = 0.0f;
+        bias = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < NP; h++)
+#pragma unroll
+            for (int i = 0; i < PE; i++) acc[h][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // the query in the order of image4, (d, d + 4), and its sum
+    __device__ __forceinline__ void order_query()
+    {
+        qsum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NCH; c++) {
+            const u32x4 w = q[c];
+#pragma unroll
+            for (int i = 0; i < 4; i++) qsum += act_lo<QT>(w[i]) + act_hi<QT>(w[i]);
+            q[c] = u32x4{__builtin_amdgcn_perm(w.z, w.x, 0x05040100u), __builtin_amdgcn_perm(w.z, w.x, 0x07060302u),
+                         __builtin_amdgcn_perm(w.w, w.y, 0x05040100u), __builtin_amdgcn_perm(w.w, w.y, 0x07060302u)};
+        }
+        qsum = over_groups(qsum, [](float x, float y) { return x + y; });
+    }
+    __device__ __forceinline__ Place place(int first) const
+    {
+        Place p;
+        const uint32_t half = uniform((uint32_t)first), span = divide(half, a->halves);
+        const int off = (int)(half - span * a->halves.d) * kHalf;
+        if (a->halves.d % HS == 0) {                             // (a piece begins at a multiple of HS halves)
+            const int id = scalar_load(table + min(span, (uint32_t)a->max_blocks - 1));
+#pragma unroll
+            for (int s = 0; s < HS; s++) p.off[s] = off + s * kHalf, p.id[s] = id;
+        } else {
+#pragma unroll
+            for (int s = 0; s < HS; s++) {
+                const uint32_t span_s = s ? divide(half + s, a->halves) : span;
+                p.off[s] = s ? (int)(half + s - span_s * a->halves.d) * kHalf : off;
+                p.id[s] = scalar_load(table + min(span_s, (uint32_t)a->max_blocks - 1));
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < HS; s++) p.n[s] = min(max(min(len, half_end * kHalf) - (first + s) * kHalf, 0), kHalf);
+        return p;
+    }
+    // a block that the table does not name holds nothing
+    __device__ __forceinline__ void settle(Place &p) const
+    {
+        if (a->halves.d % HS == 0) {
+            if ((uint32_t)p.id[0] >= (uint32_t)a->cache.num_blocks)
+#pragma unroll
+                for (int s = 0; s < HS; s++) p.n[s] = 0, p.id[s] = 0;
+        } else {
+#pragma unroll
+            for (int s = 0; s < HS; s++)
+                if ((uint32_t)p.id[s] >= (uint32_t)a->cache.num_blocks) p.n[s] = 0, p.id[s] = 0;
+        }
+    }
+    __device__ __forceinline__ uint64_t start_of(const Place &p, int s) const
+    {
+        return (uint64_t)(uint32_t)p.id[s] * (uint32_t)a->cache.key.block + (uint32_t)p.off[s] * (uint32_t)a->cache.key.token;
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char *base, const Place &p, int s) const
+    {
+        const uint32_t reach = p.n[s] > 0 ? (uint32_t)(p.n[s] - 1) * (uint32_t)a->cache.key.token + D / 2 : 0;
+        return make_rsrc((const char *)((uint64_t)base + start_of(p, s)), reach);
+    }
+    // f(descriptor, scalar offset, half): where the halves' rows are - from the first one's on, if they are whole and of one block
+    template <class F>
+    __device__ __forceinline__ void each_half(const char *base, const Place &p, F f) const
+    {
+        if (full(p) && a->halves.d % HS == 0) {
+            const __amdgpu_buffer_rsrc_t r = make_rsrc((const char *)((uint64_t)base + start_of(p, 0)), 0x7fffffffu);
+#pragma unroll
+            for (int s = 0; s < HS; s++) f(r, (uint32_t)(s * kHalf) * (uint32_t)a->cache.key.token, s);
+        } else {
+#pragma unroll
+            for (int s = 0; s < HS; s++) f(rows_of(base, p, s), 0, s);
+        }
+    }
+    // (those of a half that ends early lie in its block all the same)
+    __device__ __forceinline__ void load_params(const Place &p)
+    {
+        uint32_t start = 0;
+#pragma unroll
+        for (int s = 0; s < HS; s++) {
+            const uint32_t of_half = (uint32_t)p.id[s] * (uint32_t)a->cache.key_scale.block + (uint32_t)p.off[s] * 4;
+            start = s == 0 || g == s ? of_half : start;          // (the groups behind the last half have the first one's)
+        }
+        start += col * 4;
+        param[0] = *(const Global<float> *)(at(ksbase) + start);
+        param[1] = *(const Global<float> *)(at(kobase) + start);
+        param[2] = *(const Global<float> *)(at(vsbase) + start);
+        param[3] = *(const Global<float> *)(at(vobase) + start);
+    }
+    // (a row of D % 32 == 0 is whole pieces of 16 bytes, of which a lane takes one)
+    __device__ __forceinline__ void load_keys(const Place &p)
+    {
+        each_half(kbase, p, [&](__amdgpu_buffer_rsrc_t r, uint32_t offset, int s) {
+            if constexpr (KL >= 2) {
+                if (wide) {
+#pragma unroll
+                    for (int c = 0; c < KL; c += 2) {
+                        const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(r, koff[c], offset, kOnce);
+                        k[s][c][0] = w.x, k[s][c][1] = w.y, k[s][c + 1][0] = w.z, k[s][c + 1][1] = w.w;
+                    }
+                    return;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < KL; c++) {
+                const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(r, koff[c], offset, kOnce);
+                k[s][c][0] = w.x, k[s][c][1] = w.y;
+            }
+        });
+    }
+    __device__ __forceinline__ void load_values(const Place &p)
+    {
+        each_half(vbase, p, [&](__amdgpu_buffer_rsrc_t r, uint32_t offset, int s) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int h = 0; h < NP; h++) v[s][j][h] = __builtin_amdgcn_raw_buffer_load_b32(r, voff[j][h], offset, kOnce);
+        });
+    }
+    // parameter i of the lane's four positions of half s
+    __device__ __forceinline__ f32x4 four(int i, int s) const { return *reinterpret_cast<const f32x4 *>(lds + i * 64 + s * 16 + g * 4); }
+    // bit 4 s + r: position 4 g + r of half s is seen
+    __device__ __forceinline__ uint32_t seen(const Place &p) const
+    {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int s = 0; s < HS; s++) bits |= ((1u << min(max(p.n[s] - g * 4, 0), 4)) - 1) << (4 * s);
+        return bits;
+    }
+    __device__ static __forceinline__ bool full(const Place &p) { return p.n[0] + p.n[1] == HS * kHalf; }
+    __device__ static __forceinline__ void no_select() { asm volatile(""); }
+    // (of fmaxf the compiler would make two instructions for each, for signalling NaNs)
+    __device__ static __forceinline__ float max3(float x, float y, float z)
+    {
+        float r;
+        asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+        return r;
+    }
+
+    // z_j over its factor, four(0)
+    __device__ __forceinline__ void score(f32x4 (&z)[HS]) const
+    {
+        const float less = -kBias4 * qsum;
+#pragma unroll
+        for (int s = 0; s < HS; s++) {
+            z[s] = f32x4{less, less, less, less};
+#pragma unroll
+            for (int i = 0; i < NCH; i++) {
+                const uint32_t w = k[s][i / 2][i % 2];
+                z[s] = mfma_act<QT>(u32x4{image4<QT>(w, 0), image4<QT>(w, 1), image4<QT>(w, 2), image4<QT>(w, 3)}, q[i], z[s]);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < HS; s++) {
+            const f32x4 ko = four(1, s);
+#pragma unroll
+            for (int r = 0; r < 4; r++) z[s][r] = __builtin_fmaf(ko[r], qsum, z[s][r]);
+        }
+    }
+    __device__ __forceinline__ void store_scores(const f32x4 (&z)[HS], uint32_t valid, int b, int head0, int rows, int first) const
+    {
+        if (col >= rows) return;
+        Global<float> *to = at(a->scores) + ((int64_t)b * a->heads + head0 + col) * a->score_pitch + g * 4;
+#pragma unroll
+        for (int s = 0; s < HS; s++) {
+            const int key = (first + s) * kHalf;
+            if (first + s >= half_end || key + g * 4 >= len) continue;       // (positions are stored in fours, the pitch is one of theirs)
+            const f32x4 t = four(0, s);
+            f32x4 w;
+#pragma unroll
+            for (int r = 0; r < 4; r++) w[r] = (valid >> (4 * s + r)) & 1 ? z[s][r] * t[r] : -INFINITY;
+            *(Global<f32x4> *)(to + key) = w;
+        }
+    }
+    // probabilities times value scales
+    __device__ __forceinline__ void add(const Place &place, uint32_t valid, const f32x4 (&z)[HS], u32x4 (&terms)[TERMS])
+    {
+        constexpr int N = HS * 4;
+        float e[N];
+        const auto exponents = [&] {
+#pragma unroll
+            for (int s = 0; s < HS; s++) {
+                const f32x4 t = four(0, s);
+#pragma unroll
+                for (int r = 0; r < 4; r++) e[4 * s + r] = __builtin_fmaf(z[s][r], t[r], -m);
+            }
+            if (!full(place)) {
+                no_select();
+#pragma unroll
+                for (int i = 0; i < N; i++) e[i] = (valid >> i) & 1 ? e[i] : -INFINITY;
+            }
+        };
+        exponents();
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) top = max3(top, e[i], e[i + 1]);
+        if (__any(top > kSlack)) {
+            top = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < HS; s++) {
+                const f32x4 t = four(0, s);
+#pragma unroll
+                for (int r = 0; r < 4; r++) top = fmaxf(top, (valid >> (4 * s + r)) & 1 ? z[s][r] * t[r] : -INFINITY);
+            }
+            top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
+            const float higher = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - higher);
+            m = higher;
+            l *= f;
+            osum *= f;
+            bias *= f;
+#pragma unroll
+            for (int h = 0; h < NP; h++)
+#pragma unroll
+                for (int i = 0; i < PE; i++) acc[h][i] *= f;
+            exponents();
+        }
+#pragma unroll
+        for (int s = 0; s < HS; s++) {
+            f32x4 vs = four(2, s), vo = four(3, s);
+            float p[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                p[r] = __builtin_amdgcn_exp2f(e[4 * s + r]);
+                l += p[r];
+            }
+            if (!full(place)) {                                  // (a scale and an offset that are not seen may be anything)
+                no_select();
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    vs[r] = (valid >> (4 * s + r)) & 1 ? vs[r] : 0.0f;
+                    vo[r] = (valid >> (4 * s + r)) & 1 ? vo[r] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                osum = __builtin_fmaf(p[r], vo[r], osum);
+                p[r] = p[r] * vs[r];
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int to = s * 2 + i;
+                terms[0][to] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
+                if constexpr (TERMS > 1) terms[1][to] = pack_bf16x2(p[2 * i] - bf16_lo(terms[0][to]), p[2 * i + 1] - bf16_hi(terms[0][to]));
+            }
+        }
+    }
+    __device__ __forceinline__ void weigh(const u32x4 (&terms)[TERMS])
+    {
+#pragma unroll
+        for (int n = 0; n < TERMS; n++) bias = mfma_act<0>(u32x4{kOnes2<0>, kOnes2<0>, kOnes2<0>, kOnes2<0>}, terms[n], bias);
+#pragma unroll
+        for (int h = 0; h < NP; h++) {
+            uint32_t pairs[4][2];                                // the low and the high halves of the words of two positions
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const uint32_t x = v[w / 2][w % 2 * 2][h], y = v[w / 2][w % 2 * 2 + 1][h];
+                pairs[w][0] = __builtin_amdgcn_perm(y, x, PE == 4 && col & 1 ? 0x07060302u : 0x05040100u);
+                pairs[w][1] = PE == 4 ? 0 : __builtin_amdgcn_perm(y, x, 0x07060302u);
+            }
+#pragma unroll
+            for (int i = 0; i < PE; i++) {
+                const u32x4 image = {image4<0>(pairs[0][i / 4], i % 4), image4<0>(pairs[1][i / 4], i % 4), image4<0>(pairs[2][i / 4], i % 4),
+                                     image4<0>(pairs[3][i / 4], i % 4)};
+#pragma unroll
+                for (int n = 0; n < TERMS; n++) acc[h][i] = mfma_act<0>(image, terms[n], acc[h][i]);
+            }
+        }
+    }
+
+    // Wavefronts that have come less far go first: those of a compute unit then end together (64 sequences of up to 8192: 61.2 us, 62.7
+    // without; 32 of up to 4095 26.6 and 27.5).
+    __device__ static __forceinline__ void set_priority(int quarters)
+    {
+        if (quarters == 3) __builtin_amdgcn_s_setprio(3);
+        else if (quarters == 2) __builtin_amdgcn_s_setprio(2);
+        else if (quarters == 1) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+    }
+
+    // The wavefront's steps of the halves from `from` to half_end, requested as in Decode::run.  A step's parameters come one to a lane
+    // and are handed round through LDS, so that a step ahead of them is four registers.
+    __device__ __forceinline__ void run(int from, int b, int head0, int rows)
+    {
+        int first = from + wave * HS;
+        const int end = half_end;
+        Place cur = place(first);
+        settle(cur);
+        load_keys(cur);
+        load_params(cur);
+        __builtin_amdgcn_sched_barrier(0);
+        load_values(cur);
+        __builtin_amdgcn_sched_barrier(0);
+        order_query();
+        Place next = place(first + 4 * HS);
+        int behind = 4, quarter_end = from;                      // quarters that are not done
+        for (; first < end; first += 4 * HS) {
+            if (first >= quarter_end) {
+                quarter_end += (end - from) / 4;
+                set_priority(--behind);
+            }
+            uint32_t valid = (1u << (4 * HS)) - 1;
+            if (!full(cur)) {
+                no_select();
+                valid = seen(cur);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) lds[i * 64 + g * 16 + col] = i == 0 ? param[0] * a->scale2 : i == 3 ? param[3] * param[2] : param[i];
+            __builtin_amdgcn_wave_barrier();                     // (a wavefront's LDS accesses are done in their order)
+            f32x4 z[HS];
+            score(z);
+            if (a->scores) store_scores(z, valid, b, head0, rows, first);
+            settle(next);
+            load_keys(next);
+            load_params(next);
+            __builtin_amdgcn_sched_barrier(0);
+            u32x4 terms[TERMS];
+            add(cur, valid, z, terms);
+            weigh(terms);
+            __builtin_amdgcn_wave_barrier();
+            load_values(next);
+            __builtin_amdgcn_sched_barrier(0);
+            cur = next;
+            next = place(first + 8 * HS);
+        }
+        osum = __builtin_fmaf(-kBias4, bias[0], over_groups(osum, [](float x, float y) { return x + y; }));
+#pragma unroll
+        for (int h = 0; h < NP; h++)
+#pragma unroll
+            for (int i = 0; i < PE; i++) acc[h][i] += osum;
+        m = m == kNone ? -INFINITY : m;                          // nothing seen: sums of 0 - or NaN, from NaN scores
+    }
+};
+
 template <int QT>
 __device__ __forceinline__ void store_out(Args a, int64_t row, int d, f32x4 v)
 {
@@ -793,19 +1224,18 @@ __device__ __forceinline__ float row_sum(float v)
     return __shfl(v, 15, 16);
 }
 
-// Adds the sums of n cut pieces, first, first + step, ..., in this order, into `own`, which already holds those of number
+// Adds the sums of n cut pieces at place(0), place(1), ..., ascending, in this order, into `own`, which already holds those of number
 // `mine`.  A thread adds one quad, eight partials in flight; where there are fewer quads than threads, several share the
 // partials of a quad.  What the partials weigh is worked out meanwhile, 16 lanes to a head.
 constexpr int kFlight = 8;
 constexpr int kJoin = 64;                                        // sums of one call at most
 constexpr size_t kJoinLds = (kJoin * kHeads + 256 * 4) * sizeof(float);
-template <int DP>
-__device__ void join(Args a, const Sums<DP> &own, int mine, uint32_t first, uint32_t step, int n, int rows, float *lds)
+template <int DP, class Place>
+__device__ void join(Args a, const Sums<DP> &own, int mine, Place place, int n, int rows, float *lds)
 {
     constexpr int QPR = DP / 4;
     const int thread = thread_now();
     const uint32_t row_bytes = DP * 4, place_bytes = (uint32_t)a->rows * row_bytes;
-    const auto place = [&](int i) { return first + (uint32_t)i * step; };
     // ends with the last of them: a request for number n or a later one reads zeros
     const __amdgpu_buffer_rsrc_t part = make_rsrc(a->part, uniform((place(n - 1) + 1) * place_bytes));
     const __amdgpu_buffer_rsrc_t mls = make_rsrc(a->part_ml, uniform((place(n - 1) + 1) * kHeads * 8));
@@ -885,20 +1315,119 @@ __device__ __forceinline__ bool arrive(Global<uint32_t> *counter, int n, int *ld
     return uniform(*lds) != 0;
 }
 
-template <int DP, int BITS, int QT, Addressing AD>
-__global__ __launch_bounds__(256, resident(DP, BITS < 16)) void paged_decode_kernel(AttnArgs)
-{
-    using W = Decode<DP, BITS, QT, AD>;
-    constexpr int RP = 128 + 4;                                  // row pitch of a wavefront's sums in LDS
-    __shared__ float red[4][kHeads][RP];
-    __shared__ float ml[4][kHeads][2];
-    __shared__ float all_wide[W::NP > 1 ? kHeads : 1][Sums<DP>::RP];     // the workgroup's sums: the first wavefront's place, if they fit
-    __shared__ float all_ml[kHeads][2];
-    __shared__ int counted[2];
-    static_assert(W::NP > 1 || Sums<DP>::RP == RP, "the workgroup's sums lie where a wavefront's were");
+// What the wavefronts of a workgroup share.
+template <int DP>
+struct Shared {
+    static constexpr int RP = 128 + 4;                           // row pitch of a wavefront's sums
+    static constexpr int NP = DP / 128 ? DP / 128 : 1;           // pieces of 128 (or 64) outputs
+    alignas(16) float red[4][kHeads][RP];
+    alignas(16) float ml[4][kHeads][2];
+    alignas(16) float all_wide[NP > 1 ? kHeads : 1][Sums<DP>::RP];           // the workgroup's sums: the first wavefront's place, if they fit
+    alignas(16) float all_ml[kHeads][2];
+    int counted[2];
+    int last_here;
+    static_assert(NP > 1 || Sums<DP>::RP == RP, "the workgroup's sums lie where a wavefront's were");
     static_assert(sizeof(red) - sizeof(red[0]) >= kJoinLds, "join works behind the workgroup's sums");
-    __shared__ int last_here;
+};
 
+// The end of a piece, number `number` of n of a pair, with the sums of this workgroup's four wavefronts; place(i): where piece i's
+// sums lie in the workspace.
+template <int DP, int QT, int NP, int PE, class Place>
+__device__ __forceinline__ void end_piece(Shared<DP> &lds, const f32x4 (&acc)[NP][PE], float l, float m, int64_t out_row, int rows, int n, int number, Place place,
+                                          float shift)
+{
+    const Args a = args_now();
+    Global<uint32_t> *arrived = at(a->arrived);
+    // Of a pair that is cut, the last of its workgroups to arrive adds everybody's sums.  Where those are more than 64 KiB, groups
+    // of about the root of their number are added first, so that no workgroup has many to read (one sequence of 8000, 16
+    // query heads each: 19.5 us, 25.7 without groups; with 4 heads each and 4000 tokens 11.9 us at once, 13.8 in groups).  The
+    // counter of a group is its first piece's, that of the groups lies behind all of these.
+    int size = n, group = 0, groups = 1;
+    if (n >= kJoin || n * rows * (DP / 4) > 512 * kFlight) {
+        size = 8;
+        while (size * size < n) size += 4;
+        group = uniform(number / size), groups = uniform((n + size - 1) / size);
+    }
+    const int members = min(size, n - group * size);
+    const uint32_t whole = place(0), first = place(group * size), behind = 2 * (uint32_t)a->shares;
+    uint32_t seen = 0;                                       // how many have arrived: requested here, looked at behind what follows
+    if (n > 1 && threadIdx.x < 2)
+        seen = __hip_atomic_load(arrived + (threadIdx.x ? behind + whole : first), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+
+    // the four wavefronts' sums on a common maximum
+    const int thread = thread_now(), lane = thread & 63, wave = thread >> 6, col = lane & 15, g = lane >> 4;
+    const Sums<DP> own = {NP > 1 ? lds.all_wide : reinterpret_cast<float (*)[Sums<DP>::RP]>(lds.red[0]), lds.all_ml};
+    l = over_groups(l, [](float x, float y) { return x + y; });
+    if (g == 0) lds.ml[wave][col][0] = m, lds.ml[wave][col][1] = l;
+    __syncthreads();
+    const float top = fmaxf(fmaxf(lds.ml[0][col][0], lds.ml[1][col][0]), fmaxf(lds.ml[2][col][0], lds.ml[3][col][0]));
+    const float f = weight_of(m, top);
+    if (thread < kHeads) {
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) total += lds.ml[i][col][1] * weight_of(lds.ml[i][col][0], top);
+        lds.all_ml[col][0] = top, lds.all_ml[col][1] = total;
+    }
+#pragma unroll
+    for (int h = 0; h < NP; h++) {
+        if (h) __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int i = 0; i < PE; i += 4)
+                *reinterpret_cast<f32x4 *>(&lds.red[wave][col][(g * 4 + r) * PE + i]) =
+                    f32x4{acc[h][i][r] * f, acc[h][i + 1][r] * f, acc[h][i + 2][r] * f, acc[h][i + 3][r] * f};
+        __syncthreads();
+        constexpr int QPR = 16 * PE / 4;                  // quads of a row
+        for (int e = thread; e < rows * QPR; e += 256) {
+            const int row = e / QPR, d = (e % QPR) * 4;
+            f32x4 sum = *reinterpret_cast<const f32x4 *>(&lds.red[0][row][d]);
+#pragma unroll
+            for (int i = 1; i < 4; i++) sum += *reinterpret_cast<const f32x4 *>(&lds.red[i][row][d]);
+            own.quad(row, h * 128 + d) = sum;
+        }
+    }
+    if (thread < 2) lds.counted[thread] = (int)seen;
+    __syncthreads();
+
+    bool done = true;
+    const auto last_of = [&](Global<uint32_t> *counter, int of, int seen, uint32_t place) {
+        if (of == 1) return true;
+        if (seen == of - 1) {                                // everybody else was there already: nobody waits for these sums
+            if (thread == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            return true;
+        }
+        publish<DP>(a, own, place, rows);
+        return arrive(counter, of, &lds.last_here);
+    };
+    const int seen0 = uniform(lds.counted[0]), seen1 = uniform(lds.counted[1]);
+#pragma unroll 1
+    for (int level = 0; level < 2 && done; level++) {        // within the group, among the groups
+        const int of = level ? groups : members;
+        done = last_of(arrived + (level ? behind + whole : first), of, level ? seen1 : seen0, level ? first : place(number));
+        const int from = level ? 0 : group * size, step = level ? size : 1;
+        if (done && of > 1) join<DP>(a, own, level ? group : number - from, [&](int i) { return place(from + i * step); }, of, rows, &lds.red[1][0][0]);
+    }
+    if (done) finish<DP, QT>(args_now(), own, out_row, rows, shift);
+    __syncthreads();                                             // ml and red are free again
+}
+
+// outputs of the sequences without positions
+__device__ __forceinline__ void clear_empty()
+{
+    const Args a = args_now();
+    for (int e = blockIdx.x; e < a->batch; e += gridDim.x) {
+        if (clamp_len(a, scalar_load(a->lens + e)) != 0) continue;
+        for (int i = threadIdx.x; i < a->heads * a->cache.dim; i += 256) at(a->out)[(int64_t)e * a->heads * a->cache.dim + i] = 0;
+        for (int i = threadIdx.x; i < a->heads; i += 256)
+            if (a->lse) at(a->lse)[(int64_t)e * a->heads + i] = -INFINITY;
+    }
+}
+
+template <int DP, int QT, class W>
+__device__ __forceinline__ void decode_pieces()
+{
+    __shared__ Shared<DP> lds;
     const Pieces pieces = [] {
         const Args a = args_now();
         uint32_t lines = 0;                                      // the arguments' cache lines, for the phases that follow
@@ -933,7 +1462,7 @@ __global__ __launch_bounds__(256, resident(DP, BITS < 16)) void paged_decode_ker
                 pair = uniform(in / count), number = uniform((int)(in - pair * count));
             }
             first_cut = cut_before * (uint32_t)a->pairs + pair * count;
-            const int kvh = (int)pair / a->tiles, halves = (int)halves_of(a, len), units = (halves + kUnit - 1) / kUnit;
+            const int kvh = a->tiles == 1 ? (int)pair : uniform((int)pair / a->tiles), halves = (int)halves_of(a, len), units = (halves + kUnit - 1) / kUnit;
             head0 = kvh * a->group + ((int)pair - kvh * a->tiles) * kHeads;
             rows = min(kHeads, (kvh + 1) * a->group - head0);
             // the first units % n pieces have one more unit
@@ -948,92 +1477,133 @@ __global__ __launch_bounds__(256, resident(DP, BITS < 16)) void paged_decode_ker
                 for (int i = 0; i < W::PE; i++) acc[h][i] = w.acc[h][i];
         }
 
-        const Args a = args_now();
-        const int64_t out_row = (int64_t)b * a->heads + head0;
-        Global<uint32_t> *arrived = at(a->arrived);
-        // Of a pair that is cut, the last of its workgroups to arrive adds everybody's sums.  Where those are more than 64 KiB, groups
-        // of about the root of their number are added first, so that no workgroup has many to read (one sequence of 8000, 16
-        // query heads each: 19.5 us, 25.7 without groups; with 4 heads each and 4000 tokens 11.9 us at once, 13.8 in groups).  The
-        // counter of a group is its first piece's, that of the groups lies behind all of these.
-        int size = n;
-        if (n >= kJoin || n * rows * (DP / 4) > 512 * kFlight) {
-            size = 8;
-            while (size * size < n) size += 4;
-        }
-        const int group = number / size, groups = (n + size - 1) / size, members = min(size, n - group * size);
-        const uint32_t first = first_cut + group * size, behind = 2 * (uint32_t)a->shares;
-        uint32_t seen = 0;                                       // how many have arrived: requested here, looked at behind what follows
-        if (n > 1 && threadIdx.x < 2)
-            seen = __hip_atomic_load(arrived + (threadIdx.x ? behind + first_cut : first), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-
-        // the four wavefronts' sums on a common maximum
-        const int thread = thread_now(), lane = thread & 63, wave = thread >> 6, col = lane & 15, g = lane >> 4;
-        const Sums<DP> own = {W::NP > 1 ? all_wide : reinterpret_cast<float (*)[Sums<DP>::RP]>(red[0]), all_ml};
-        l = over_groups(l, [](float x, float y) { return x + y; });
-        if (g == 0) ml[wave][col][0] = m, ml[wave][col][1] = l;
-        __syncthreads();
-        const float top = fmaxf(fmaxf(ml[0][col][0], ml[1][col][0]), fmaxf(ml[2][col][0], ml[3][col][0]));
-        const float f = weight_of(m, top);
-        if (thread < kHeads) {
-            float total = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) total += ml[i][col][1] * weight_of(ml[i][col][0], top);
-            all_ml[col][0] = top, all_ml[col][1] = total;
-        }
-#pragma unroll
-        for (int h = 0; h < W::NP; h++) {
-            if (h) __syncthreads();
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int i = 0; i < W::PE; i += 4)
-                    *reinterpret_cast<f32x4 *>(&red[wave][col][(g * 4 + r) * W::PE + i]) =
-                        f32x4{acc[h][i][r] * f, acc[h][i + 1][r] * f, acc[h][i + 2][r] * f, acc[h][i + 3][r] * f};
-            __syncthreads();
-            constexpr int QPR = 16 * W::PE / 4;                  // quads of a row
-            for (int e = thread; e < rows * QPR; e += 256) {
-                const int row = e / QPR, d = (e % QPR) * 4;
-                f32x4 sum = *reinterpret_cast<const f32x4 *>(&red[0][row][d]);
-#pragma unroll
-                for (int i = 1; i < 4; i++) sum += *reinterpret_cast<const f32x4 *>(&red[i][row][d]);
-                own.quad(row, h * 128 + d) = sum;
-            }
-        }
-        if (thread < 2) counted[thread] = (int)seen;
-        __syncthreads();
-
-        bool done = true;
-        const auto last_of = [&](Global<uint32_t> *counter, int of, int seen, uint32_t place) {
-            if (of == 1) return true;
-            if (seen == of - 1) {                                // everybody else was there already: nobody waits for these sums
-                if (thread == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                return true;
-            }
-            publish<DP>(a, own, place, rows);
-            return arrive(counter, of, &last_here);
-        };
-        const int seen0 = uniform(counted[0]), seen1 = uniform(counted[1]);
-#pragma unroll 1
-        for (int level = 0; level < 2 && done; level++) {        // within the group, among the groups
-            const int of = level ? groups : members;
-            done = last_of(arrived + (level ? behind + first_cut : first), of, level ? seen1 : seen0, first + (level ? 0 : number - group * size));
-            if (done && of > 1)
-                join<DP>(a, own, level ? group : number - group * size, level ? first_cut : first, level ? (uint32_t)size : 1u, of, rows, &red[1][0][0]);
-        }
-        if (done) finish<DP, QT>(args_now(), own, out_row, rows, W::kShift);
-        __syncthreads();                                         // ml and red are free again
+        end_piece<DP, QT>(lds, acc, l, m, (int64_t)b * args_now()->heads + head0, rows, n, number, [&](int i) { return first_cut + (uint32_t)i; }, W::kShift);
     }
 
-    if (!pieces.empty) return;
-    const Args a = args_now();
-    for (int e = blockIdx.x; e < a->batch; e += gridDim.x) {
-        if (clamp_len(a, scalar_load(a->lens + e)) != 0) continue;
-        for (int i = threadIdx.x; i < a->heads * a->cache.dim; i += 256) at(a->out)[(int64_t)e * a->heads * a->cache.dim + i] = 0;
-        for (int i = threadIdx.x; i < a->heads; i += 256)
-            if (a->lse) at(a->lse)[(int64_t)e * a->heads + i] = -INFINITY;
-    }
+    if (pieces.empty) clear_empty();
 }
 
+// How Decode4's work is cut up: kStart and the halves of all sequences, one after the other, into ranges of `share`, the same for every
+// pair, as many as the card holds workgroups at once.  A workgroup takes one range of one pair, which may end one sequence and begin the
+// next; a sequence's pieces are the ranges that it touches.  Equal pieces per pair (Pieces) are more than fit at once, and the last
+// few run alone; here, where a start and an end cost as much as 400 positions, that is what counts most.
+struct Ranges {
+    uint32_t share, before, mine, total;     // halves of a range; of the runs before this lane's, of it, of all
+    int run, len;                            // sequences per lane; the length of the first
+    bool empty;                              // there is a sequence without positions
+
+    __device__ explicit Ranges(Args a)
+    {
+        const int lane = threadIdx.x & 63, batch = a->batch;
+        run = (batch + 63) / 64;
+        const int first = lane * run, end = min(first + run, batch);
+        len = first < batch ? clamp_len(a, at(a->lens)[first]) : 0;
+        mine = cost_of(a, len);
+        bool none = first < batch && len == 0;
+        for (int i = first + 1; i < end; i++) {
+            const uint32_t cost = cost_of(a, clamp_len(a, at(a->lens)[i]));
+            none = none || cost == 0;
+            mine += cost;
+        }
+        empty = __any(none);
+        const uint32_t scan = scan_lanes(mine, Add());
+        before = scan - mine;
+        total = (uint32_t)__builtin_amdgcn_readlane((int)scan, 63);
+        // (at least one step of the workgroup)
+        share = max(divide(total + a->ranges - 1, a->by_ranges), (uint32_t)(kStep + kStart));
+    }
+    __device__ static uint32_t cost_of(Args a, int len) { return len ? halves_of(a, len) + kStart : 0; }
+    // the sequence that holds y, its length, and what comes before it
+    __device__ void find(Args a, uint32_t y, int &b, int &length, uint32_t &start) const
+    {
+        const int lane = __builtin_ctzll(__ballot(y >= before && y - before < mine));
+        b = lane * run;
+        start = (uint32_t)__builtin_amdgcn_readlane((int)before, lane);
+        length = __builtin_amdgcn_readlane(len, lane);
+        uint32_t cost = cost_of(a, length);
+        while (y - start >= cost) {
+            start += cost;
+            length = clamp_len(a, scalar_load(a->lens + ++b));
+            cost = cost_of(a, length);
+        }
+    }
+};
+
+template <int DP, int QT, bool TOGETHER>
+__global__ __launch_bounds__(256, resident4(DP)) void paged_decode4_kernel(AttnArgs)
+{
+    using W = Decode4<DP, QT, TOGETHER>;
+    __shared__ Shared<DP> lds;
+    static_assert(sizeof(lds.red[0]) >= 4 * 64 * sizeof(float), "a wavefront's parameters lie where its sums will be");
+    const Ranges ranges = [] {
+        const Args a = args_now();
+        uint32_t lines = 0;                                      // the arguments' cache lines, for the phases that follow
+#pragma unroll
+        for (size_t i = 0; i < sizeof(AttnArgs); i += 64) lines |= *(const __attribute__((address_space(4))) uint32_t *)((const __attribute__((address_space(4))) char *)a + i);
+        const Ranges r(a);
+        asm volatile("" ::"s"(lines));
+        return r;
+    }();
+    const uint32_t share = uniform(ranges.share), total = uniform(ranges.total), pairs = (uint32_t)args_now()->pairs, all = args_now()->ranges * pairs;
+
+    for (uint32_t turn = blockIdx.x; turn < (all + kDealt - 1) / kDealt * kDealt; turn += gridDim.x) {
+        // TOGETHER: the pairs of a range side by side, eight of them on one XCD
+        const uint32_t piece = TOGETHER ? (turn & ~(kDealt - 1)) | ((turn & 7) << 3) | ((turn >> 3) & 7) : turn;
+        const uint32_t major = TOGETHER ? divide(piece, args_now()->by_pairs) : divide(piece, args_now()->by_ranges);
+        const uint32_t range = TOGETHER ? major : piece - major * args_now()->ranges, pair = TOGETHER ? piece - major * pairs : major;
+        if (piece >= all || range * share >= total) continue;
+        const uint32_t range_end = min(range * share + share, total);
+        uint32_t from = range * share, start;
+        int b, len;
+        ranges.find(args_now(), from, b, len, start);
+        b = uniform(b), len = uniform(len), start = uniform(start);
+#pragma unroll 1
+        for (;;) {
+            int head0, rows, n, number;
+            float l, m;
+            f32x4 acc[W::NP][W::PE];
+            // a sequence's first kStart are its cost alone, its halves follow; it is cut at multiples of a step of a wavefront
+            const uint32_t halves = uniform(halves_of(args_now(), len)), begin = start + kStart;
+            const auto cut = [&](uint32_t at) { return begin + min(at > begin ? (at - begin + W::HS - 1) / W::HS * W::HS : 0, halves); };
+            const uint32_t to = cut(range_end);
+            from = cut(from);
+            // the ranges that hold the first and the last of its steps: this one as a rule, and divisions take a while
+            const uint32_t last = begin + (halves - 1) / W::HS * W::HS;
+            const uint32_t first_range = begin >= range * share ? range : uniform(begin / share), last_range = last < range_end ? range : uniform(last / share);
+            if (from < to) {
+                {
+                    const Args a = args_now();
+                    W w(a, &lds.red[uniform(thread_now() >> 6)][0][0]);
+                    const int kvh = a->tiles == 1 ? (int)pair : uniform((int)pair / a->tiles);
+                    head0 = kvh * a->group + ((int)pair - kvh * a->tiles) * kHeads;
+                    rows = min(kHeads, (kvh + 1) * a->group - head0);
+                    n = (int)(last_range - first_range + 1), number = (int)(range - first_range);
+                    w.begin(b, kvh, head0, rows, len, (int)(to - begin));
+                    w.run((int)(from - begin), b, head0, rows);
+                    l = w.l, m = w.m;
+#pragma unroll
+                    for (int h = 0; h < W::NP; h++)
+#pragma unroll
+                        for (int i = 0; i < W::PE; i++) acc[h][i] = w.acc[h][i];
+                }
+                // a range has a piece that goes on in the next one, and one that came from the range before and ends here, at most
+                const auto place = [&](int i) { return ((first_range + i) * 2 + (i < n - 1 ? 1 : 0)) * pairs + pair; };
+                end_piece<DP, QT>(lds, acc, l, m, (int64_t)b * args_now()->heads + head0, rows, n, number, place, W::kShift);
+            }
+            if (begin + halves >= range_end) break;
+            from = start = begin + halves;
+            do len = uniform(clamp_len(args_now(), scalar_load(args_now()->lens + ++b)));
+            while (len == 0);                                    // (there are halves left, so a sequence with some follows)
+        }
+    }
+    if (ranges.empty) clear_empty();
+}
+
+template <int DP, int BITS, int QT, Addressing AD>
+__global__ __launch_bounds__(256, resident(DP, BITS < 16)) void paged_decode_kernel(AttnArgs)
+{
+    decode_pieces<DP, QT, Decode<DP, BITS, QT, AD>>();
+}
 // attn_sums[b, kv head, j] += sum over the kv head's query heads of 2^(z_j - lse2), in the heads' order.  Four positions per
 // thread, four heads requested at once; what was hidden has z = -infinity.  Bound by latency: 16 sequences of 4097, 32 heads on
 // 8, 12.6 MB in 5.2 us (5.8 with one head at a time).
@@ -1112,6 +1682,7 @@ bool plan_attention(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head
     return true;
 }
 static_assert(resident(256, false) <= resident(256, true), "the workspace's size");
+static_assert(resident4(128) <= resident(128, true) && resident4(256) <= resident(256, true), "a range leaves two sums at most");
 static_assert(kNumCU * 3 * 4 * sizeof(uint32_t) <= kWorkspaceCounterBytes, "arrival counters");
 static_assert(kNumCU * 3 <= (kJoin / 2) * (kJoin / 2), "groups of pieces, and members of a group");
 
@@ -1125,12 +1696,23 @@ void launch_attention(const AttnArgs &a, Addressing ad, unsigned workgroups, hip
     else if constexpr (BITS < 16) hipLaunchKernelGGL((paged_decode_kernel<DP, BITS, QT, kBlockAlike>), grid, block, 0, s, a);
 }
 
+template <int DP, int QT>
+void launch_attention4(const AttnArgs &a, Addressing ad, unsigned workgroups, hipStream_t s)
+{
+    const dim3 grid(workgroups), block(256);
+    if (ad == kPlain && a.together) hipLaunchKernelGGL((paged_decode4_kernel<DP, QT, true>), grid, block, 0, s, a);
+    else if (ad == kPlain) hipLaunchKernelGGL((paged_decode4_kernel<DP, QT, false>), grid, block, 0, s, a);
+    else if (ad == kRows) hipLaunchKernelGGL((paged_decode_kernel<DP, 4, QT, kRows>), grid, block, 0, s, a);
+    else if (ad == kBlockMask) hipLaunchKernelGGL((paged_decode_kernel<DP, 4, QT, kBlockMask>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((paged_decode_kernel<DP, 4, QT, kBlock>), grid, block, 0, s, a);
+}
+
 template <int DP>
 void launch_attention(const AttnArgs &a, int bits, bool fp16, Addressing ad, unsigned workgroups, hipStream_t s)
 {
     if (bits == 4) {
-        if (fp16) launch_attention<DP, 4, 1>(a, ad, workgroups, s);
-        else launch_attention<DP, 4, 0>(a, ad, workgroups, s);
+        if (fp16) launch_attention4<DP, 1>(a, ad, workgroups, s);
+        else launch_attention4<DP, 0>(a, ad, workgroups, s);
     } else if (bits == 8) {
         if (fp16) launch_attention<DP, 8, 1>(a, ad, workgroups, s);
         else launch_attention<DP, 8, 0>(a, ad, workgroups, s);
@@ -1223,7 +1805,11 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     const auto alike = [](const PagedArray &x, const PagedArray &y) { return x.block == y.block && x.token == y.token && x.head == y.head; };
     const bool same = quant && scales && alike(a.cache.key, a.cache.value) && alike(a.cache.key_scale, a.cache.value_scale) &&
                       (bits == 8 || (alike(a.cache.key_scale, a.cache.key_offset) && alike(a.cache.key_scale, a.cache.value_offset)));
-    const Addressing ad = !blocks ? kRows : mask ? kBlockMask : same ? kBlockAlike : kBlock;
+    // Decode4: offsets into a whole array of parameters have 32 bits, and so do the halves of all sequences; a few steps behind the
+    // last position still have a number in 31
+    const bool plain = bits == 4 && same && cache->block_size % 16 == 0 && a.cache.key_scale.block <= 0xffffffffll / cache->num_blocks &&
+                       a.capacity < 0x7fff0000 && batch * (a.capacity / kHalf + (int64_t)kStart) < 0x7fff0000;
+    const Addressing ad = !blocks ? kRows : mask ? kBlockMask : plain ? kPlain : same && bits == 8 ? kBlockAlike : kBlock;
     // Rows of several heads in a cache line, with other heads' rows of the same token: work on them at the same time and on one XCD,
     // so that the line comes once (16 sequences of up to 1001 tokens, 32 heads of 80: 32.4 -> 28.6 us; int8, 32 sequences of up to
     // 4095, 8 heads of 64: 34.5 -> 26.2 us).  Where heads have lines of their own, that would make the workgroups ask the same
@@ -1232,6 +1818,15 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     a.together = shared(a.cache.key) || shared(a.cache.value);
     a.span = ad != kRows ? a.cache.page : fast_div(kHalf);
     a.halves = fast_div((a.span.d + kHalf - 1) / kHalf);
+    if (ad == kPlain) {
+        a.shares = kNumCU * resident4((int)p.dp);
+        // as many as the card holds, or as full sequences would make
+        const int64_t most = (batch * (a.capacity / kHalf + (int64_t)kStart) + kStep + kStart - 1) / (kStep + kStart), fit = a.shares / p.pairs;
+        a.ranges = (uint32_t)(fit < 1 ? 1 : fit < most ? fit : most);
+        a.by_ranges = fast_div(a.ranges);
+        const int64_t pieces = a.ranges * p.pairs;
+        p.workgroups = pieces < 2048 ? (pieces + kDealt - 1) / kDealt * kDealt : 2048;
+    }
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (p.dp == 64) launch_attention<64>(a, bits, fp16, ad, (unsigned)p.workgroups, s);
     else if (p.dp == 128) launch_attention<128>(a, bits, fp16, ad, (unsigned)p.workgroups, s);

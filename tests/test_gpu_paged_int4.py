@@ -6,7 +6,10 @@ itself may be small:
   exponent   (D + 12) 2^-24 times scale_value * max_j |ks_j| (31 + |ko_j - 24|) * sum_d |q_d|, and 2^-20 for the exponential and the sums
              of probabilities
   output     u |o| for its one rounding; with S = sum_j p_j |vs_j| (31 + |vo_j - 24|): twice the exponent's error, 2^-16 for the two bf16
-             terms that a probability times a scale is rounded to, and 2^-18 for float32 sums (of at most 300 terms a lane here), of S
+             terms that a probability times a scale is rounded to, and 2^-18 for float32 sums (of at most 300 terms a lane here), of S.
+             bfloat16 outputs may come from one bf16 term r_j = p_j vs_j (1 + e_j), |e_j| <= 2^-8: with the sum of these very r_j the images'
+             24 is taken off again, so sum_j r_j (c_j + 24) - 24 sum_j r_j + sum_j p_j vs_j o_j is off by sum_j p_j vs_j e_j c_j, and
+             |c_j| <= 8: by 2^-5 of sum_j p_j |vs_j|
   lse        the exponent's error alone;  attn_sums: twice it, and one float32 addition
 Codes, scales, offsets, values read back and moved rows are exact.
 """
@@ -76,14 +79,17 @@ def check_attention(got, cache, q, table, lens, scale=None, mask=None, sums=None
     span = lambda s, o: torch.where(bad, 0.0, s.double().abs() * (31 + (o.double() - 24).abs()))  # noqa: E731
     err = (dim + 12) * 2.0 ** -24 * abs(scale) * span(cache.ks, cache.ko).max() * q.double().abs().sum(-1) + 2.0 ** -20            # [B, H]
     page = k.shape[1]
-    S = torch.zeros_like(lse)
+    S, one_term = torch.zeros_like(lse), torch.zeros_like(lse)
     for b in range(q.shape[0]):
         n = weights.shape[-1]
         ids, at = table[b].long()[torch.arange(n) // page], torch.arange(n) % page
         there = (ids >= 0) & (ids < k.shape[0])
         wide = torch.where(there[:, None], span(cache.vs, cache.vo)[ids.clamp(0, k.shape[0] - 1), at], 0.0)                         # [n, kv]
         S[b] = (weights[b] * wide.t().repeat_interleave(heads // kv, 0)).sum(-1)
-    bound = U[dt] * out.abs() + ((2 * err + 2.0 ** -16 + 2.0 ** -18) * S * (1 + U[dt]))[..., None] + 2.0 ** -24
+        if dt == torch.bfloat16:
+            scales = torch.where(there[:, None], cache.vs.double().abs().nan_to_num(0.0)[ids.clamp(0, k.shape[0] - 1), at], 0.0)
+            one_term[b] = 2.0 ** -5 * (weights[b] * scales.t().repeat_interleave(heads // kv, 0)).sum(-1)
+    bound = U[dt] * out.abs() + (((2 * err + 2.0 ** -16 + 2.0 ** -18) * S + one_term) * (1 + U[dt]))[..., None] + 2.0 ** -24
     diff = (got[0].cpu().double() - out).abs()
     assert got[0].dtype == dt and bool((diff <= bound).all()), f"output off by {(diff / bound).max():.3g} bounds"
     empty = lse == -math.inf
