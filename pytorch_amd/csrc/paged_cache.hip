@@ -83,40 +83,48 @@ struct RowQuant {
 // one the correctly rounded quotient, where nothing leaves the normal range: for hi - lo in [2^-60, 2^60] only quotients below 2^-40
 // do, which round to 0 either way.  The sum with 1.5 * 2^23 rounds, ties to even; its low bits are the number, 0 to 15.
 struct RowQuant4 {
-    float lo, span, scale, offset, r;
-    bool flat, fast, finite;
+    float lo, span;
+    bool flat, finite, fast;
     __device__ RowQuant4(float lo_, float hi) : lo(lo_), span(hi - lo_)
     {
         flat = span <= 0x1p-120f;
         finite = span <= 0x1p124f;                           // 15 times it is a number (false for NaN)
-        scale = flat ? 1.0f : finite ? span / 15.0f : NAN;
-        offset = flat ? lo : lo / scale + 8.0f;
-        r = 1.0f / span;
         fast = span >= 0x1p-60f && span <= 0x1p60f;
     }
-    // the code plus 8
-    __device__ __forceinline__ uint32_t operator()(float x) const
+    // span / 15: for every significand the product with 1 / 15, corrected once, is the correctly rounded quotient (checked exhaustively)
+    __device__ __forceinline__ float scale() const
     {
-        const float t = (x - lo) * 15.0f;
+        const float c = 1.0f / 15.0f, q = span * c;
+        return flat ? 1.0f : finite ? __builtin_fmaf(__builtin_fmaf(-15.0f, q, span), c, q) : NAN;
+    }
+    // `quotient` = lo / scale()
+    __device__ __forceinline__ float offset(float quotient) const { return flat ? lo : quotient + 8.0f; }
+    // codes of eight elements in a word; r = 1 / span
+    template <bool FP16>
+    __device__ __forceinline__ uint32_t word(u32x4 v, float r) const
+    {
+        uint32_t w = 0;
         if (fast) {
-            float q = t * r;
-            q = __builtin_fmaf(__builtin_fmaf(-span, q, t), r, q);
-            q = __builtin_fmaf(__builtin_fmaf(-span, q, t), r, q);
-            return __float_as_uint(q + 12582912.0f) & 15u;
+            constexpr uint32_t kOne = 0x4b400000u;           // 1.5 * 2^23, which eight shifted sums leave in the word three times
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float t = ((i % 2 ? act_hi<FP16>(v[i / 2]) : act_lo<FP16>(v[i / 2])) - lo) * 15.0f;
+                float q = t * r;
+                q = __builtin_fmaf(__builtin_fmaf(-span, q, t), r, q);
+                q = __builtin_fmaf(__builtin_fmaf(-span, q, t), r, q);
+                w += __float_as_uint(q + 12582912.0f) << (4 * i);
+            }
+            w -= kOne + (kOne << 4) + (kOne << 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float t = ((i % 2 ? act_hi<FP16>(v[i / 2]) : act_lo<FP16>(v[i / 2])) - lo) * 15.0f;
+                w |= (flat ? 8u : finite ? (uint32_t)(int)__builtin_rintf(t / span) & 15u : 0u) << (4 * i);
+            }
         }
-        if (flat) return 8;
-        return finite ? (uint32_t)(int)__builtin_rintf(t / span) & 15u : 0;
+        return w ^ 0x88888888u;                              // u - 8 in two's complement
     }
 };
-// codes of eight elements in a word
-template <bool FP16>
-__device__ __forceinline__ uint32_t quant_word(const RowQuant4 &q, u32x4 v)
-{
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) w |= q(act_lo<FP16>(v[i])) << (8 * i) | q(act_hi<FP16>(v[i])) << (8 * i + 4);
-    return w ^ 0x88888888u;                                  // u - 8 in two's complement
-}
 // 16-bit values as integers in their order (and back: its own inverse); NaN lies beyond the infinities
 __device__ __forceinline__ uint32_t order16(uint32_t two)
 {
@@ -141,6 +149,23 @@ template <bool FP16>
 __device__ __forceinline__ RowQuant4 quant_of(uint32_t range)
 {
     return RowQuant4(act_1<FP16>((uint16_t)order16(~range >> 16)), act_1<FP16>((uint16_t)order16(range & 0xffffu)));
+}
+// the lane of another place among the four, eight, 16 (32) neighbours
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_of_four(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+// range over GL lanes, in all of them: neighbours, pairs, mirrored fours, mirrored eights, rows of 16
+template <int GL>
+__device__ __forceinline__ uint32_t over_row(uint32_t v)
+{
+    v = max16(v, lane_of_four<0xb1>(v));
+    v = max16(v, lane_of_four<0x4e>(v));
+    v = max16(v, lane_of_four<0x141>(v));
+    if constexpr (GL >= 16) v = max16(v, lane_of_four<0x140>(v));
+    if constexpr (GL >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max16(r[0], r[1]);
+    }
+    return v;
 }
 __device__ __forceinline__ float nibble_f32(uint32_t w, int i) { return (float)((int32_t)(w << (28 - 4 * i)) >> 28); }
 
@@ -167,21 +192,31 @@ __global__ __launch_bounds__(256) void paged_write_kernel(RowArgs a)
     char *scale = BITS < 16 ? sc.base + a.cache.offset(sc, (uint32_t)slot, (int)(part * N)) : nullptr;
     const PagedArray &of = plane ? a.cache.value_offset : a.cache.key_offset;
     char *offset = BITS == 4 ? of.base + a.cache.offset(of, (uint32_t)slot, (int)(part * N)) : nullptr;
+    if constexpr (BITS == 4) {
+        // Lanes 0 and 1 (of four) divide 1 by the rows' spans, lanes 2 and 3 their least values by their scales: one division, an exact
+        // one is eleven instructions, for up to four.
+        static_assert(N <= 2, "a lane for each quotient");
+        uint32_t range[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) range[i] = over_row<GL>(mine ? range8(v[i]) : kNoRange);
+        const RowQuant4 first = quant_of<FP16>(range[0]), second = quant_of<FP16>(range[N - 1]), &own = lane & 1 ? second : first;
+        const float own_scale = own.scale(), quotient = (lane & 2 ? own.lo : 1.0f) / (lane & 2 ? own_scale : own.span);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float r = __uint_as_float(i ? lane_of_four<0x55>(__float_as_uint(quotient)) : lane_of_four<0x00>(__float_as_uint(quotient)));
+            const uint32_t word = (i ? second : first).template word<FP16>(v[i], r);
+            if (mine) *reinterpret_cast<uint32_t *>(dst + i * to.head) = word;
+        }
+        if (lane >= 2 && lane < 2 + N) {
+            *reinterpret_cast<float *>(scale + (lane - 2) * sc.head) = own_scale;
+            *reinterpret_cast<float *>(offset + (lane - 2) * of.head) = own.offset(quotient);
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < N; i++) {
         if constexpr (BITS == 16) {
             if (mine) *reinterpret_cast<u32x4 *>(dst + i * to.head) = v[i];
-        } else if constexpr (BITS == 4) {
-            uint32_t range = mine ? range8(v[i]) : kNoRange;
-#pragma unroll
-            for (int off = GL / 2; off >= 1; off >>= 1) range = max16(range, (uint32_t)__shfl_xor((int)range, off, GL));
-            const RowQuant4 q = quant_of<FP16>(range);
-            const uint32_t word = quant_word<FP16>(q, v[i]);
-            if (mine) *reinterpret_cast<uint32_t *>(dst + i * to.head) = word;
-            if (lane == 0) {
-                *reinterpret_cast<float *>(scale + i * sc.head) = q.scale;
-                *reinterpret_cast<float *>(offset + i * of.head) = q.offset;
-            }
         } else {
             uint32_t m = absmax8(v[i]);
 #pragma unroll
@@ -221,16 +256,17 @@ __global__ __launch_bounds__(256) void paged_write_any_kernel(RowArgs a, int fp1
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) range = max16(range, (uint32_t)__shfl_xor((int)range, off, 64));
         const RowQuant4 q = fp16 ? quant_of<true>(range) : quant_of<false>(range);
+        const float r = 1.0f / q.span, scale = q.scale();
         for (int w = lane; w < a.cache.dim / 8; w += 64) {
             u32x4 v;
 #pragma unroll
             for (int i = 0; i < 4; i++) v[i] = x[8 * w + 2 * i] | (uint32_t)x[8 * w + 2 * i + 1] << 16;
-            reinterpret_cast<uint32_t *>(dst)[w] = fp16 ? quant_word<true>(q, v) : quant_word<false>(q, v);
+            reinterpret_cast<uint32_t *>(dst)[w] = fp16 ? q.word<true>(v, r) : q.word<false>(v, r);
         }
         if (lane == 0) {
             const PagedArray &s = plane ? a.cache.value_scale : a.cache.key_scale, &o = plane ? a.cache.value_offset : a.cache.key_offset;
-            *reinterpret_cast<float *>(s.base + a.cache.offset(s, (uint32_t)slot, (int)h)) = q.scale;
-            *reinterpret_cast<float *>(o.base + a.cache.offset(o, (uint32_t)slot, (int)h)) = q.offset;
+            *reinterpret_cast<float *>(s.base + a.cache.offset(s, (uint32_t)slot, (int)h)) = scale;
+            *reinterpret_cast<float *>(o.base + a.cache.offset(o, (uint32_t)slot, (int)h)) = q.offset(q.lo / scale);
         }
     } else {
         uint32_t m = 0;
@@ -360,10 +396,12 @@ template <bool WRITE, int GL>
 void launch_rows(RowArgs &a, int bits, bool fp16, hipStream_t s)
 {
     // One row per group of lanes while that leaves the card short of workgroups.  Beyond: 8192 tokens to int8, 8 heads of 128,
-    // 14.3 us with one row per group, 13.2 with two, 13.9 with four; 32768 tokens from int8 33.6, 31.3 and 31.2.
+    // 14.3 us with one row per group, 13.2 with two, 13.9 with four; 32768 tokens from int8 33.6, 31.3 and 31.2.  8192 tokens to int4
+    // (43 MB) 15.6 us with one row, 14.5 with two; from int4 8.6 with four.
     const bool many = (int64_t)a.tokens * a.cache.heads * 2 / (256 / GL) >= kNumCU * 16;
-    if (many && !WRITE && a.cache.heads % 4 == 0) launch_rows<WRITE, GL, 4>(a, bits, fp16, s);
-    else if (many && a.cache.heads % 2 == 0) launch_rows<WRITE, GL, 2>(a, bits, fp16, s);
+    if constexpr (!WRITE)
+        if (many && a.cache.heads % 4 == 0) return launch_rows<WRITE, GL, 4>(a, bits, fp16, s);
+    if (many && a.cache.heads % 2 == 0) launch_rows<WRITE, GL, 2>(a, bits, fp16, s);
     else launch_rows<WRITE, GL, 1>(a, bits, fp16, s);
 }
 
