@@ -1,9 +1,11 @@
 """The attention block of a W8A8 decoder over a paged, budgeted key-value cache, one token per sequence and step.
 
-    python examples/decode_paged_cache.py --batch 16 --budget 1024 --steps 64 [--int8-cache] [--graph]
+    python examples/decode_paged_cache.py --batch 16 --budget 1024 --steps 64 [--int8-cache | --int4-cache] [--layer] [--graph]
 
 Random weights and prompts.  Per step: npu_dynamic_quant, npu_quant_matmul (qkv), PagedKVCache.append, attend and evict,
-npu_dynamic_quant, npu_quant_matmul (output).  With --graph the steps are replays of one captured step.
+npu_dynamic_quant, npu_quant_matmul (output).  With --layer the step also has a decoder layer's norms and positions:
+npu_add_rms_norm_dynamic_quant in place of the first npu_dynamic_quant, PagedKVCache.rotate before append, and npu_add_rms_norm,
+which adds the residual, at the end.  With --graph the steps are replays of one captured step.
 """
 import argparse
 import os
@@ -25,14 +27,17 @@ def linear(features_in, features_out, generator):
 
 
 def project(layer, x):
-    codes, scale = pa.npu_dynamic_quant(x)
+    return project_codes(layer, *pa.npu_dynamic_quant(x))
+
+
+def project_codes(layer, codes, scale):
     return pa.npu_quant_matmul(codes, layer[0], layer[1], pertoken_scale=scale, output_dtype=torch.bfloat16)
 
 
 class DecodeAttention:
     def __init__(self, hidden, heads, cache, generator):
         self.heads, self.cache = heads, cache
-        self.kv_heads, self.head_dim = cache.key_cache.shape[2:]
+        self.kv_heads, self.head_dim = cache.key_cache.shape[2], hidden // heads
         self.qkv = linear(hidden, (heads + 2 * self.kv_heads) * self.head_dim, generator)
         self.o = linear(heads * self.head_dim, hidden, generator)
 
@@ -53,17 +58,49 @@ class DecodeAttention:
         return x + project(self.o, out.flatten(1))
 
 
+class DecodeLayer(DecodeAttention):
+    """With the norms on both sides and rotary positions; a step returns what the MLP reads."""
+
+    def __init__(self, hidden, heads, cache, generator, positions):
+        super().__init__(hidden, heads, cache, generator)
+        self.gamma = [(1 + 0.1 * torch.randn(hidden, generator=generator)).to(torch.bfloat16).cuda() for _ in range(2)]
+        angles = torch.arange(float(positions))[:, None] * 10000.0 ** (-torch.arange(0, self.head_dim, 2) / self.head_dim)
+        self.cos_sin = torch.cat((angles.cos(), angles.sin()), 1).cuda()
+
+    def split(self, x):
+        codes, scale, _ = pa.npu_add_rms_norm_dynamic_quant(x, None, self.gamma[0])
+        qkv = project_codes(self.qkv, codes, scale).view(x.shape[0], self.heads + 2 * self.kv_heads, self.head_dim)
+        return qkv.split((self.heads, self.kv_heads, self.kv_heads), 1)
+
+    def prefill(self, sequence, x):
+        q, k, v = self.split(x)
+        _, k = pa.npu_mrope(torch.arange(x.shape[0], device=x.device), q, k, self.cos_sin, self.head_dim)
+        self.cache.prefill(sequence, k, v)
+
+    def step(self, x):
+        q, k, v = self.split(x)
+        q, k = self.cache.rotate(q, k, self.cos_sin)
+        self.cache.append(k, v)
+        out = self.cache.attend(q)
+        self.cache.evict()
+        return pa.npu_add_rms_norm(x, project(self.o, out.flatten(1)), self.gamma[1])[0]
+
+
 def main(argv=None):
     p = argparse.ArgumentParser()
     for name, value in (("batch", 16), ("hidden", 4096), ("heads", 32), ("kv-heads", 8), ("budget", 1024), ("prompt", 1000), ("steps", 64)):
         p.add_argument("--" + name, type=int, default=value)
-    p.add_argument("--int8-cache", action="store_true")
+    codes = p.add_mutually_exclusive_group()
+    codes.add_argument("--int8-cache", action="store_true")
+    codes.add_argument("--int4-cache", action="store_true")
+    p.add_argument("--layer", action="store_true")
     p.add_argument("--graph", action="store_true")
     a = p.parse_args(argv)
     g = torch.Generator().manual_seed(0)
     room = max(a.prompt, a.budget) + 1
-    cache = PagedKVCache(a.batch, room, a.kv_heads, a.hidden // a.heads, budget=a.budget, quantized=a.int8_cache, device="cuda")
-    block = DecodeAttention(a.hidden, a.heads, cache, g)
+    cache = PagedKVCache(a.batch, room, a.kv_heads, a.hidden // a.heads, budget=a.budget, quantized=a.int8_cache or a.int4_cache, bits=4 if a.int4_cache else 8,
+                         device="cuda")
+    block = DecodeLayer(a.hidden, a.heads, cache, g, a.prompt + a.steps + 2) if a.layer else DecodeAttention(a.hidden, a.heads, cache, g)
     for b in range(a.batch):
         block.prefill(b, torch.randn(a.prompt - b % 2, a.hidden, generator=g).to(torch.bfloat16).cuda())
     x = torch.randn(a.batch, a.hidden, generator=g).to(torch.bfloat16).cuda()
@@ -82,7 +119,7 @@ def main(argv=None):
     y = y if a.graph else out
     ms = (time.perf_counter() - start) / a.steps * 1e3
     print(f"{a.batch} sequences, {int(cache.context_lens.max())} of {cache.capacity} tokens held, {ms:.3f} ms per step, "
-          f"{a.batch / ms * 1e3:.0f} tokens/s of one attention block")
+          f"{a.batch / ms * 1e3:.0f} tokens/s of one {'layer without its MLP' if a.layer else 'attention block'}")
     return y, cache
 
 

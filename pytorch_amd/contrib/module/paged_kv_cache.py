@@ -20,15 +20,16 @@ __all__ = ["PagedKVCache"]
 
 class PagedKVCache:
     """``max_tokens``: what a sequence can hold at once.  ``quantized``: codes in place of ``dtype``, of ``bits`` 8 (int8, a float32
-    scale per token and head) or 4 (eight in an int32 word, a scale and an offset; head_dim a multiple of 8).  ``budget``: the tokens that ``evict`` leaves, each key/value head choosing its own by the attention
-    they got from ``attend``; the newest ``recent`` (default: a quarter) always stay.  The cache needs room for at least one token
-    beyond it.  Tokens of a prompt have got none before the first ``attend``: an ``evict`` before it keeps the recent tokens and
-    the first ones.
+    scale per token and head) or 4 (eight in an int32 word, a scale and an offset; head_dim a multiple of 8).  ``budget``: the tokens
+    that ``evict`` leaves, each key/value head choosing its own by the attention they got from ``attend``; the newest ``recent``
+    (default: a quarter) always stay.  The cache needs room for at least one token beyond it.  Tokens of a prompt have got none before
+    the first ``attend``: an ``evict`` before it keeps the recent tokens and the first ones.
 
-    Tensors on ``device``: ``key_cache``, ``value_cache`` [blocks, block_size, kv_heads, head_dim] (4 bits: head_dim / 8; ``key_scale``,
-    ``value_scale``, ``key_offset``, ``value_offset`` without the last dimension), stored so that the tokens of one head of a block follow each other; ``block_table`` [batch, blocks per
-    sequence], which an allocator of blocks may rewrite; ``context_lens`` [batch]; with a budget ``attn_sums`` and
-    ``positions`` [batch, kv_heads, capacity] and ``next_position`` [batch].
+    Tensors on ``device``: ``key_cache``, ``value_cache`` [blocks, block_size, kv_heads, head_dim] (4 bits: head_dim / 8) and, with
+    codes, ``key_scale`` and ``value_scale``, with 4 bits also ``key_offset`` and ``value_offset``, without the last dimension; all
+    stored so that the tokens of one head of a block follow each other; ``block_table`` [batch, blocks per sequence], which an
+    allocator of blocks may rewrite; ``context_lens`` [batch]; with a budget ``attn_sums`` and ``positions``
+    [batch, kv_heads, capacity] and ``next_position`` [batch].
 
     A call that would overfill a sequence raises, as far as the host knows the lengths: replays of a captured step pass it by.
     What does not fit then is not written and gets no position, and a length stays at the capacity.  ``append`` takes a token for
