@@ -6,10 +6,11 @@
 // and one rounding to 16 bits.  The other D - R elements are copied.  Cosines and sines come from a table [positions][R], the
 // cosines first.  A position outside the table counts as cos = sin = 0.
 //
-// Bound by memory: every element is read and written once.  A thread takes eight frequencies (two pieces of 16 bytes) of several
-// heads of a token, which share its cosines and sines; neighbouring threads take neighbouring pieces, then neighbouring heads.
-// 32767 tokens on three axes, 32 + 8 heads of 128, 689 MB: 124 us, 5.6 TB/s; 64 tokens, bound by the launch and a trip to memory
-// for the positions, one for the table and one for the heads: 3.1 to 3.6 us.
+// Bound by memory: every element is read and written once.  A thread takes eight frequencies (two pieces of 16 bytes) of one head
+// of a token; neighbouring threads take neighbouring pieces, then neighbouring heads.  The heads of a token share its cosines and sines,
+// which the caches hand out: with two or four heads a thread the table is read less, and 32767 tokens on three axes, 32 + 8 heads of
+// 128, 689 MB, take 115 or 124 us, not 110 (6.2 TB/s), 64 tokens 3.8 or 5.1, not 3.0 (the launch and a trip to memory for the
+// positions, one for the table and one for the heads).
 #include "paged_cache.h"
 #include "weight_quant_common.h"
 
@@ -30,8 +31,8 @@ struct RopeArgs {
     int pos64, axes, end[kAxes];       // frequencies of the axes up to and with this one
     int dim, half;                     // half = R / 2
     int interleaved;
-    uint32_t tokens, units;            // units = tokens * groups * pieces
-    FastDiv pieces, groups;            // pieces of a head; threads that share the heads of a token
+    uint32_t tokens, units;            // units = tokens * rows * pieces
+    FastDiv pieces, rows;              // pieces of a head; heads of a token, queries first
 };
 
 __device__ __forceinline__ int64_t position(const RopeArgs &a, uint32_t token, int axis)
@@ -100,35 +101,24 @@ __device__ __forceinline__ void turn8(u32x4 &x, u32x4 &y, const float (&c)[8], c
     }
 }
 
-// N heads at most per thread, `groups` threads side by side for those of a token.  SPLIT: an axis may end inside eight
-// frequencies.  Rows on 16-byte boundaries, half a multiple of 8 and dim of 16.
-template <int N, bool FP16, int TABLE, bool INTERLEAVED, bool SPLIT>
+// SPLIT: an axis may end inside eight frequencies.  Rows on 16-byte boundaries, half a multiple of 8 and dim of 16.  The results are
+// not kept in the caches (32767 tokens: 110 us, 117 kept); what is read may be there, from the projection (4096 tokens: 14.2 us, 17.5 past the caches).
+template <bool FP16, int TABLE, bool INTERLEAVED, bool SPLIT>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a)
 {
     const uint32_t unit = blockIdx.x * 256 + threadIdx.x;
     if (unit >= a.units) return;
     const uint32_t rest = div_by(unit, a.pieces), piece = unit - rest * a.pieces.d;
-    const uint32_t token = div_by(rest, a.groups), first = rest - token * a.groups.d;
-    const int turned = a.half / 8, f = (int)piece * 8, heads = a.heads[0] + a.heads[1];
+    const uint32_t token = div_by(rest, a.rows), row = rest - token * a.rows.d;
+    const int turned = a.half / 8, f = (int)piece * 8, which = (int)row >= a.heads[0], head = (int)row - (which ? a.heads[0] : 0);
     const bool copied = (int)piece >= turned;
     // first elements of the two pieces of 8
     const int e0 = copied || INTERLEAVED ? (int)piece * 16 : f, e1 = copied || INTERLEAVED ? e0 + 8 : a.half + f;
 
-    u32x4 x[N], y[N];
-    const auto row_in = [&](int head) {
-        const int which = head >= a.heads[0];
-        return a.in[which] + token * a.tok[which] + (head - (which ? a.heads[0] : 0)) * a.head[which];
-    };
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int head = (int)(first + i * a.groups.d);
-        if (head >= heads) continue;
-        const uint16_t *row = row_in(head);
-        x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + e0));
-        y[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + e1));
-    }
-    float c[8], s[8];
+    const uint16_t *from = a.in[which] + token * a.tok[which] + head * a.head[which];
+    u32x4 x = *reinterpret_cast<const u32x4 *>(from + e0), y = *reinterpret_cast<const u32x4 *>(from + e1);
     if (!copied) {
+        float c[8], s[8];
         if constexpr (SPLIT) {
 #pragma unroll
             for (int i = 0; i < 8; i++) turn_of<TABLE>(a, token, f + i, c[i], s[i]);
@@ -142,20 +132,14 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a)
                 for (int i = 0; i < 8; i++) c[i] = s[i] = 0.0f;
             }
         }
+        turn8<FP16, INTERLEAVED>(x, y, c, s);
     }
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int head = (int)(first + i * a.groups.d);
-        if (head >= heads) continue;
-        if (!copied) turn8<FP16, INTERLEAVED>(x[i], y[i], c, s);
-        const int which = head >= a.heads[0];
-        uint16_t *row = a.out[which] + ((int64_t)token * a.heads[which] + (head - (which ? a.heads[0] : 0))) * a.dim;
-        __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4 *>(row + e0));
-        __builtin_nontemporal_store(y[i], reinterpret_cast<u32x4 *>(row + e1));
-    }
+    uint16_t *to = a.out[which] + ((int64_t)token * a.heads[which] + head) * a.dim;
+    __builtin_nontemporal_store(x, reinterpret_cast<u32x4 *>(to + e0));
+    __builtin_nontemporal_store(y, reinterpret_cast<u32x4 *>(to + e1));
 }
 
-// Any width, alignment and strides: a thread per pair or copied element.  pieces = half + (dim - R), groups = heads.
+// Any width, alignment and strides: a thread per pair or copied element.  pieces = half + (dim - R).
 template <int TABLE>
 __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int fp16)
 {
@@ -163,8 +147,8 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int fp16)
     if (unit >= a.units) return;
     const uint32_t rest = div_by(unit, a.pieces);
     const int piece = (int)(unit - rest * a.pieces.d);
-    const uint32_t token = div_by(rest, a.groups);
-    int head = (int)(rest - token * a.groups.d);
+    const uint32_t token = div_by(rest, a.rows);
+    int head = (int)(rest - token * a.rows.d);
     const int which = head >= a.heads[0];
     head -= which ? a.heads[0] : 0;
     const uint16_t *row = a.in[which] + token * a.tok[which] + head * a.head[which];
@@ -183,28 +167,27 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int fp16)
     out[e1] = (uint16_t)(w >> 16);
 }
 
-template <int N, bool FP16, int TABLE>
+template <bool FP16, int TABLE>
 void launch_rope(const RopeArgs &a, bool split, unsigned blocks, hipStream_t s)
 {
     const dim3 grid(blocks), block(256);
     if (a.interleaved) {
-        if (split) hipLaunchKernelGGL((rope_kernel<N, FP16, TABLE, true, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((rope_kernel<N, FP16, TABLE, true, false>), grid, block, 0, s, a);
+        if (split) hipLaunchKernelGGL((rope_kernel<FP16, TABLE, true, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((rope_kernel<FP16, TABLE, true, false>), grid, block, 0, s, a);
     } else {
-        if (split) hipLaunchKernelGGL((rope_kernel<N, FP16, TABLE, false, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((rope_kernel<N, FP16, TABLE, false, false>), grid, block, 0, s, a);
+        if (split) hipLaunchKernelGGL((rope_kernel<FP16, TABLE, false, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((rope_kernel<FP16, TABLE, false, false>), grid, block, 0, s, a);
     }
 }
-template <int N>
 void launch_rope(const RopeArgs &a, bool fp16, int table, bool split, unsigned blocks, hipStream_t s)
 {
     if (table == MI355_DTYPE_FP32) {
-        if (fp16) launch_rope<N, true, 2>(a, split, blocks, s);
-        else launch_rope<N, false, 2>(a, split, blocks, s);
+        if (fp16) launch_rope<true, 2>(a, split, blocks, s);
+        else launch_rope<false, 2>(a, split, blocks, s);
     } else if (fp16) {
-        launch_rope<N, true, 1>(a, split, blocks, s);
+        launch_rope<true, 1>(a, split, blocks, s);
     } else {
-        launch_rope<N, false, 0>(a, split, blocks, s);
+        launch_rope<false, 0>(a, split, blocks, s);
     }
 }
 
@@ -271,23 +254,20 @@ extern "C" int mi355_mrope(const void *positions, int positions_dtype, int64_t p
     a.interleaved = interleaved != 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t all = heads + kv_heads, pieces = vec ? head_dim / 16 : a.half + (head_dim - rotary_dim);
-    const bool many = all * pieces * tokens >= (int64_t)kNumCU * 8 * 256;
-    const int64_t per_thread = !vec ? 1 : many ? 4 : 1, groups = (all + per_thread - 1) / per_thread;
     a.pieces = fast_div((uint32_t)pieces);
-    a.groups = fast_div((uint32_t)groups);
-    const int64_t most = kUnitsPerLaunch / (groups * pieces) > 0 ? kUnitsPerLaunch / (groups * pieces) : 1;
-    if (groups * pieces > 0x7fffff00) return MI355_ERR_UNSUPPORTED;
+    a.rows = fast_div((uint32_t)all);
+    const int64_t most = kUnitsPerLaunch / (all * pieces) > 0 ? kUnitsPerLaunch / (all * pieces) : 1;
+    if (all * pieces > 0x7fffff00) return MI355_ERR_UNSUPPORTED;
     for (int64_t t0 = 0; t0 < tokens; t0 += most) {
         a.tokens = (uint32_t)(tokens - t0 < most ? tokens - t0 : most);
-        a.units = (uint32_t)(a.tokens * groups * pieces);
+        a.units = (uint32_t)(a.tokens * all * pieces);
         a.pos = static_cast<const char *>(positions) + t0 * positions_stride_token * pos_bytes;
         for (int i = 0; i < 2; i++) {
             a.in[i] = static_cast<const uint16_t *>(in[i]) + t0 * a.tok[i];
             a.out[i] = static_cast<uint16_t *>(out[i]) + t0 * a.heads[i] * head_dim;
         }
         const unsigned blocks = (a.units + 255) / 256;
-        if (vec && many) launch_rope<4>(a, fp16, cos_sin_dtype, split, blocks, s);
-        else if (vec) launch_rope<1>(a, fp16, cos_sin_dtype, split, blocks, s);
+        if (vec) launch_rope(a, fp16, cos_sin_dtype, split, blocks, s);
         else if (cos_sin_dtype == MI355_DTYPE_FP32) hipLaunchKernelGGL(rope_any_kernel<2>, dim3(blocks), dim3(256), 0, s, a, fp16);
         else if (fp16) hipLaunchKernelGGL(rope_any_kernel<1>, dim3(blocks), dim3(256), 0, s, a, 1);
         else hipLaunchKernelGGL(rope_any_kernel<0>, dim3(blocks), dim3(256), 0, s, a, 0);
