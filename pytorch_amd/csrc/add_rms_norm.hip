@@ -10,8 +10,8 @@
 //
 // One row per workgroup (or per wavefront, where rows are short), held in registers from its only load to its only store.
 //
-// Bound by memory where rows are many: 8191 rows of 8192 to int8, 470 MB, in 82 us, 5.7 TB/s; 2047 of 5128 in 16 bits, 84 MB, in 16.5 us,
-// 5.1 TB/s.  Few rows are bound by the launch and one trip to memory and back: one row of 4096 to int8 in 3.1 us, 64 of 8192 in 3.9.
+// Bound by memory where rows are many: 8191 rows of 8192 to int8, 470 MB, in 80 us, 5.9 TB/s; 2047 of 5128 in 16 bits, 84 MB, in 15.0 us,
+// 5.6 TB/s.  Few rows are bound by the launch and one trip to memory and back: one row of 4096 to int8 in 2.9 us, 64 of 8192 in 3.8.
 #include "common.h"
 #include "weight_quant_common.h"
 
@@ -26,15 +26,18 @@ struct NormArgs {
     uint16_t *sum;                           // [rows, cols], with x2
     int64_t rows, x1_stride, x2_stride;
     int cols, gamma32;
+    int once;                                // the inputs are more than the caches hold
     float epsilon;
 };
 
-// Eight consecutive elements, of which n (1 to 8) exist; ANY: from any address, else 16-byte aligned and whole.
-template <bool ANY>
+// Eight consecutive elements, of which n (1 to 8) exist; ANY: from any address, else 16-byte aligned and whole, ONCE: past the caches.
+template <bool ANY, bool ONCE = false>
 __device__ __forceinline__ u32x4 load8(const uint16_t *p, int n)
 {
-    if constexpr (!ANY) {
+    if constexpr (!ANY && ONCE) {
         return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+    } else if constexpr (!ANY) {
+        return *reinterpret_cast<const u32x4 *>(p);
     } else {
         typedef u32x4 anywhere __attribute__((aligned(2)));
         if (n >= 8) return *reinterpret_cast<const anywhere *>(p);
@@ -204,15 +207,19 @@ __global__ __launch_bounds__(BLOCK) void norm_rows_kernel(NormArgs a)
     const uint16_t *x1 = a.x1 + row * a.x1_stride, *x2 = a.x2 + row * a.x2_stride;
 
     u32x4 v1[VPT], v2[VPT];
+    const auto load = [&](auto eight) {
 #pragma unroll
-    for (int i = 0; i < VPT; i++) {
-        const int col = (t + i * TPR) * 8;
-        v1[i] = v2[i] = u32x4{0, 0, 0, 0};
-        if (col < a.cols) {
-            v1[i] = load8<ANY>(x1 + col, a.cols - col);
-            if (a.x2) v2[i] = load8<ANY>(x2 + col, a.cols - col);
+        for (int i = 0; i < VPT; i++) {
+            const int col = (t + i * TPR) * 8;
+            v1[i] = v2[i] = u32x4{0, 0, 0, 0};
+            if (col < a.cols) {
+                v1[i] = eight(x1 + col, a.cols - col);
+                if (a.x2) v2[i] = eight(x2 + col, a.cols - col);
+            }
         }
-    }
+    };
+    if (!ANY && a.once) load([](const uint16_t *p, int n) { return load8<ANY, true>(p, n); });
+    else load([](const uint16_t *p, int n) { return load8<ANY>(p, n); });
     float s[VPT][8], g[VPT][8], sum = 0.0f;
     uint32_t top = 0;
 #pragma unroll
@@ -345,6 +352,10 @@ int add_rms_norm(const void *x1, const void *x2, int dtype, const void *gamma, i
     a.epsilon = epsilon;
     const bool any = cols % 8 || x1_stride % 8 || a.x2_stride % 8 || !aligned(x1, 16) || !aligned(x2, 16) || !aligned(x, 16) || !aligned(gamma, 16) ||
                      !aligned(y, INT8 ? 8 : 16);
+    // Inputs that fit into the Infinity Cache may still be there, from the operators that wrote them (2047 rows of 5128: 15.0 us, 17.0 past
+    // the caches; 8192 of 2048, 67 MB: 22.4 and 25); larger ones only drive each other out (8192 of 4096, 134 MB: 50 us, 48 past the
+    // caches; 8191 of 8192 to int8 85 and 82; all of them 2 to 4 us less since the loads of a row stand together).
+    a.once = rows * cols * (x2 ? 4 : 2) > (int64_t)96 << 20;
     for (int64_t r0 = 0; r0 < rows; r0 += kRowsPerLaunch) {
         a.rows = rows - r0 < kRowsPerLaunch ? rows - r0 : kRowsPerLaunch;
         a.x1 = static_cast<const uint16_t *>(x1) + r0 * x1_stride;
