@@ -62,12 +62,13 @@ constexpr int kSC1 = 16;                     // cache-policy bit: agent scope, p
 // 4095, 280 MB: 62 us for 768 pieces, 66 for 512, 64 for 1024, 68 for 1536).  Heads of up to 64 take 103 to 124 registers, of
 // which four would fit; they are cut for three like the others.
 constexpr int resident(int dp, bool quant) { return dp < 256 ? 3 : quant ? 2 : 1; }
-// int4, Decode4: halves of a step of a workgroup; its workgroups of a compute unit (135 to 138 registers for heads of 65 to 128, 207 and 211 for
-// wider ones); and what the start and the end of a sequence cost, in halves (32 sequences of up to 4095, 78 MB: 25.7 us with 24, 26.2 with 16 or
-// 30, 27.8 with 8, 26.7 with 40, 30.0 with 64; 64 of up to 8192, 308 MB: 60.4 to 61.3, with 8 and 64 63)
+// int4, Decode4: halves of a step of a workgroup; its workgroups of a compute unit (135 to 138 registers for heads of 65 to 128, 205 to 211 for
+// wider ones); what the start and the end of a range cost, in halves (dense, 32 sequences of up to 4095, 78 MB: 25.7 us with 24, 26.2 with 16 or
+// 30, 27.8 with 8, 26.7 with 40, 30.0 with 64; 64 of up to 8192, 308 MB: 60.4 to 61.3, with 8 and 64 63); and the addition of a sequence's
+// pieces (a step is 1.5 us where work is short, the addition 2.8; 128 of 300 with 16, whole in two rounds, 21.8 us, with 8, dense, 26.8)
 constexpr int kStep = 8;
 constexpr int resident4(int dp) { return dp < 256 ? 3 : 2; }
-constexpr uint32_t kStart = 24;
+constexpr uint32_t kStart = 24, kCut = 16;
 // what removes the bias of int4 images, offset - 24, is computed with the offsets
 constexpr float kBias4 = 24.0f;
 
@@ -1484,14 +1485,19 @@ __device__ __forceinline__ void decode_pieces()
     if (pieces.empty) clear_empty();
 }
 
-// How Decode4's work is cut up: kStart and the halves of all sequences, one after the other, into ranges of `share`, the same for every
-// pair, as many as the card holds workgroups at once.  A workgroup takes one range of one pair, which may end one sequence and begin the
-// next; a sequence's pieces are the ranges that it touches.  Equal pieces per pair (Pieces) are more than fit at once, and the last
-// few run alone; here, where a start and an end cost as much as 400 positions, that is what counts most.
+// How Decode4's work is cut up: the sequences, one after the other, into ranges of `share` halves, the same for every pair.  A
+// workgroup takes one range of one pair; a sequence's pieces are the ranges that it touches.  There are `ranges` workgroups for a pair at once,
+// the start and the end of a range cost as much as kStart halves, and the addition of a sequence's pieces as much as kCut.  Taken is the least of
+//   whole   every sequence a range of its own, in rounds if there are more than `ranges`
+//   cut     every sequence into pieces of its own of `share` halves, no longer than the average range, at most `ranges` in all
+//   dense   kStart and the halves of a sequence behind those of the one before, so that a range may end one and begin the next
+// What is short takes as long as its longest piece: 64 sequences of up to 100, 8 heads of 128, 9.4 us, 16 dense, 8 of up to 600 13 and 15, one of
+// 1200 11.7 and 15.  What is long and cut evenly leaves the last pieces to run alone: 32 of up to 4095 26.3 us dense, 27.3 in pieces of its
+// sequences in one round, 33.9 in Pieces, which are more than fit at once.
 struct Ranges {
-    uint32_t share, before, mine, total;     // halves of a range; of the runs before this lane's, of it, of all
+    uint32_t share, count, before, mine, total;      // halves of a range; ranges at most; halves in the runs before this lane's, in it, in all
     int run, len;                            // sequences per lane; the length of the first
-    bool empty;                              // there is a sequence without positions
+    bool dense, empty;                       // there is a sequence without positions
 
     __device__ explicit Ranges(Args a)
     {
@@ -1499,21 +1505,51 @@ struct Ranges {
         run = (batch + 63) / 64;
         const int first = lane * run, end = min(first + run, batch);
         len = first < batch ? clamp_len(a, at(a->lens)[first]) : 0;
-        mine = cost_of(a, len);
-        bool none = first < batch && len == 0;
+        const uint32_t own = halves_of(a, len);
+        uint32_t halves = own, units = units_in(own), longest = units, there = own > 0;
+        bool none = first < batch && own == 0;
         for (int i = first + 1; i < end; i++) {
-            const uint32_t cost = cost_of(a, clamp_len(a, at(a->lens)[i]));
-            none = none || cost == 0;
-            mine += cost;
+            const uint32_t h = halves_of(a, clamp_len(a, at(a->lens)[i]));
+            halves += h, units += units_in(h), longest = max(longest, units_in(h)), there += h > 0;
+            none = none || h == 0;
         }
         empty = __any(none);
+        const uint32_t ranges = a->ranges;
+        uint32_t sequences = (uint32_t)__builtin_popcountll(__ballot(there)), chosen = kStep, most = sequences;
+        bool close = false;
+        if (run > 1 || sequences > ranges || __any(units > 1)) {            // (else one step each: choosing would take longer than the work)
+            if (run > 1) sequences = over_lanes(there, Add());
+            const uint32_t all = over_lanes(halves, Add());
+            longest = over_lanes(longest, Max());
+            const uint32_t average = max(divide(all + sequences * kStart + ranges - 1, a->by_ranges), (uint32_t)kStep);
+            // pieces of u units, no longer than the average range
+            uint32_t u = average / kStep;
+            bool cut = false;
+            if (run == 1) {
+                const auto pieces = [units](uint32_t u) { return over_lanes((units + u - 1) / u, Add()); };
+                while (u > 0 && pieces(u) <= ranges) u--, cut = true;
+                u += cut;
+            } else if (sequences < ranges) {                 // (as many pieces as units / u and one more for each sequence)
+                cut = over_lanes(units, Add()) <= (uint64_t)u * (ranges - sequences);
+            }
+            const uint32_t rounds = divide(sequences + ranges - 1, a->by_ranges);
+            const bool whole = (uint64_t)rounds * (kStart + longest * kStep) <= kStart + kCut + (cut ? u * kStep : average);
+            close = !whole && !cut;
+            chosen = whole ? longest * kStep : cut ? u * kStep : average;
+            most = whole ? sequences : ranges;
+        }
+        dense = close, share = chosen, count = most;
+        mine = cost_of(own);
+        for (int i = first + 1; i < end; i++) mine += cost_of(halves_of(a, clamp_len(a, at(a->lens)[i])));
         const uint32_t scan = scan_lanes(mine, Add());
         before = scan - mine;
         total = (uint32_t)__builtin_amdgcn_readlane((int)scan, 63);
-        // (at least one step of the workgroup)
-        share = max(divide(total + a->ranges - 1, a->by_ranges), (uint32_t)(kStep + kStart));
     }
-    __device__ static uint32_t cost_of(Args a, int len) { return len ? halves_of(a, len) + kStart : 0; }
+    __device__ static uint32_t units_in(uint32_t halves) { return (halves + kStep - 1) / kStep; }
+    template <class Op>
+    __device__ static uint32_t over_lanes(uint32_t v, Op op) { return (uint32_t)__builtin_amdgcn_readlane((int)scan_lanes(v, op), 63); }
+    __device__ uint32_t start() const { return dense ? kStart : 0; }
+    __device__ uint32_t cost_of(uint32_t halves) const { return dense ? halves ? halves + kStart : 0 : (halves + share - 1) / share * share; }
     // the sequence that holds y, its length, and what comes before it
     __device__ void find(Args a, uint32_t y, int &b, int &length, uint32_t &start) const
     {
@@ -1521,11 +1557,12 @@ struct Ranges {
         b = lane * run;
         start = (uint32_t)__builtin_amdgcn_readlane((int)before, lane);
         length = __builtin_amdgcn_readlane(len, lane);
-        uint32_t cost = cost_of(a, length);
+        if (run == 1) return;
+        uint32_t cost = cost_of(halves_of(a, length));
         while (y - start >= cost) {
             start += cost;
             length = clamp_len(a, scalar_load(a->lens + ++b));
-            cost = cost_of(a, length);
+            cost = cost_of(halves_of(a, length));
         }
     }
 };
@@ -1545,13 +1582,20 @@ __global__ __launch_bounds__(256, resident4(DP)) void paged_decode4_kernel(AttnA
         asm volatile("" ::"s"(lines));
         return r;
     }();
-    const uint32_t share = uniform(ranges.share), total = uniform(ranges.total), pairs = (uint32_t)args_now()->pairs, all = args_now()->ranges * pairs;
+    const uint32_t share = uniform(ranges.share), total = uniform(ranges.total), count = uniform(ranges.count), pairs = (uint32_t)args_now()->pairs;
+    const uint32_t all = count * pairs;
 
     for (uint32_t turn = blockIdx.x; turn < (all + kDealt - 1) / kDealt * kDealt; turn += gridDim.x) {
         // TOGETHER: the pairs of a range side by side, eight of them on one XCD
         const uint32_t piece = TOGETHER ? (turn & ~(kDealt - 1)) | ((turn & 7) << 3) | ((turn >> 3) & 7) : turn;
-        const uint32_t major = TOGETHER ? divide(piece, args_now()->by_pairs) : divide(piece, args_now()->by_ranges);
-        const uint32_t range = TOGETHER ? major : piece - major * args_now()->ranges, pair = TOGETHER ? piece - major * pairs : major;
+        uint32_t range, pair;
+        if (TOGETHER) {
+            range = divide(piece, args_now()->by_pairs);
+            pair = piece - range * pairs;
+        } else {
+            pair = count == args_now()->ranges ? divide(piece, args_now()->by_ranges) : uniform(piece / count);
+            range = piece - pair * count;
+        }
         if (piece >= all || range * share >= total) continue;
         const uint32_t range_end = min(range * share + share, total);
         uint32_t from = range * share, start;
@@ -1563,8 +1607,8 @@ __global__ __launch_bounds__(256, resident4(DP)) void paged_decode4_kernel(AttnA
             int head0, rows, n, number;
             float l, m;
             f32x4 acc[W::NP][W::PE];
-            // a sequence's first kStart are its cost alone, its halves follow; it is cut at multiples of a step of a wavefront
-            const uint32_t halves = uniform(halves_of(args_now(), len)), begin = start + kStart;
+            // dense: a sequence's first kStart are its cost alone, its halves follow; it is cut at multiples of a step of a wavefront
+            const uint32_t halves = uniform(halves_of(args_now(), len)), begin = start + ranges.start();
             const auto cut = [&](uint32_t at) { return begin + min(at > begin ? (at - begin + W::HS - 1) / W::HS * W::HS : 0, halves); };
             const uint32_t to = cut(range_end);
             from = cut(from);
@@ -1587,11 +1631,11 @@ __global__ __launch_bounds__(256, resident4(DP)) void paged_decode4_kernel(AttnA
 #pragma unroll
                         for (int i = 0; i < W::PE; i++) acc[h][i] = w.acc[h][i];
                 }
-                // a range has a piece that goes on in the next one, and one that came from the range before and ends here, at most
+                // dense: a range has a piece that goes on in the next one, and one that came from the range before and ends here, at most
                 const auto place = [&](int i) { return ((first_range + i) * 2 + (i < n - 1 ? 1 : 0)) * pairs + pair; };
                 end_piece<DP, QT>(lds, acc, l, m, (int64_t)b * args_now()->heads + head0, rows, n, number, place, W::kShift);
             }
-            if (begin + halves >= range_end) break;
+            if (!ranges.dense || begin + halves >= range_end) break;
             from = start = begin + halves;
             do len = uniform(clamp_len(args_now(), scalar_load(args_now()->lens + ++b)));
             while (len == 0);                                    // (there are halves left, so a sequence with some follows)
@@ -1821,9 +1865,9 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     a.halves = fast_div((a.span.d + kHalf - 1) / kHalf);
     if (ad == kPlain) {
         a.shares = kNumCU * resident4((int)p.dp);
-        // as many as the card holds, or as full sequences would make
-        const int64_t most = (batch * (a.capacity / kHalf + (int64_t)kStart) + kStep + kStart - 1) / (kStep + kStart), fit = a.shares / p.pairs;
-        a.ranges = (uint32_t)(fit < 1 ? 1 : fit < most ? fit : most);
+        // as many as the card holds, or as full sequences have steps
+        const int64_t most = batch * ((a.capacity / kHalf + kStep - 1) / kStep), fit = a.shares / p.pairs;
+        a.ranges = (uint32_t)(fit < 1 || most < 1 ? 1 : fit < most ? fit : most);
         a.by_ranges = fast_div(a.ranges);
         const int64_t pieces = a.ranges * p.pairs;
         p.workgroups = pieces < 2048 ? (pieces + kDealt - 1) / kDealt * kDealt : 2048;
