@@ -41,7 +41,7 @@
 // do not depend on it: the launch, two trips to memory for lengths and blocks, the first rows, and at the end the four
 // wavefronts' sums, their trip through the workspace and the addition.  With 32 query heads on 8 heads of 128: 32 sequences of up to 4095 tokens
 // (280 MB) 62 us, one of 131071 (537 MB) 104 us, int8, 64 of up to 8192 (563 MB) 120 us, one of 37 6.5 us.  int4: 32 of up to 4095 (78 MB)
-// 25.7 us, 64 of up to 8192 (308 MB) 61.2 us, one of 131071 (151 MB) 39.8 us, one of 37 6.7 us.
+// 26.1 us, 64 of up to 8192 (308 MB) 61.3 us, one of 131071 (151 MB) 38.9 us, one of 37 7.0 us.
 #include "paged_cache.h"
 #include "weight_quant_common.h"
 
@@ -731,7 +731,7 @@ struct Decode {
 //   of a head is left out as a rule; sums stay below 2^kSlack of what they would be, far from the end of float32
 //   scales and offsets come one position to a lane and are handed round through LDS: one load where Decode has four
 // Against Decode as kBlock, 8 heads of 128: 32 sequences of up to 4095 25.7 and 33.9 us, 64 of up to 8192 61.2 and 91.9, one of 131071
-// 39.8 and 45.8, one of 37 6.7 and 6.7; 64 of up to 8192, heads of 64 49 and 64, of 80 61 and 94; 32 of them, of 256 64 and 92.
+// 38.9 and 45.8, one of 37 7.0 and 6.7; 64 of up to 8192, heads of 64 49 and 64, of 80 61 and 94; 32 of them, of 256 64 and 92.
 // TOGETHER: a token's heads share cache lines, and other workgroups want what this one leaves.  Where heads have lines of their own, nobody
 // does, and requests are marked so (64 of up to 8192: 61.2 us, 66.5 unmarked; heads of 64 48.6 and 49.6, of 80 62 and 65; one of 131071 39.8
 // and 42) - but rows of 65 bytes and more come in two requests for the same line, which the mark makes two trips (heads of 256: 68 us and
@@ -1631,8 +1631,11 @@ __global__ __launch_bounds__(256, resident4(DP)) void paged_decode4_kernel(AttnA
 #pragma unroll
                         for (int i = 0; i < W::PE; i++) acc[h][i] = w.acc[h][i];
                 }
-                // dense: a range has a piece that goes on in the next one, and one that came from the range before and ends here, at most
-                const auto place = [&](int i) { return ((first_range + i) * 2 + (i < n - 1 ? 1 : 0)) * pairs + pair; };
+                // Dense: a range has a piece that goes on in the next one, and one that came from the range before and ends here, at most.
+                // Pair by pair, so that the arrivals of different pairs count in cache lines of their own (one sequence of 9353, 32 heads: 19 us,
+                // 29 with the pairs' counters side by side; one of 131071, 8 heads: 38.9 and 40.2)
+                const uint32_t places = pair * args_now()->ranges * 2 + first_range * 2;
+                const auto place = [&](int i) { return places + (uint32_t)(i * 2 + (i < n - 1 ? 1 : 0)); };
                 end_piece<DP, QT>(lds, acc, l, m, (int64_t)b * args_now()->heads + head0, rows, n, number, place, W::kShift);
             }
             if (!ranges.dense || begin + halves >= range_end) break;
