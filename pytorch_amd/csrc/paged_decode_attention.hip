@@ -41,7 +41,7 @@
 // do not depend on it: the launch, two trips to memory for lengths and blocks, the first rows, and at the end the four
 // wavefronts' sums, their trip through the workspace and the addition.  With 32 query heads on 8 heads of 128: 32 sequences of up to 4095 tokens
 // (280 MB) 62 us, one of 131071 (537 MB) 104 us, int8, 64 of up to 8192 (563 MB) 120 us, one of 37 6.5 us.  int4: 32 of up to 4095 (78 MB)
-// 26.1 us, 64 of up to 8192 (308 MB) 61.3 us, one of 131071 (151 MB) 38.9 us, one of 37 7.0 us.
+// 26.1 us, 64 of up to 8192 (308 MB) 61.3 us, one of 131071 (151 MB) 39.1 us, one of 37 7.0 us.
 #include "paged_cache.h"
 #include "weight_quant_common.h"
 
@@ -97,6 +97,7 @@ struct AttnArgs {
     uint32_t part_bytes, part_ml_bytes;
     float scale2;                            // scale * log2(e)
     int together;                            // the heads of a token share cache lines
+    int regular;                             // int4: no mask, blocks of a multiple of 16, parameters of a head's tokens side by side
 };
 
 // The kernel's arguments where the launch put them, in constant memory.  A kernel of several phases would otherwise load every
@@ -719,9 +720,8 @@ struct Decode {
     }
 };
 
-// int4, the layout that a cache has as a rule: blocks of a multiple of 16 tokens, keys and values alike, scales and offsets alike
-// with those of four tokens of a head in 16 aligned bytes, no mask.  Every half of a tile then lies in one block and starts at 16
-// times its number.  A row is 72 bytes of memory for as much arithmetic as one of 256 in 16 bits, so it is instructions that Decode runs short
+// int4, where keys and values lie alike, and scales and offsets, in blocks of 8 tokens and more, so that every half of a tile lies in one
+// block.  A row is 72 bytes of memory for as much arithmetic as one of 256 in 16 bits, so it is instructions that Decode runs short
 // of, not memory or matrix cycles, and this is about their number:
 //   the bias of the key images is what the first MFMA's sum starts from; that of the value images is taken off at the end, with the
 //   sum of the rounded products P_j scale_j that one more MFMA keeps, so it cancels exactly and one bf16 term is enough: 2^-8 of the
@@ -730,22 +730,26 @@ struct Decode {
 //   exponents are taken from a number m that is raised only where a score is more than kSlack above it, so the look at all lanes
 //   of a head is left out as a rule; sums stay below 2^kSlack of what they would be, far from the end of float32
 //   scales and offsets come one position to a lane and are handed round through LDS: one load where Decode has four
-// Against Decode as kBlock, 8 heads of 128: 32 sequences of up to 4095 25.7 and 33.9 us, 64 of up to 8192 61.2 and 91.9, one of 131071
-// 38.9 and 45.8, one of 37 7.0 and 6.7; 64 of up to 8192, heads of 64 49 and 64, of 80 61 and 94; 32 of them, of 256 64 and 92.
-// TOGETHER: a token's heads share cache lines, and other workgroups want what this one leaves.  Where heads have lines of their own, nobody
-// does, and requests are marked so (64 of up to 8192: 61.2 us, 66.5 unmarked; heads of 64 48.6 and 49.6, of 80 62 and 65; one of 131071 39.8
-// and 42) - but rows of 65 bytes and more come in two requests for the same line, which the mark makes two trips (heads of 256: 68 us and
-// 66; 32 of up to 4095, token by token, 50 and 44).
-template <int DP, int QT, bool TOGETHER>
+// Against Decode, 8 heads of 128: 32 sequences of up to 4095 26.1 and 33.9 us, 64 of up to 8192 61.3 and 91.9, one of 131071 39.1 and 45.8,
+// one of 37 7.0 and 6.7; 64 of up to 8192, heads of 64 50 and 64, of 80 62 and 94; 32 of them, of 256 65 and 92.
+//   kTogether  a token's heads share cache lines, and other workgroups want what this one leaves
+//   kAlone     heads have lines of their own, which nobody else wants, and requests are marked so (64 of up to 8192: 61.2 us, 66.5 unmarked; heads
+//              of 64 48.6 and 49.6, of 80 62 and 65; one of 131071 39.8 and 42) - but rows of 65 bytes and more come in two requests for the
+//              same line, which the mark makes two trips (heads of 256: 68 us and 66; 32 of up to 4095, token by token, 50 and 44)
+//   kAny       a mask, blocks of other than a multiple of 16 tokens, scales and offsets that do not lie token by token.  What that takes would cost the
+//              others 2 to 3 of a hundred.  Masked, 64 of up to 8192 80 us, 104 with Decode, 32 of up to 4095 30 and 36, 8 of up to 500 11.6 and 11;
+//              blocks of 24, 32 of up to 4095 32 and 41, 4 of 1000 13.5 and 12.7
+enum Kind { kAlone, kTogether, kAny };
+template <int DP, int QT, Kind KIND>
 struct Decode4 {
     static constexpr int NCH = DP / 32, KL = NCH / 2, PE = DP >= 128 ? 8 : 4, NP = DP / (16 * PE);
     static constexpr int TERMS = QT == 1 ? 2 : 1;
     static constexpr float kShift = 0.0f, kSlack = 8.0f, kNone = -3.402823466e38f;
     static constexpr int HS = kStep / 4;                         // halves of a step of a wavefront: a tile
-    static constexpr int kOnce = TOGETHER || DP == 256 ? 0 : 2;              // cache-policy bit: not temporal
+    static constexpr int kOnce = KIND == kAlone && DP < 256 ? 2 : 0;             // cache-policy bit: not temporal
 
     struct Place {                                               // of a step's halves
-        int n[HS], off[HS], id[HS];                              // positions seen, the first one's token within its block, its block
+        int n[HS], key[HS], off[HS], id[HS];                     // positions that are there, the first of them, its token within its block, its block
     };
 
     const Args a;
@@ -754,6 +758,7 @@ struct Decode4 {
     uint32_t koff[KL], voff[4][NP];
     uint32_t k[HS][KL][2], v[HS][4][NP];
     float param[4];                                              // of position `lane` of the step: key scale, offset, value scale, offset
+    bool hidden;                                                 // and what the mask says of it
     float *const lds;                                            // [4][64], of the whole step: key scale times scale2, key offset, value scale, value
                                                                  // offset times value scale
     u32x4 q[NCH];
@@ -762,6 +767,7 @@ struct Decode4 {
 
     int len, half_end;
     const int32_t *table;
+    const uint8_t *mask;
     const char *kbase, *vbase;
     const char *ksbase, *kobase, *vsbase, *vobase;
 
@@ -790,6 +796,10 @@ struct Decode4 {
     {
         len = len_, half_end = half_end_;
         table = a->table + b * a->table_stride;
+        if constexpr (KIND == kAny) {
+            mask = a->mask ? a->mask + b * a->mask_stride : nullptr;
+            hidden = false;
+        }
         kbase = a->cache.key.base + kvh * a->cache.key.head;
         vbase = a->cache.value.base + kvh * a->cache.value.head;
         ksbase = a->cache.key_scale.base + kvh * a->cache.key_scale.head;
@@ -827,6 +837,9 @@ struct Decode4 {
         }
         qsum = over_groups(qsum, [](float x, float y) { return x + y; });
     }
+    // the first position of half `half`, at token `off` of the sequence's block `span`, and how many tokens of it the block has
+    __device__ __forceinline__ int key_of(int half, uint32_t span, int off) const { return KIND == kAny ? (int)(span * a->span.d) + off : half * kHalf; }
+    __device__ __forceinline__ int in_block(const Place &p, int s) const { return KIND == kAny ? min((int)a->span.d - p.off[s], kHalf) : kHalf; }
     __device__ __forceinline__ Place place(int first) const
     {
         Place p;
@@ -835,17 +848,20 @@ struct Decode4 {
         if (a->halves.d % HS == 0) {                             // (a piece begins at a multiple of HS halves)
             const int id = scalar_load(table + min(span, (uint32_t)a->max_blocks - 1));
 #pragma unroll
-            for (int s = 0; s < HS; s++) p.off[s] = off + s * kHalf, p.id[s] = id;
+            for (int s = 0; s < HS; s++) p.off[s] = off + s * kHalf, p.key[s] = key_of(first + s, span, p.off[s]), p.id[s] = id;
         } else {
 #pragma unroll
             for (int s = 0; s < HS; s++) {
                 const uint32_t span_s = s ? divide(half + s, a->halves) : span;
                 p.off[s] = s ? (int)(half + s - span_s * a->halves.d) * kHalf : off;
+                p.key[s] = key_of(first + s, span_s, p.off[s]);
                 p.id[s] = scalar_load(table + min(span_s, (uint32_t)a->max_blocks - 1));
             }
         }
 #pragma unroll
-        for (int s = 0; s < HS; s++) p.n[s] = min(max(min(len, half_end * kHalf) - (first + s) * kHalf, 0), kHalf);
+        for (int s = 0; s < HS; s++)
+            p.n[s] = KIND == kAny ? first + s < half_end ? min(max(len - p.key[s], 0), in_block(p, s)) : 0
+                                  : min(max(min(len, half_end * kHalf) - p.key[s], 0), kHalf);
         return p;
     }
     // a block that the table does not name holds nothing
@@ -883,20 +899,27 @@ struct Decode4 {
             for (int s = 0; s < HS; s++) f(rows_of(base, p, s), 0, s);
         }
     }
-    // (those of a half that ends early lie in its block all the same)
+    // (those of a half that ends early lie in its block; of one that the block ends the last ones are read twice)
     __device__ __forceinline__ void load_params(const Place &p)
     {
+        const uint32_t token = KIND == kAny ? (uint32_t)a->cache.key_scale.token : 4;
         uint32_t start = 0;
+        int n = 0, key = 0;
 #pragma unroll
         for (int s = 0; s < HS; s++) {
-            const uint32_t of_half = (uint32_t)p.id[s] * (uint32_t)a->cache.key_scale.block + (uint32_t)p.off[s] * 4;
-            start = s == 0 || g == s ? of_half : start;          // (the groups behind the last half have the first one's)
+            const uint32_t of_half = (uint32_t)p.id[s] * (uint32_t)a->cache.key_scale.block + (uint32_t)p.off[s] * token;
+            const bool here = s == 0 || g == s;                  // (the groups behind the last half have the first one's)
+            start = here ? of_half : start;
+            n = here ? p.n[s] : n;
+            key = here ? p.key[s] : key;
         }
-        start += col * 4;
+        start += (uint32_t)(KIND == kAny ? min(col, max(n - 1, 0)) : col) * token;
         param[0] = *(const Global<float> *)(at(ksbase) + start);
         param[1] = *(const Global<float> *)(at(kobase) + start);
         param[2] = *(const Global<float> *)(at(vsbase) + start);
         param[3] = *(const Global<float> *)(at(vobase) + start);
+        if constexpr (KIND == kAny)
+            if (mask) hidden = col < n && at(mask)[key + col] != 0;
     }
     // (a row of D % 32 == 0 is whole pieces of 16 bytes, of which a lane takes one)
     __device__ __forceinline__ void load_keys(const Place &p)
@@ -968,23 +991,22 @@ struct Decode4 {
             for (int r = 0; r < 4; r++) z[s][r] = __builtin_fmaf(ko[r], qsum, z[s][r]);
         }
     }
-    __device__ __forceinline__ void store_scores(const f32x4 (&z)[HS], uint32_t valid, int b, int head0, int rows, int first) const
+    __device__ __forceinline__ void store_scores(const Place &p, const f32x4 (&z)[HS], uint32_t valid, int b, int head0, int rows, int first) const
     {
         if (col >= rows) return;
         Global<float> *to = at(a->scores) + ((int64_t)b * a->heads + head0 + col) * a->score_pitch + g * 4;
 #pragma unroll
         for (int s = 0; s < HS; s++) {
-            const int key = (first + s) * kHalf;
-            if (first + s >= half_end || key + g * 4 >= len) continue;       // (positions are stored in fours, the pitch is one of theirs)
+            if (first + s >= half_end || g * 4 >= min(len - p.key[s], in_block(p, s))) continue;       // (positions are stored in fours)
             const f32x4 t = four(0, s);
             f32x4 w;
 #pragma unroll
             for (int r = 0; r < 4; r++) w[r] = (valid >> (4 * s + r)) & 1 ? z[s][r] * t[r] : -INFINITY;
-            *(Global<f32x4> *)(to + key) = w;
+            *(Global<f32x4> *)(to + p.key[s]) = w;
         }
     }
     // probabilities times value scales
-    __device__ __forceinline__ void add(const Place &place, uint32_t valid, const f32x4 (&z)[HS], u32x4 (&terms)[TERMS])
+    __device__ __forceinline__ void add(bool whole, uint32_t valid, const f32x4 (&z)[HS], u32x4 (&terms)[TERMS])
     {
         constexpr int N = HS * 4;
         float e[N];
@@ -995,7 +1017,7 @@ struct Decode4 {
 #pragma unroll
                 for (int r = 0; r < 4; r++) e[4 * s + r] = __builtin_fmaf(z[s][r], t[r], -m);
             }
-            if (!full(place)) {
+            if (!whole) {
                 no_select();
 #pragma unroll
                 for (int i = 0; i < N; i++) e[i] = (valid >> i) & 1 ? e[i] : -INFINITY;
@@ -1034,7 +1056,7 @@ struct Decode4 {
                 p[r] = __builtin_amdgcn_exp2f(e[4 * s + r]);
                 l += p[r];
             }
-            if (!full(place)) {                                  // (a scale and an offset that are not seen may be anything)
+            if (!whole) {                                        // (a scale and an offset that are not seen may be anything)
                 no_select();
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
@@ -1110,22 +1132,28 @@ struct Decode4 {
                 set_priority(--behind);
             }
             uint32_t valid = (1u << (4 * HS)) - 1;
-            if (!full(cur)) {
+            bool whole = full(cur);
+            if (!whole) {
                 no_select();
                 valid = seen(cur);
+            }
+            if (KIND == kAny && mask) {
+                const uint32_t out = (uint32_t)__ballot(hidden) >> (g * 4);
+                valid &= ~((out & 15) | (out >> 16 & 15) << 4);
+                whole = whole && !__any(hidden);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) lds[i * 64 + g * 16 + col] = i == 0 ? param[0] * a->scale2 : i == 3 ? param[3] * param[2] : param[i];
             __builtin_amdgcn_wave_barrier();                     // (a wavefront's LDS accesses are done in their order)
             f32x4 z[HS];
             score(z);
-            if (a->scores) store_scores(z, valid, b, head0, rows, first);
+            if (a->scores) store_scores(cur, z, valid, b, head0, rows, first);
             settle(next);
             load_keys(next);
             load_params(next);
             __builtin_amdgcn_sched_barrier(0);
             u32x4 terms[TERMS];
-            add(cur, valid, z, terms);
+            add(whole, valid, z, terms);
             weigh(terms);
             __builtin_amdgcn_wave_barrier();
             load_values(next);
@@ -1522,8 +1550,9 @@ struct Ranges {
             const uint32_t all = over_lanes(halves, Add());
             longest = over_lanes(longest, Max());
             const uint32_t average = max(divide(all + sequences * kStart + ranges - 1, a->by_ranges), (uint32_t)kStep);
-            // pieces of u units, no longer than the average range
-            uint32_t u = average / kStep;
+            // pieces of u units, no longer than the average range, or, where that is short, taking no more steps (4 sequences of 4000, 8 heads:
+            // 15.1 us and 16.8)
+            uint32_t u = average <= 2 * kStep ? units_in(average) : average / kStep;
             bool cut = false;
             if (run == 1) {
                 const auto pieces = [units](uint32_t u) { return over_lanes((units + u - 1) / u, Add()); };
@@ -1567,10 +1596,10 @@ struct Ranges {
     }
 };
 
-template <int DP, int QT, bool TOGETHER>
+template <int DP, int QT, Kind KIND>
 __global__ __launch_bounds__(256, resident4(DP)) void paged_decode4_kernel(AttnArgs)
 {
-    using W = Decode4<DP, QT, TOGETHER>;
+    using W = Decode4<DP, QT, KIND>;
     __shared__ Shared<DP> lds;
     static_assert(sizeof(lds.red[0]) >= 4 * 64 * sizeof(float), "a wavefront's parameters lie where its sums will be");
     const Ranges ranges = [] {
@@ -1586,10 +1615,11 @@ __global__ __launch_bounds__(256, resident4(DP)) void paged_decode4_kernel(AttnA
     const uint32_t all = count * pairs;
 
     for (uint32_t turn = blockIdx.x; turn < (all + kDealt - 1) / kDealt * kDealt; turn += gridDim.x) {
-        // TOGETHER: the pairs of a range side by side, eight of them on one XCD
-        const uint32_t piece = TOGETHER ? (turn & ~(kDealt - 1)) | ((turn & 7) << 3) | ((turn >> 3) & 7) : turn;
+        // together: the pairs of a range side by side, eight of them on one XCD
+        const bool together = KIND == kAny ? args_now()->together : KIND == kTogether;
+        const uint32_t piece = together ? (turn & ~(kDealt - 1)) | ((turn & 7) << 3) | ((turn >> 3) & 7) : turn;
         uint32_t range, pair;
-        if (TOGETHER) {
+        if (together) {
             range = divide(piece, args_now()->by_pairs);
             pair = piece - range * pairs;
         } else {
@@ -1748,8 +1778,9 @@ template <int DP, int QT>
 void launch_attention4(const AttnArgs &a, Addressing ad, unsigned workgroups, hipStream_t s)
 {
     const dim3 grid(workgroups), block(256);
-    if (ad == kPlain && a.together) hipLaunchKernelGGL((paged_decode4_kernel<DP, QT, true>), grid, block, 0, s, a);
-    else if (ad == kPlain) hipLaunchKernelGGL((paged_decode4_kernel<DP, QT, false>), grid, block, 0, s, a);
+    if (ad == kPlain && !a.regular) hipLaunchKernelGGL((paged_decode4_kernel<DP, QT, kAny>), grid, block, 0, s, a);
+    else if (ad == kPlain && a.together) hipLaunchKernelGGL((paged_decode4_kernel<DP, QT, kTogether>), grid, block, 0, s, a);
+    else if (ad == kPlain) hipLaunchKernelGGL((paged_decode4_kernel<DP, QT, kAlone>), grid, block, 0, s, a);
     else if (ad == kRows) hipLaunchKernelGGL((paged_decode_kernel<DP, 4, QT, kRows>), grid, block, 0, s, a);
     else if (ad == kBlockMask) hipLaunchKernelGGL((paged_decode_kernel<DP, 4, QT, kBlockMask>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((paged_decode_kernel<DP, 4, QT, kBlock>), grid, block, 0, s, a);
@@ -1844,20 +1875,22 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     // Halves that lie in one block: block by block, the last half of a block may be short, so blocks of fewer than 8 tokens
     // would leave most of a tile empty.  Offsets within a block have 31 bits, a block's own offset is a 32 x 32-bit product.
     const PagedArray *const arrays[] = {&a.cache.key, &a.cache.value, &a.cache.key_scale, &a.cache.value_scale, &a.cache.key_offset, &a.cache.value_offset};
-    bool blocks = pieces && cache->block_size >= 8 && (!mask || cache->block_size % 4 == 0), scales = cache->block_size % 4 == 0;
+    bool blocks = pieces && cache->block_size >= 8, scales = cache->block_size % 4 == 0;
     for (int i = 0; i < (bits == 4 ? 6 : quant ? 4 : 2); i++) {
         const PagedArray &x = *arrays[i];
         blocks = blocks && x.block >= 0 && x.block <= 0xffffffffll && x.token >= 0 && x.token <= 0x7fffffff / (cache->block_size + 16);
         if (i >= 2) scales = scales && x.token == 4 && aligned(x.base, 16) && x.block % 16 == 0 && x.head % 16 == 0;
     }
     const auto alike = [](const PagedArray &x, const PagedArray &y) { return x.block == y.block && x.token == y.token && x.head == y.head; };
-    const bool same = quant && scales && alike(a.cache.key, a.cache.value) && alike(a.cache.key_scale, a.cache.value_scale) &&
-                      (bits == 8 || (alike(a.cache.key_scale, a.cache.key_offset) && alike(a.cache.key_scale, a.cache.value_offset)));
+    const bool same = quant && alike(a.cache.key, a.cache.value) && alike(a.cache.key_scale, a.cache.value_scale);
     // Decode4: offsets into a whole array of parameters have 32 bits, and so do the halves of all sequences; a few steps behind the
     // last position still have a number in 31
-    const bool plain = bits == 4 && same && cache->block_size % 16 == 0 && a.cache.key_scale.block <= 0xffffffffll / cache->num_blocks &&
-                       a.capacity < 0x7fff0000 && batch * (a.capacity / kHalf + (int64_t)kStart) < 0x7fff0000;
-    const Addressing ad = !blocks ? kRows : mask ? kBlockMask : plain ? kPlain : same && bits == 8 ? kBlockAlike : kBlock;
+    const PagedArray &par = a.cache.key_scale;
+    const int64_t halves = max_blocks * ((cache->block_size + kHalf - 1) / kHalf);       // of a sequence at most
+    const bool plain = bits == 4 && same && alike(par, a.cache.key_offset) && alike(par, a.cache.value_offset) && par.block >= 0 && par.token >= 0 &&
+                       par.block <= 0xffffffffll / cache->num_blocks && par.block * cache->num_blocks + par.token * cache->block_size <= 0xffffffffll &&
+                       (!attn_sums || cache->block_size % 4 == 0) && a.capacity < 0x7fff0000 && batch * (halves + kStart) < 0x7fff0000;
+    const Addressing ad = !blocks ? kRows : plain ? kPlain : mask ? (cache->block_size % 4 == 0 ? kBlockMask : kRows) : same && scales && bits == 8 ? kBlockAlike : kBlock;
     // Rows of several heads in a cache line, with other heads' rows of the same token: work on them at the same time and on one XCD,
     // so that the line comes once (16 sequences of up to 1001 tokens, 32 heads of 80: 32.4 -> 28.6 us; int8, 32 sequences of up to
     // 4095, 8 heads of 64: 34.5 -> 26.2 us).  Where heads have lines of their own, that would make the workgroups ask the same
@@ -1866,10 +1899,11 @@ extern "C" int mi355_paged_decode_attention(const mi355_paged_cache *cache, cons
     a.together = shared(a.cache.key) || shared(a.cache.value);
     a.span = ad != kRows ? a.cache.page : fast_div(kHalf);
     a.halves = fast_div((a.span.d + kHalf - 1) / kHalf);
+    a.regular = !mask && cache->block_size % 16 == 0 && par.token == 4;
     if (ad == kPlain) {
         a.shares = kNumCU * resident4((int)p.dp);
         // as many as the card holds, or as full sequences have steps
-        const int64_t most = batch * ((a.capacity / kHalf + kStep - 1) / kStep), fit = a.shares / p.pairs;
+        const int64_t most = batch * ((halves + kStep - 1) / kStep), fit = a.shares / p.pairs;
         a.ranges = (uint32_t)(fit < 1 || most < 1 ? 1 : fit < most ? fit : most);
         a.by_ranges = fast_div(a.ranges);
         const int64_t pieces = a.ranges * p.pairs;

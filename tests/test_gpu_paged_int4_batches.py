@@ -39,6 +39,49 @@ def test_ragged_batches(pa, batch, longest, page, heads, kv, dim, dt, order):  #
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
 
 
+@pytest.mark.parametrize("page", [8, 9, 10, 16, 24, 31, 40, 100])
+@pytest.mark.parametrize("params", ["head", "token", "spread"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_blocks_and_masks(pa, page, params, masked):  # noqa: F811
+    """Blocks that end inside a tile, with and without a mask; scales and offsets of what is not seen are NaN, unnamed blocks among the others."""
+    g = torch.Generator().manual_seed(page)
+    dt, order = (torch.bfloat16, "token") if page % 2 else (torch.float16, "head")
+    lens = [700, 0, 33, page, page + 1, 250, 1]
+    batch, width = len(lens), -(-700 // page)
+    cache = Cache(g, batch * width + 1, page, 2, 80, order=order, params=params)
+    table = tables(g, batch, width, batch * width + 1, page)
+    q, lens = torch.randn(batch, 8, 80, generator=g).to(dt), torch.tensor(lens, dtype=torch.int32)
+    mask = torch.rand(batch, width * page, generator=g) < 0.4 if masked else None
+    if masked:
+        mask[3] = True
+    table[0, 2], table[5, 1] = -1, batch * width + 1
+    at = torch.arange(width * page)
+    unseen = torch.ones(batch * width + 1, page, dtype=torch.bool)
+    for b in range(batch):
+        see = (at < lens[b]) & ((table[b].long() >= 0) & (table[b] < len(unseen)))[at // page]
+        see = see & ~mask[b] if masked else see
+        unseen[table[b].long()[at[see] // page], at[see] % page] = False
+    for t in (cache.ks, cache.vs, cache.ko, cache.vo):
+        t[unseen] = math.nan
+    got = attend(pa, cache, q, table, lens, atten_mask=None if mask is None else mask.cuda())
+    assert bool(got[0].isfinite().all())
+    check_attention(got, cache, q, table, lens, mask=mask)
+
+
+@pytest.mark.parametrize("page", [8, 12, 24, 64])
+def test_sums_over_blocks(pa, page):  # noqa: F811
+    """Weights added to the sums of the positions that they belong to, where blocks end inside a tile and sequences are cut."""
+    g = torch.Generator().manual_seed(page)
+    cache, q, table, lens = batch_of(g, [2100, 30, 0, 333], page, 8, 2, 128, torch.bfloat16, "head")
+    width = table.shape[1]
+    mask = torch.rand(4, width * page, generator=g) < 0.3
+    for m in (None, mask):
+        before = torch.rand(4, 2, width * page, generator=g)
+        sums = before.cuda()
+        got = attend(pa, cache, q, table, lens, atten_mask=None if m is None else m.cuda(), attn_sums=sums)
+        check_attention(got, cache, q, table, lens, mask=m, sums=(before, sums))
+
+
 def test_batches_of_nothing(pa):  # noqa: F811
     g = torch.Generator().manual_seed(0)
     for lens in ([0], [0] * 70, [0, 0, 1, 0], [-3, 5, 0]):
