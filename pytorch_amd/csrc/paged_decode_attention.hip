@@ -35,7 +35,7 @@
 // are cut into halves of a tile, 16 positions of one block (fewer at a block's end), eight halves make a unit, and a pair
 // of more units than the card's fair share is cut into equal pieces of at most that.  A workgroup takes a piece at a time; a
 // pair of one piece is finished there, else the workgroup leaves (sums, m, l) in the workspace, and the last one to arrive adds
-// them in their order.
+// them in their order.  (int4: Ranges.)
 //
 // Bound by memory, at 5.5 to 5.9 TB/s where the work is long (32 sequences of 8192, 1.07 GB, in 188 us), behind about 12 us that
 // do not depend on it: the launch, two trips to memory for lengths and blocks, the first rows, and at the end the four
@@ -255,7 +255,7 @@ __device__ __forceinline__ float over_groups(float v, Op op)
 // 32 sequences of up to 4095, 8 heads of 128, blocks of 16: 62.9 us as kBlock, 74.4 as kRows; 16 masked ones, 32 heads of 80,
 // blocks of 24: 28.6 as kBlockMask, 36.4 as kRows; int8, 64 of up to 8192: 219.9 as kRows.  A short half wastes its operand's
 // rows, so kBlock loses with small blocks: 66.2 and 74.8 us for blocks of 8, 79.8 and 75 for 5, 84.9 and 75.4 for 4.
-//   kPlain  int4: as Decode4 wants it
+//   kPlain  int4: Decode4, which has the conditions
 enum Addressing { kRows, kBlock, kBlockAlike, kBlockMask, kPlain };
 
 // The images of an int4 word's codes i and i + 4: its bits 4 i and 16 + 4 i on, as the top mantissa bits of 16.0, the sign bit turned.
