@@ -41,7 +41,7 @@
 // do not depend on it: the launch, two trips to memory for lengths and blocks, the first rows, and at the end the four
 // wavefronts' sums, their trip through the workspace and the addition.  With 32 query heads on 8 heads of 128: 32 sequences of up to 4095 tokens
 // (280 MB) 62 us, one of 131071 (537 MB) 104 us, int8, 64 of up to 8192 (563 MB) 120 us, one of 37 6.5 us.  int4: 32 of up to 4095 (78 MB)
-// 26.1 us, 64 of up to 8192 (308 MB) 61.3 us, one of 131071 (151 MB) 39.1 us, one of 37 7.0 us.
+// 26.1 us, 64 of up to 8192 (308 MB) 61.3 us, one of 131071 (151 MB) 39.1 us, one of 37 6.9 us.
 #include "paged_cache.h"
 #include "weight_quant_common.h"
 
@@ -731,7 +731,7 @@ struct Decode {
 //   of a head is left out as a rule; sums stay below 2^kSlack of what they would be, far from the end of float32
 //   scales and offsets come one position to a lane and are handed round through LDS: one load where Decode has four
 // Against Decode, 8 heads of 128: 32 sequences of up to 4095 26.1 and 33.9 us, 64 of up to 8192 61.3 and 91.9, one of 131071 39.1 and 45.8,
-// one of 37 7.0 and 6.7; 64 of up to 8192, heads of 64 50 and 64, of 80 62 and 94; 32 of them, of 256 65 and 92.
+// one of 37 6.9 and 6.7; 64 of up to 8192, heads of 64 50 and 64, of 80 62 and 94; 32 of them, of 256 65 and 92.
 //   kTogether  a token's heads share cache lines, and other workgroups want what this one leaves
 //   kAlone     heads have lines of their own, which nobody else wants, and requests are marked so (64 of up to 8192: 61.2 us, 66.5 unmarked; heads
 //              of 64 48.6 and 49.6, of 80 62 and 65; one of 131071 39.8 and 42) - but rows of 65 bytes and more come in two requests for the
@@ -1519,8 +1519,8 @@ __device__ __forceinline__ void decode_pieces()
 //   whole   every sequence a range of its own, in rounds if there are more than `ranges`
 //   cut     every sequence into pieces of its own of `share` halves, no longer than the average range, at most `ranges` in all
 //   dense   kStart and the halves of a sequence behind those of the one before, so that a range may end one and begin the next
-// What is short takes as long as its longest piece: 64 sequences of up to 100, 8 heads of 128, 9.4 us, 16 dense, 8 of up to 600 13 and 15, one of
-// 1200 11.7 and 15.  What is long and cut evenly leaves the last pieces to run alone: 32 of up to 4095 26.3 us dense, 27.3 in pieces of its
+// What is short takes as long as its longest piece: 64 sequences of up to 100, 8 heads of 128, 9.4 us, 16 dense, 8 of up to 600 12.3 and 15, one of
+// 1200 11.2 and 15.  What is long and cut evenly leaves the last pieces to run alone: 32 of up to 4095 26.3 us dense, 27.3 in pieces of its
 // sequences in one round, 33.9 in Pieces, which are more than fit at once.
 struct Ranges {
     uint32_t share, count, before, mine, total;      // halves of a range; ranges at most; halves in the runs before this lane's, in it, in all
@@ -1534,21 +1534,23 @@ struct Ranges {
         const int first = lane * run, end = min(first + run, batch);
         len = first < batch ? clamp_len(a, at(a->lens)[first]) : 0;
         const uint32_t own = halves_of(a, len);
+        const auto others = [&](auto f) {                        // halves of the lane's other sequences
+            for (int i = first + 1; i < end; i++) f(halves_of(a, clamp_len(a, at(a->lens)[i])));
+        };
         uint32_t halves = own, units = units_in(own), longest = units, there = own > 0;
         bool none = first < batch && own == 0;
-        for (int i = first + 1; i < end; i++) {
-            const uint32_t h = halves_of(a, clamp_len(a, at(a->lens)[i]));
-            halves += h, units += units_in(h), longest = max(longest, units_in(h)), there += h > 0;
-            none = none || h == 0;
-        }
+        others([&](uint32_t h) { halves += h, units += units_in(h), longest = max(longest, units_in(h)), there += h > 0, none = none || h == 0; });
         empty = __any(none);
-        const uint32_t ranges = a->ranges;
-        uint32_t sequences = (uint32_t)__builtin_popcountll(__ballot(there)), chosen = kStep, most = sequences;
+        const uint32_t ranges = a->ranges, sequences = run == 1 ? (uint32_t)__builtin_popcountll(__ballot(there)) : over_lanes(there, Add());
+        const uint32_t steps = over_lanes(units, Add());
+        uint32_t chosen = kStep, most = ranges, cost = units * kStep;
         bool close = false;
-        if (run > 1 || sequences > ranges || __any(units > 1)) {            // (else one step each: choosing would take longer than the work)
-            if (run > 1) sequences = over_lanes(there, Add());
-            const uint32_t all = over_lanes(halves, Add());
-            longest = over_lanes(longest, Max());
+        if (sequences <= ranges && !__any(longest > 2)) {        // whole: two steps take less than an addition
+            if (__any(longest > 1)) chosen = 2 * kStep;
+            cost = there * chosen;
+            most = sequences;
+        } else if (steps > ranges) {                             // (else cut into single steps)
+            const uint32_t all = over_lanes(halves, Add()), tallest = over_lanes(longest, Max());
             const uint32_t average = max(divide(all + sequences * kStart + ranges - 1, a->by_ranges), (uint32_t)kStep);
             // pieces of u units, no longer than the average range, or, where that is short, taking no more steps (4 sequences of 4000, 8 heads:
             // 15.1 us and 16.8)
@@ -1556,20 +1558,20 @@ struct Ranges {
             bool cut = false;
             if (run == 1) {
                 const auto pieces = [units](uint32_t u) { return over_lanes((units + u - 1) / u, Add()); };
-                while (u > 0 && pieces(u) <= ranges) u--, cut = true;
+                while (u > 1 && pieces(u) <= ranges) u--, cut = true;
                 u += cut;
-            } else if (sequences < ranges) {                 // (as many pieces as units / u and one more for each sequence)
-                cut = over_lanes(units, Add()) <= (uint64_t)u * (ranges - sequences);
+            } else if (sequences < ranges) {                     // (as many pieces as units / u and one more for each sequence)
+                cut = steps <= (uint64_t)u * (ranges - sequences);
             }
             const uint32_t rounds = divide(sequences + ranges - 1, a->by_ranges);
-            const bool whole = (uint64_t)rounds * (kStart + longest * kStep) <= kStart + kCut + (cut ? u * kStep : average);
+            const bool whole = (uint64_t)rounds * (kStart + tallest * kStep) < kStart + kCut + (cut ? u * kStep : average);
             close = !whole && !cut;
-            chosen = whole ? longest * kStep : cut ? u * kStep : average;
+            chosen = whole ? tallest * kStep : cut ? u * kStep : average;
             most = whole ? sequences : ranges;
+            cost = cost_of(own, close, chosen);
+            others([&](uint32_t h) { cost += cost_of(h, close, chosen); });
         }
-        dense = close, share = chosen, count = most;
-        mine = cost_of(own);
-        for (int i = first + 1; i < end; i++) mine += cost_of(halves_of(a, clamp_len(a, at(a->lens)[i])));
+        dense = close, share = chosen, count = most, mine = cost;
         const uint32_t scan = scan_lanes(mine, Add());
         before = scan - mine;
         total = (uint32_t)__builtin_amdgcn_readlane((int)scan, 63);
@@ -1578,7 +1580,10 @@ struct Ranges {
     template <class Op>
     __device__ static uint32_t over_lanes(uint32_t v, Op op) { return (uint32_t)__builtin_amdgcn_readlane((int)scan_lanes(v, op), 63); }
     __device__ uint32_t start() const { return dense ? kStart : 0; }
-    __device__ uint32_t cost_of(uint32_t halves) const { return dense ? halves ? halves + kStart : 0 : (halves + share - 1) / share * share; }
+    __device__ static uint32_t cost_of(uint32_t halves, bool dense, uint32_t share)
+    {
+        return dense ? halves ? halves + kStart : 0 : (halves + share - 1) / share * share;
+    }
     // the sequence that holds y, its length, and what comes before it
     __device__ void find(Args a, uint32_t y, int &b, int &length, uint32_t &start) const
     {
@@ -1587,11 +1592,11 @@ struct Ranges {
         start = (uint32_t)__builtin_amdgcn_readlane((int)before, lane);
         length = __builtin_amdgcn_readlane(len, lane);
         if (run == 1) return;
-        uint32_t cost = cost_of(halves_of(a, length));
+        uint32_t cost = cost_of(halves_of(a, length), dense, share);
         while (y - start >= cost) {
             start += cost;
             length = clamp_len(a, scalar_load(a->lens + ++b));
-            cost = cost_of(halves_of(a, length));
+            cost = cost_of(halves_of(a, length), dense, share);
         }
     }
 };
