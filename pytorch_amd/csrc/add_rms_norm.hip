@@ -8,7 +8,7 @@
 // rstd is one positive factor of a whole row, so it cancels in the codes: they are those of u, do not depend on the order in
 // which squares are added, and the sum and the maximum are reduced together, behind one barrier.
 //
-// One row per workgroup (or per wavefront, where rows are short), held in registers from its only load to its only store.
+// One row per workgroup (per wavefront or per 16 lanes, where rows are short), held in registers from its only load to its only store.
 //
 // Bound by memory where rows are many: 8191 rows of 8192 to int8, 470 MB, in 80 us, 5.9 TB/s; 2047 of 5128 in 16 bits, 84 MB, in 15.0 us,
 // 5.6 TB/s.  Few rows are bound by the launch and one trip to memory and back: one row of 4096 to int8 in 2.9 us, 64 of 8192 in 3.8.
@@ -131,11 +131,21 @@ __device__ __forceinline__ void reduce_wave(float &sum, uint32_t &top)
     sum = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(sum), 63));
     top = (uint32_t)__builtin_amdgcn_readlane((int)top, 63);
 }
-// the same over the wavefronts of a workgroup that works on one row
-template <int WAVES>
+// over 16 lanes, in all of them: neighbours, pairs, mirrored fours, mirrored eights
+__device__ __forceinline__ void reduce_16(float &sum, uint32_t &top)
+{
+    reduce_step<0xb1, 0xf>(sum, top);
+    reduce_step<0x4e, 0xf>(sum, top);
+    reduce_step<0x141, 0xf>(sum, top);
+    reduce_step<0x140, 0xf>(sum, top);
+}
+// the same over the threads of a row: 16 lanes, a wavefront, or the wavefronts of a workgroup
+template <int TPR>
 __device__ __forceinline__ void reduce_row(float &sum, uint32_t &top, float (&sums)[16], uint32_t (&tops)[16])
 {
-    reduce_wave(sum, top);
+    constexpr int WAVES = TPR / 64;
+    if constexpr (TPR == 16) reduce_16(sum, top);
+    else reduce_wave(sum, top);
     if constexpr (WAVES > 1) {
         if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum, tops[threadIdx.x >> 6] = top;
         __syncthreads();
@@ -198,12 +208,12 @@ __device__ __forceinline__ void add8(const NormArgs &a, u32x4 v1, u32x4 v2, floa
 template <int BLOCK, int TPR, int VPT, bool INT8, bool FP16, bool ANY>
 __global__ __launch_bounds__(BLOCK) void norm_rows_kernel(NormArgs a)
 {
-    static_assert(TPR == 64 || TPR == BLOCK, "a row belongs to a wavefront or to the workgroup");
+    static_assert(TPR == 16 || TPR == 64 || TPR == BLOCK, "a row belongs to 16 lanes, a wavefront or the workgroup");
     __shared__ float sums[16];
     __shared__ uint32_t tops[16];
     const int t = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
-    if (row >= a.rows) return;                                   // whole wavefronts, and no barrier follows if they are rows
+    if (row >= a.rows) return;                                   // all threads of a row, and no barrier follows if those are not the workgroup
     const uint16_t *x1 = a.x1 + row * a.x1_stride, *x2 = a.x2 + row * a.x2_stride;
 
     u32x4 v1[VPT], v2[VPT];
@@ -245,7 +255,7 @@ __global__ __launch_bounds__(BLOCK) void norm_rows_kernel(NormArgs a)
             }
         }
     }
-    reduce_row<TPR / 64>(sum, top, sums, tops);
+    reduce_row<TPR>(sum, top, sums, tops);
     const float rstd = rstd_of(sum, a);
     if constexpr (INT8) {
         const Codes codes(__uint_as_float(top));
@@ -288,7 +298,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
 #pragma unroll
         for (int k = 0; k < 8; k++) top = max(top, __float_as_uint(s[k] * g[k]) & 0x7fffffffu);
     }
-    reduce_row<16>(sum, top, sums, tops);
+    reduce_row<1024>(sum, top, sums, tops);
     const float rstd = rstd_of(sum, a);
     const Codes codes(__uint_as_float(top));
     if (threadIdx.x == 0 && a.stat) a.stat[row] = INT8 ? codes.step * rstd : rstd;
@@ -318,7 +328,14 @@ void launch_norm(const NormArgs &a, bool any, hipStream_t s)
     // Two pieces a thread from 1025 columns on, as long as a workgroup has the threads: 64 rows of 8192 take 5.0 us with four pieces for 256
     // threads, 3.9 with two for 512, 3.8 with one for 1024; 8191 rows to int8 85, 82 and 87; one row of 4096 3.1 us with two for 256 or one for 512.
     const int pieces = (a.cols - 1) / 8 + 1;
-    if (pieces <= 64) launch_rows<256, 64, 1, INT8, FP16>(a, any, s);
+    // Up to 256 columns 16 lanes a row: a wavefront's lanes would idle, and a row's divisions count for it alone (20000 rows of 72 7.7 and 4.4 us, to
+    // int8 15.4 and 6.5; 64 of 64 2.9 and 2.2; 1000 of 200 2.8 and 3.2).  Up to 512 they need four pieces a thread, which pays for many
+    // rows to int8 (8191 of 512 9.6 and 7.9 us, of 300 11.2 and 8.9; in 16 bits 6.9 and 7.7; 1000 of 512 3.8 and 5.1).
+    if (pieces <= 16) launch_rows<256, 16, 1, INT8, FP16>(a, any, s);
+    else if (pieces <= 32) launch_rows<256, 16, 2, INT8, FP16>(a, any, s);
+    else if (pieces <= 64 && INT8 && a.rows >= 4096) {
+        if constexpr (INT8) launch_rows<256, 16, 4, INT8, FP16>(a, any, s);
+    } else if (pieces <= 64) launch_rows<256, 64, 1, INT8, FP16>(a, any, s);
     else if (pieces <= 256) launch_rows<256, 256, 1, INT8, FP16>(a, any, s);
     else if (pieces <= 512) launch_rows<256, 256, 2, INT8, FP16>(a, any, s);
     else if (pieces <= 1024) launch_rows<512, 512, 2, INT8, FP16>(a, any, s);

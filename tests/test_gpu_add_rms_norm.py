@@ -100,6 +100,12 @@ def test_rows(pa, rows, cols):
     check(pa, *make(rows, cols, torch.bfloat16, seed=rows))
 
 
+@pytest.mark.parametrize("rows", [5, 17, 4095, 4099])
+@pytest.mark.parametrize("cols", [3, 8, 72, 100, 128, 129, 250, 256, 257, 300, 511, 512])
+def test_rows_that_share_a_wavefront(pa, rows, cols):
+    check(pa, *make(rows, cols, torch.bfloat16 if cols % 3 else torch.float16, seed=rows + cols))
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("cols", [77, 512, 4096])
 def test_float32_gamma(pa, cols, dt):
