@@ -506,8 +506,10 @@ int mi355_paged_cache_read(const mi355_paged_cache *cache, void *key, const int6
  *   s_j = scale * sum_d q[b,h,d] key[j,d]       lse = log sum_j exp(s_j)
  *   out[b,h,:] = sum_j exp(s_j - lse) value[j,:]
  *   attn_sums[b, kv head, j] += sum over the kv head's query heads of exp(s_j - lse)
- * Scores, sums and outputs are accumulated in float32.  Where nothing is seen out is 0 and lse -infinity.  Values and keys
- * that are not seen have no influence, NaN included.
+ * Scores, sums and outputs are accumulated in float32.  The weights w_j = exp(s_j - lse) are rounded for the second product: to the
+ * type of a 16-bit cache, by 2^-8 (bf16) or 2^-11 of each; times the scale of a code, by 2^-16, on int4 caches, in every layout, by at most
+ * 2^-11 of sum_j w_j |scale_j| in an element of out.  Where nothing is seen out is 0 and lse -infinity.  Values and keys that are not seen
+ * have no influence, NaN included.
  *   q             [batch, heads, head_dim] of q_dtype (the cache's own type; bf16 or fp16 with int8 and int4), strides in elements
  *   out           [batch, heads, head_dim] of q_dtype, contiguous; lse float32 [batch, heads] or NULL
  *   block_table   int32 [batch, max_blocks], rows table_stride elements apart; entries outside [0, num_blocks) name no block

@@ -29,7 +29,7 @@
 // values' own type: 2^-8 of each in bf16, 2^-11 in fp16, which is what the values themselves carry, and l sums them unrounded.
 // Against probabilities kept in float32 the outputs' error grows from 0.0017 to 0.0018 of their norm for 37 bf16 positions, and by
 // less over more of them; the rounding of out to its own type makes the rest.  Products with value scales, on int8 caches, whose
-// values are exact, keep two bf16 terms, 2^-16; int4 caches as int8 ones, or as Decode4 says.
+// values are exact, keep two bf16 terms, 2^-16; int4 caches as int8 ones.
 //
 // Work is dealt out on the device, because the lengths are known only there: the positions of every (sequence, head) pair
 // are cut into halves of a tile, 16 positions of one block (fewer at a block's end), eight halves make a unit, and a pair
@@ -724,9 +724,9 @@ struct Decode {
 // block.  A row is 72 bytes of memory for as much arithmetic as one of 256 in 16 bits, so it is instructions that Decode runs short
 // of, not memory or matrix cycles, and this is about their number:
 //   the bias of the key images is what the first MFMA's sum starts from; that of the value images is taken off at the end, with the
-//   sum of the rounded products P_j scale_j that one more MFMA keeps, so it cancels exactly and one bf16 term is enough: 2^-8 of the
-//   codes' part of a value, which is what 16-bit outputs carry (against 64 bits, outputs are off by 0.0023 of their norm for 37 positions
-//   and by 0.0017 over thousands; with two terms by 0.0017 and 0.0016, and 64 sequences of up to 8192 take 64.5 us, not 61.2).  float16 has two
+//   sum of the rounded products P_j scale_j that two more MFMAs keep, so it cancels exactly, and the two bf16 terms, 2^-16 of P_j scale_j,
+//   count for the code alone.  (With one term, 2^-8, 64 sequences of up to 8192 took 60.3 us, not 62.2, but an output whose code and offset
+//   cancel was off by up to 2^-5 of the scale, and over 37 positions outputs by 0.0023 of their norm, not by the 0.0017 of their own rounding)
 //   exponents are taken from a number m that is raised only where a score is more than kSlack above it, so the look at all lanes
 //   of a head is left out as a rule; sums stay below 2^kSlack of what they would be, far from the end of float32
 //   scales and offsets come one position to a lane and are handed round through LDS: one load where Decode has four
@@ -743,7 +743,6 @@ enum Kind { kAlone, kTogether, kAny };
 template <int DP, int QT, Kind KIND>
 struct Decode4 {
     static constexpr int NCH = DP / 32, KL = NCH / 2, PE = DP >= 128 ? 8 : 4, NP = DP / (16 * PE);
-    static constexpr int TERMS = QT == 1 ? 2 : 1;
     static constexpr float kShift = 0.0f, kSlack = 8.0f, kNone = -3.402823466e38f;
     static constexpr int HS = kStep / 4;                         // halves of a step of a wavefront: a tile
     static constexpr int kOnce = KIND == kAlone && DP < 256 ? 2 : 0;             // cache-policy bit: not temporal
@@ -1006,7 +1005,7 @@ struct Decode4 {
         }
     }
     // probabilities times value scales
-    __device__ __forceinline__ void add(bool whole, uint32_t valid, const f32x4 (&z)[HS], u32x4 (&terms)[TERMS])
+    __device__ __forceinline__ void add(bool whole, uint32_t valid, const f32x4 (&z)[HS], u32x4 (&terms)[2])
     {
         constexpr int N = HS * 4;
         float e[N];
@@ -1073,14 +1072,14 @@ struct Decode4 {
             for (int i = 0; i < 2; i++) {
                 const int to = s * 2 + i;
                 terms[0][to] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
-                if constexpr (TERMS > 1) terms[1][to] = pack_bf16x2(p[2 * i] - bf16_lo(terms[0][to]), p[2 * i + 1] - bf16_hi(terms[0][to]));
+                terms[1][to] = pack_bf16x2(p[2 * i] - bf16_lo(terms[0][to]), p[2 * i + 1] - bf16_hi(terms[0][to]));
             }
         }
     }
-    __device__ __forceinline__ void weigh(const u32x4 (&terms)[TERMS])
+    __device__ __forceinline__ void weigh(const u32x4 (&terms)[2])
     {
 #pragma unroll
-        for (int n = 0; n < TERMS; n++) bias = mfma_act<0>(u32x4{kOnes2<0>, kOnes2<0>, kOnes2<0>, kOnes2<0>}, terms[n], bias);
+        for (int n = 0; n < 2; n++) bias = mfma_act<0>(u32x4{kOnes2<0>, kOnes2<0>, kOnes2<0>, kOnes2<0>}, terms[n], bias);
 #pragma unroll
         for (int h = 0; h < NP; h++) {
             uint32_t pairs[4][2];                                // the low and the high halves of the words of two positions
@@ -1095,7 +1094,7 @@ struct Decode4 {
                 const u32x4 image = {image4<0>(pairs[0][i / 4], i % 4), image4<0>(pairs[1][i / 4], i % 4), image4<0>(pairs[2][i / 4], i % 4),
                                      image4<0>(pairs[3][i / 4], i % 4)};
 #pragma unroll
-                for (int n = 0; n < TERMS; n++) acc[h][i] = mfma_act<0>(image, terms[n], acc[h][i]);
+                for (int n = 0; n < 2; n++) acc[h][i] = mfma_act<0>(image, terms[n], acc[h][i]);
             }
         }
     }
@@ -1152,7 +1151,7 @@ struct Decode4 {
             load_keys(next);
             load_params(next);
             __builtin_amdgcn_sched_barrier(0);
-            u32x4 terms[TERMS];
+            u32x4 terms[2];
             add(whole, valid, z, terms);
             weigh(terms);
             __builtin_amdgcn_wave_barrier();
