@@ -426,6 +426,7 @@ int mi355_probe_empty_launch(int workgroups, void *stream);
  *   s = x1 + x2     rstd = 1 / sqrt(sum s^2 / cols + epsilon)     y = (s * rstd) * gamma     x = s
  *   gamma  [cols] of dtype or float32 (gamma_dtype)      y  [rows, cols] of dtype, contiguous
  *   rstd   float32 [rows] or NULL                        x  [rows, cols] of dtype, contiguous; with x2, else NULL
+ * A row's results depend on nothing else in the call, to the last bit (here and in the int8 form).
  */
 int mi355_add_rms_norm(const void *x1, const void *x2, int dtype, const void *gamma, int gamma_dtype, void *y, float *rstd, void *x,
                        int64_t rows, int64_t cols, int64_t x1_stride, int64_t x2_stride, float epsilon, void *stream);
