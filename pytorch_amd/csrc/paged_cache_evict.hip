@@ -61,8 +61,9 @@ __device__ __forceinline__ uint32_t scan_threads(uint32_t v, uint32_t *lds, uint
 }
 
 // Moves rows of keys and values (and their scales and offsets) within one (sequence, head), W bytes per access: pieces first,
-// first + step, ... of all of them.  per_row = pieces of a row of keys, then of the row of values.
-template <int W>
+// first + step, ... of all of them.  per_row = pieces of a row of keys, then of the row of values.  BITS: of the cache's elements
+// (looked up while it runs, what a row carries cost every eviction 0.3 to 0.4 us, and 6 of a hundred where 64 heads move 15000 rows each).
+template <int W, int BITS>
 __device__ __forceinline__ void move_pieces(const EvictArgs &a, int row, uint32_t count, uint32_t first, uint32_t step, const FastDiv &per_row)
 {
     typedef uint32_t word __attribute__((ext_vector_type(W >= 4 ? W / 4 : 1)));
@@ -86,13 +87,13 @@ __device__ __forceinline__ void move_pieces(const EvictArgs &a, int row, uint32_
         if constexpr (W >= 4) *reinterpret_cast<word *>(d) = *reinterpret_cast<const word *>(s);
         else if constexpr (W == 2) *reinterpret_cast<uint16_t *>(d) = *reinterpret_cast<const uint16_t *>(s);
         else *d = *s;
-        if (at == 0 && a.cache.key_scale.base) {
+        if (BITS < 16 && at == 0) {
             const auto move = [&](const PagedArray &one) {
                 *reinterpret_cast<float *>(one.base + a.cache.offset(one, dst_slot, head)) =
                     *reinterpret_cast<const float *>(one.base + a.cache.offset(one, src_slot, head));
             };
             move(value ? a.cache.value_scale : a.cache.key_scale);
-            if (a.cache.key_offset.base) move(value ? a.cache.value_offset : a.cache.key_offset);
+            if constexpr (BITS == 4) move(value ? a.cache.value_offset : a.cache.key_offset);
         }
     }
 }
@@ -100,7 +101,7 @@ __device__ __forceinline__ void move_pieces(const EvictArgs &a, int row, uint32_
 // KPT: rounds of 1024 places whose keys are held, KPT * 1024 >= capacity; 0: any number, read again for every digit (64 rows of
 // 16000 places halved: 52 us held, 82 read again; of 32000, held in part in scratch, 114 and 157).
 // W: bytes per access of the moves that this kernel makes itself; 0: it leaves them to paged_move_kernel.
-template <int KPT, int W>
+template <int KPT, int W, int BITS>
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs a, FastDiv per_row)
 {
     // places per scan of the counts below: 64 rounds with one count per thread
@@ -256,42 +257,54 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(EvictArgs 
         new_sums[place] = sums[src];
         new_pos[place] = pos[src];
     }
-    if constexpr (W > 0) move_pieces<W>(a, row, holes, tid, kSelectThreads, per_row);
+    if constexpr (W > 0) move_pieces<W, BITS>(a, row, holes, tid, kSelectThreads, per_row);
     else if (tid == 0) a.count[row] = (int32_t)holes;
 }
 
-template <int W>
+template <int W, int BITS>
 __global__ __launch_bounds__(256) void paged_move_kernel(EvictArgs a, FastDiv per_row)
 {
-    move_pieces<W>(a, blockIdx.y, (uint32_t)a.count[blockIdx.y], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, per_row);
+    move_pieces<W, BITS>(a, blockIdx.y, (uint32_t)a.count[blockIdx.y], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, per_row);
 }
 
 // A workgroup that chooses moves its rows itself where there can be few: up to this many bytes of keys.  (128 heads, rows of 256
 // bytes, 16 moves 9.7 us against 11.9 with a second launch, 64 moves 11.7 and 13.3, 256 moves 17.4 and 17.6; 512 heads, 64 moves
 // 22.5 and 22.9, 128 moves 33.7 and 31.5.)
 constexpr int64_t kMovedBySelect = 16384;
+template <int BITS>
+constexpr int kNarrow = BITS == 4 ? 4 : BITS / 8;
 
-template <int KPT>
-void launch_select(const EvictArgs &a, unsigned rows, int width, const FastDiv &per_row, hipStream_t s)
+// `wide`: rows in pieces of 16 bytes, else element by element (4 bits: word by word)
+template <int KPT, int BITS>
+void launch_select(const EvictArgs &a, unsigned rows, bool here, bool wide, const FastDiv &per_row, hipStream_t s)
 {
     const dim3 grid(rows), block(kSelectThreads);
-    if (width == 16) hipLaunchKernelGGL((paged_select_kernel<KPT, 16>), grid, block, 0, s, a, per_row);
-    else if (width == 4) hipLaunchKernelGGL((paged_select_kernel<KPT, 4>), grid, block, 0, s, a, per_row);
-    else if (width == 2) hipLaunchKernelGGL((paged_select_kernel<KPT, 2>), grid, block, 0, s, a, per_row);
-    else if (width == 1) hipLaunchKernelGGL((paged_select_kernel<KPT, 1>), grid, block, 0, s, a, per_row);
-    else hipLaunchKernelGGL((paged_select_kernel<KPT, 0>), grid, block, 0, s, a, per_row);
+    if (!here) hipLaunchKernelGGL((paged_select_kernel<KPT, 0, 16>), grid, block, 0, s, a, per_row);
+    else if (wide) hipLaunchKernelGGL((paged_select_kernel<KPT, 16, BITS>), grid, block, 0, s, a, per_row);
+    else hipLaunchKernelGGL((paged_select_kernel<KPT, kNarrow<BITS>, BITS>), grid, block, 0, s, a, per_row);
 }
 // Rounds in steps of 2^k + 1: budgets are powers of two as a rule, and a cache that is kept at one has a block or two more.  A
 // round too many costs 0.2 to 0.6 us (one token over 8192: 11.9 us in 9 rounds, 15.1 in 16, 24 where nothing is held).
-void launch_select(const EvictArgs &a, unsigned rows, int width, const FastDiv &per_row, hipStream_t s)
+template <int BITS>
+void launch_select(const EvictArgs &a, unsigned rows, bool here, bool wide, const FastDiv &per_row, hipStream_t s)
 {
-    if (a.capacity <= 2 * kSelectThreads) launch_select<2>(a, rows, width, per_row, s);
-    else if (a.capacity <= 3 * kSelectThreads) launch_select<3>(a, rows, width, per_row, s);
-    else if (a.capacity <= 5 * kSelectThreads) launch_select<5>(a, rows, width, per_row, s);
-    else if (a.capacity <= 9 * kSelectThreads) launch_select<9>(a, rows, width, per_row, s);
-    else if (a.capacity <= 17 * kSelectThreads) launch_select<17>(a, rows, width, per_row, s);
-    else if (a.capacity <= 33 * kSelectThreads) launch_select<33>(a, rows, width, per_row, s);
-    else launch_select<0>(a, rows, width, per_row, s);
+    if (a.capacity <= 2 * kSelectThreads) launch_select<2, BITS>(a, rows, here, wide, per_row, s);
+    else if (a.capacity <= 3 * kSelectThreads) launch_select<3, BITS>(a, rows, here, wide, per_row, s);
+    else if (a.capacity <= 5 * kSelectThreads) launch_select<5, BITS>(a, rows, here, wide, per_row, s);
+    else if (a.capacity <= 9 * kSelectThreads) launch_select<9, BITS>(a, rows, here, wide, per_row, s);
+    else if (a.capacity <= 17 * kSelectThreads) launch_select<17, BITS>(a, rows, here, wide, per_row, s);
+    else if (a.capacity <= 33 * kSelectThreads) launch_select<33, BITS>(a, rows, here, wide, per_row, s);
+    else launch_select<0, BITS>(a, rows, here, wide, per_row, s);
+}
+template <int BITS>
+void launch_evict(const EvictArgs &a, unsigned rows, bool here, bool wide, const FastDiv &per_row, hipStream_t s)
+{
+    launch_select<BITS>(a, rows, here, wide, per_row, s);
+    if (here) return;
+    const int64_t chunks = (a.most * per_row.d + 255) / 256;
+    const dim3 grid((unsigned)(chunks < 64 ? chunks : 64), rows);
+    if (wide) hipLaunchKernelGGL((paged_move_kernel<16, BITS>), grid, dim3(256), 0, s, a, per_row);
+    else hipLaunchKernelGGL((paged_move_kernel<kNarrow<BITS>, BITS>), grid, dim3(256), 0, s, a, per_row);
 }
 
 // moves of one row at most
@@ -346,7 +359,7 @@ extern "C" int mi355_paged_cache_evict(const mi355_paged_cache *cache, const int
     a.count = static_cast<int32_t *>(workspace);
     a.moves = reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + (rows * 4 + 255) / 256 * 256);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int elem = cache_elem_bytes(cache->dtype), bytes = (int)(cache->head_dim * cache_bits(cache->dtype) / 8);
+    const int bits = cache_bits(cache->dtype), elem = cache_elem_bytes(cache->dtype), bytes = (int)(cache->head_dim * bits / 8);
     const bool wide = bytes % 16 == 0 && rows_aligned(a.cache.key, 16) && rows_aligned(a.cache.value, 16);
     const FastDiv per_row = fast_div((uint32_t)(bytes / (wide ? 16 : elem)) * 2);
     const bool here = a.most * bytes <= kMovedBySelect;
@@ -365,14 +378,9 @@ extern "C" int mi355_paged_cache_evict(const mi355_paged_cache *cache, const int
         c.new_positions += r0 * capacity;
         c.count += r0;
         c.moves += r0 * 2 * a.most;
-        launch_select(c, (unsigned)n, here ? (wide ? 16 : elem) : 0, per_row, s);
-        if (here) continue;
-        const int64_t chunks = (a.most * per_row.d + 255) / 256;
-        const dim3 grid((unsigned)(chunks < 64 ? chunks : 64), (unsigned)n);
-        if (wide) hipLaunchKernelGGL(paged_move_kernel<16>, grid, dim3(256), 0, s, c, per_row);
-        else if (elem == 4) hipLaunchKernelGGL(paged_move_kernel<4>, grid, dim3(256), 0, s, c, per_row);
-        else if (elem == 2) hipLaunchKernelGGL(paged_move_kernel<2>, grid, dim3(256), 0, s, c, per_row);
-        else hipLaunchKernelGGL(paged_move_kernel<1>, grid, dim3(256), 0, s, c, per_row);
+        if (bits == 16) launch_evict<16>(c, (unsigned)n, here, wide, per_row, s);
+        else if (bits == 8) launch_evict<8>(c, (unsigned)n, here, wide, per_row, s);
+        else launch_evict<4>(c, (unsigned)n, here, wide, per_row, s);
     }
     return check_launch();
 }
