@@ -41,7 +41,7 @@
 // do not depend on it: the launch, two trips to memory for lengths and blocks, the first rows, and at the end the four
 // wavefronts' sums, their trip through the workspace and the addition.  With 32 query heads on 8 heads of 128: 32 sequences of up to 4095 tokens
 // (280 MB) 62 us, one of 131071 (537 MB) 104 us, int8, 64 of up to 8192 (563 MB) 120 us, one of 37 6.5 us.  int4: 32 of up to 4095 (78 MB)
-// 26.1 us, 64 of up to 8192 (308 MB) 61.3 us, one of 131071 (151 MB) 39.1 us, one of 37 6.9 us.
+// 25.7 us, 64 of up to 8192 (308 MB) 62 to 65 us, one of 131071 (151 MB) 40 us, one of 37 7.2 us; 64 of up to 8192 with attn_sums 92.6 us.
 #include "paged_cache.h"
 #include "weight_quant_common.h"
 
@@ -62,10 +62,11 @@ constexpr int kSC1 = 16;                     // cache-policy bit: agent scope, p
 // 4095, 280 MB: 62 us for 768 pieces, 66 for 512, 64 for 1024, 68 for 1536).  Heads of up to 64 take 103 to 124 registers, of
 // which four would fit; they are cut for three like the others.
 constexpr int resident(int dp, bool quant) { return dp < 256 ? 3 : quant ? 2 : 1; }
-// int4, Decode4: halves of a step of a workgroup; its workgroups of a compute unit (135 to 138 registers for heads of 65 to 128, 205 to 211 for
-// wider ones); what the start and the end of a range cost, in halves (dense, 32 sequences of up to 4095, 78 MB: 25.7 us with 24, 26.2 with 16 or
-// 30, 27.8 with 8, 26.7 with 40, 30.0 with 64; 64 of up to 8192, 308 MB: 60.4 to 61.3, with 8 and 64 63); and the addition of a sequence's
-// pieces (a step is 1.5 us where work is short, the addition 2.8; 128 of 300 with 16, whole in two rounds, 21.8 us, with 8, dense, 26.8)
+// int4, Decode4: halves of a step of a workgroup; its workgroups of a compute unit (119 or 120 registers for heads of up to 64, 137 to 143
+// of 65 to 128, 207 to 209 for wider ones); what the start and the end of a range cost, in halves (dense, 32 sequences of up to 4095, 78 MB: 25.7
+// us with 24, 27.2 with 16, 26.4 with 30, 28.8 with 8, 27.1 with 40, 27.2 with 64; 64 of up to 8192, 308 MB: 64 to 65, with 8 71, with 40 and 64 67); and
+// the addition of a sequence's pieces (a step is 1.5 us where work is short, the addition 2.8; 128 of 300 with 16, whole in two rounds, 22.1 us,
+// with 8, dense, 27.1)
 constexpr int kStep = 8;
 constexpr int resident4(int dp) { return dp < 256 ? 3 : 2; }
 constexpr uint32_t kStart = 24, kCut = 16;
@@ -725,20 +726,20 @@ struct Decode {
 // of, not memory or matrix cycles, and this is about their number:
 //   the bias of the key images is what the first MFMA's sum starts from; that of the value images is taken off at the end, with the
 //   sum of the rounded products P_j scale_j that two more MFMAs keep, so it cancels exactly, and the two bf16 terms, 2^-16 of P_j scale_j,
-//   count for the code alone.  (With one term, 2^-8, 64 sequences of up to 8192 took 60.3 us, not 62.2, but an output whose code and offset
-//   cancel was off by up to 2^-5 of the scale, and over 37 positions outputs by 0.0023 of their norm, not by the 0.0017 of their own rounding)
+//   count for the code alone.  (With one term, 2^-8, 64 sequences of up to 8192 take 60 to 63 us, not 62 to 65, but an output whose code and offset
+//   cancel is off by up to 2^-5 of the scale, and over 37 positions outputs by 0.0023 of their norm, not by the 0.0017 of their own rounding)
 //   exponents are taken from a number m that is raised only where a score is more than kSlack above it, so the look at all lanes
 //   of a head is left out as a rule; sums stay below 2^kSlack of what they would be, far from the end of float32
 //   scales and offsets come one position to a lane and are handed round through LDS: one load where Decode has four
-// Against Decode, 8 heads of 128: 32 sequences of up to 4095 26.1 and 33.9 us, 64 of up to 8192 61.3 and 91.9, one of 131071 39.1 and 45.8,
-// one of 37 6.9 and 6.7; 64 of up to 8192, heads of 64 50 and 64, of 80 62 and 94; 32 of them, of 256 65 and 92.
+// Against Decode, 8 heads of 128: 32 sequences of up to 4095 25.7 and 34.0 us, 64 of up to 8192 65 and 92, one of 131071 40.1 and 45.8,
+// one of 37 7.3 and 7.0; 64 of up to 8192, heads of 64 51 and 61, of 80 65 and 95; 32 of them, of 256 66 and 89.
 //   kTogether  a token's heads share cache lines, and other workgroups want what this one leaves
-//   kAlone     heads have lines of their own, which nobody else wants, and requests are marked so (64 of up to 8192: 61.2 us, 66.5 unmarked; heads
-//              of 64 48.6 and 49.6, of 80 62 and 65; one of 131071 39.8 and 42) - but rows of 65 bytes and more come in two requests for the
-//              same line, which the mark makes two trips (heads of 256: 68 us and 66; 32 of up to 4095, token by token, 50 and 44)
+//   kAlone     heads have lines of their own, which nobody else wants, and requests are marked so (64 of up to 8192: 66.1 us, 71.8 unmarked; heads
+//              of 64 51.0 and 52.0, of 80 65.1 and 67.5; one of 131071 39.5 and 42.3) - but rows of 65 bytes and more come in two requests for the
+//              same line, which the mark makes two trips (heads of 256: 66.9 us marked and 65.7; 32 of up to 4095, token by token, 49 and 41)
 //   kAny       a mask, blocks of other than a multiple of 16 tokens, scales and offsets that do not lie token by token.  What that takes would cost the
-//              others 2 to 3 of a hundred.  Masked, 64 of up to 8192 80 us, 104 with Decode, 32 of up to 4095 30 and 36, 8 of up to 500 11.6 and 11;
-//              blocks of 24, 32 of up to 4095 32 and 41, 4 of 1000 13.5 and 12.7
+//              others 3 to 10 of a hundred.  Masked, 64 of up to 8192 81 us, 95 with Decode, 32 of up to 4095 29.5 and 34.8, 8 of up to 500 11.2 and
+//              10.5; blocks of 24, 32 of up to 4095 33 and 40, 4 of 1000 12.8 and 12.3
 enum Kind { kAlone, kTogether, kAny };
 template <int DP, int QT, Kind KIND>
 struct Decode4 {
@@ -1099,8 +1100,8 @@ struct Decode4 {
         }
     }
 
-    // Wavefronts that have come less far go first: those of a compute unit then end together (64 sequences of up to 8192: 61.2 us, 62.7
-    // without; 32 of up to 4095 26.6 and 27.5).
+    // Wavefronts that have come less far go first: those of a compute unit then end together (64 sequences of up to 8192: 65.1 us, 68.6
+    // without; 32 of up to 4095 25.7 and 27.0).
     __device__ static __forceinline__ void set_priority(int quarters)
     {
         if (quarters == 3) __builtin_amdgcn_s_setprio(3);
@@ -1518,9 +1519,9 @@ __device__ __forceinline__ void decode_pieces()
 //   whole   every sequence a range of its own, in rounds if there are more than `ranges`
 //   cut     every sequence into pieces of its own of `share` halves, no longer than the average range, at most `ranges` in all
 //   dense   kStart and the halves of a sequence behind those of the one before, so that a range may end one and begin the next
-// What is short takes as long as its longest piece: 64 sequences of up to 100, 8 heads of 128, 9.4 us, 16 dense, 8 of up to 600 12.3 and 15, one of
-// 1200 11.2 and 15.  What is long and cut evenly leaves the last pieces to run alone: 32 of up to 4095 26.3 us dense, 27.3 in pieces of its
-// sequences in one round, 33.9 in Pieces, which are more than fit at once.
+// What is short takes as long as its longest piece: 64 sequences of up to 100, 8 heads of 128, 9.0 us, 17.1 dense, 8 of up to 600 10.7 and 12.3, one of
+// 1200 10.6 and 12.0.  What is long and cut evenly leaves the last pieces to run alone: 32 of up to 4095, with one bf16 term for the weights, 26.3 us
+// dense, 27.3 in pieces of its sequences in one round, 33.9 in Pieces, which are more than fit at once.
 struct Ranges {
     uint32_t share, count, before, mine, total;      // halves of a range; ranges at most; halves in the runs before this lane's, in it, in all
     int run, len;                            // sequences per lane; the length of the first
@@ -1552,7 +1553,7 @@ struct Ranges {
             const uint32_t all = over_lanes(halves, Add()), tallest = over_lanes(longest, Max());
             const uint32_t average = max(divide(all + sequences * kStart + ranges - 1, a->by_ranges), (uint32_t)kStep);
             // pieces of u units, no longer than the average range, or, where that is short, taking no more steps (4 sequences of 4000, 8 heads:
-            // 15.1 us and 16.8)
+            // 15.7 us, 17.2 dense)
             uint32_t u = average <= 2 * kStep ? units_in(average) : average / kStep;
             bool cut = false;
             if (run == 1) {
@@ -1666,7 +1667,7 @@ __global__ __launch_bounds__(256, resident4(DP)) void paged_decode4_kernel(AttnA
                         for (int i = 0; i < W::PE; i++) acc[h][i] = w.acc[h][i];
                 }
                 // Dense: a range has a piece that goes on in the next one, and one that came from the range before and ends here, at most.
-                // Pair by pair, so that the arrivals of different pairs count in cache lines of their own (one sequence of 9353, 32 heads: 19 us,
+                // Pair by pair, so that the arrivals of different pairs count in cache lines of their own (one sequence of 9353, 32 heads: 20 us,
                 // 29 with the pairs' counters side by side; one of 131071, 8 heads: 38.9 and 40.2)
                 const uint32_t places = pair * args_now()->ranges * 2 + first_range * 2;
                 const auto place = [&](int i) { return places + (uint32_t)(i * 2 + (i < n - 1 ? 1 : 0)); };
